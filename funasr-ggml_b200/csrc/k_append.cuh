@@ -45,6 +45,30 @@ __device__ __forceinline__ HeadRowMeta qkv_head_meta(const AppendArgs& a, int m,
     return h;
 }
 
+// RMSNorm and rotation of one head vector in a warp: x holds the lane's dims l, l+32, l+64,
+// l+96, w their norm weights, rot the rotations (cos, sin) of the pairs (l, l+64) and
+// (l+32, l+96).
+__device__ __forceinline__ void head_norm_rope(const float (&w)[4], const float2 (&rot)[2], float eps, float (&x)[4]) {
+    constexpr int D = 128;
+    double ss = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) ss += (double)__fmul_rn(x[k], x[k]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float mean = (float)(ss * (1.0 / D));      // D = 128: exactly ss / D
+    const float scale = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, eps)));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = __fmul_rn(__fmul_rn(x[k], scale), w[k]);
+    // pair (x[0], x[2]) uses rotation index lane, pair (x[1], x[3]) index lane + 32
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float2 r = rot[k];
+        const float x0 = x[k], x1 = x[k + 2];
+        x[k] = __fsub_rn(__fmul_rn(x0, r.x), __fmul_rn(x1, r.y));
+        x[k + 2] = __fadd_rn(__fmul_rn(x0, r.y), __fmul_rn(x1, r.x));
+    }
+}
+
 // q_dst (optional): where a q head goes instead of a.q_out (128 floats, any address space);
 // kv_dst (optional): a second copy of a K / V head's 128 f16 values besides the page.
 __device__ __forceinline__ void qkv_head_apply(const AppendArgs& a, const HeadRowMeta& h, int m, int j, int lane,
@@ -59,32 +83,13 @@ __device__ __forceinline__ void qkv_head_apply(const AppendArgs& a, const HeadRo
     }
 
     if (is_q || is_k) {
-        double ss = 0.0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) ss += (double)__fmul_rn(x[k], x[k]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float mean = (float)(ss * (1.0 / D));      // D = 128: exactly ss / D
-        const float scale = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, a.eps)));
-        float y[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = __fmul_rn(__fmul_rn(x[k], scale), h.w[k]);
-        // pair (y[0], y[2]) uses rotation index lane, pair (y[1], y[3]) index lane + 32
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const float2 r = h.rot[k];
-            const float x0 = y[k], x1 = y[k + 2];
-            y[k] = __fsub_rn(__fmul_rn(x0, r.x), __fmul_rn(x1, r.y));
-            y[k + 2] = __fadd_rn(__fmul_rn(x0, r.y), __fmul_rn(x1, r.x));
-        }
+        head_norm_rope(h.w, h.rot, a.eps, x);
         if (is_q) {
             float* dst = q_dst ? q_dst : a.q_out + ((size_t)m * a.Hq + j) * D;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) dst[lane + 32 * k] = __fmul_rn(y[k], a.q_scale);
+            for (int k = 0; k < 4; ++k) dst[lane + 32 * k] = __fmul_rn(x[k], a.q_scale);
             return;
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = y[k];
     }
 
     // K (rotated) or V (as projected) into the page of this row's token.

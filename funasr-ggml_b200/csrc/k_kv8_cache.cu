@@ -1,0 +1,377 @@
+// Writing the 8-bit page pool (k_kv8.cuh) and reading it back: the raw append, kernel (1)
+// with an 8-bit end (per-head Q/K RMSNorm + NEOX RoPE + append), and the gather into
+// head-major slabs. The f16 pool's forms of the three are in k_append.cu.
+//
+// All three are bound by HBM: a vector costs 132 bytes in the pool against its 256 (f16) or
+// 512 (f32) outside.
+#include "k_append.cuh"
+#include "k_kv8.cuh"
+#include "funasr_dec.h"
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+namespace fa {
+
+int report_op_error(int code, const char* msg);   // fa_api.cu
+
+namespace {
+
+using namespace kv8;
+
+// Where a row's token goes: its page, or -1 (padding, or an error that is flagged once).
+__device__ __forceinline__ int token_page(const int* bt, int bt_stride, int n_pages, int slot, int pos, int* err,
+                                          bool flag) {
+    if (pos == -1) return -1;
+    if (pos < 0 || pos / kPageTokens >= bt_stride || slot < 0) {
+        if (flag) record_error(err, kDevErrBadPos);
+        return -1;
+    }
+    const int page = bt[(size_t)slot * bt_stride + pos / kPageTokens];
+    if (page < 0 || page >= n_pages) {
+        if (flag) record_error(err, kDevErrBadPage);
+        return -1;
+    }
+    return page;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<__half>(const __half* p, float (&x)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = h2_to_f2(w[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+template <>
+__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
+struct Kv8AppendArgs {
+    const void* k;           // [M] rows of [n_layers][Hkv][128], row_stride elements apart
+    const void* v;
+    long long row_stride;
+    int M, n_layers, Hkv;
+    const int* pos;
+    const int* slot;
+    const int* block_table;
+    int bt_stride;
+    int n_pages;
+    unsigned char* pool;
+    int* err;
+};
+
+// Raw append: a warp per (row, layer, KV head), its half-warps the K and the V vector, a
+// lane 8 consecutive values.
+template <int FMT, typename T>
+__global__ void __launch_bounds__(256) kv8_append_kernel(Kv8AppendArgs a) {
+    const long long gw = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (gw >= (long long)a.M * a.n_layers * a.Hkv) return;
+    const int h = (int)(gw % a.Hkv);
+    const int l = (int)(gw / a.Hkv % a.n_layers);
+    const int m = (int)(gw / a.Hkv / a.n_layers);
+    const int pos = a.pos[m];
+    const int page = token_page(a.block_table, a.bt_stride, a.n_pages, a.slot[m], pos, a.err, lane == 0);
+    if (page < 0) return;
+    const int part = lane >> 4, c = lane & 15;
+    float x[8];
+    load8(reinterpret_cast<const T*>(part ? a.v : a.k) + (size_t)m * a.row_stride + ((size_t)l * a.Hkv + h) * D + 8 * c,
+          x);
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float d = scale_of<FMT>(amax);
+    uint2 q = make_uint2(0, 0);
+    if (amax < 0x7f800000u) {
+        const float inv = __frcp_rn(d);
+        q = make_uint2(pack4<FMT>(x, d, inv), pack4<FMT>(x + 4, d, inv));
+    }
+    unsigned char* tile = a.pool + (((size_t)l * a.n_pages + page) * a.Hkv + h) * kTileBytes;
+    const int t = pos % kPageTokens;
+    *reinterpret_cast<uint2*>(tile + part * kPartBytes + t * D + 8 * c) = q;
+    if (c == 0) reinterpret_cast<float*>(tile + kScaleOff)[part * kPageTokens + t] = d;
+}
+
+struct Kv8QkvArgs {
+    const float* qkv;        // [M][(Hq + 2 Hkv) * 128]
+    int M, Hq, Hkv;
+    const int* pos;
+    const int* slot;
+    const int* block_table;
+    int bt_stride;
+    int n_pages;
+    const float* qn_w;
+    const float* kn_w;
+    float eps, q_scale;
+    const float2* rope;      // [max_pos][64]
+    int max_pos;
+    unsigned char* pool;     // one layer
+    float* q_out;            // [M][Hq][128]
+    int* err;
+};
+
+// Kernel (1) with an 8-bit end: a warp per (row, head vector), lane l holding dims l, l+32,
+// l+64, l+96 (both rotation pairs of a lane stay in it).
+template <int FMT>
+__global__ void __launch_bounds__(256) kv8_qkv_kernel(Kv8QkvArgs a) {
+    const int m = blockIdx.x;
+    const int j = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (j >= a.Hq + 2 * a.Hkv) return;
+    const int pos = a.pos[m];
+    if (pos == -1) return;
+    if (pos < 0 || pos >= a.max_pos) {
+        if (lane == 0) record_error(a.err, kDevErrBadPos);
+        return;
+    }
+    const bool is_q = j < a.Hq, is_k = !is_q && j < a.Hq + a.Hkv;
+    float x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = a.qkv[((size_t)m * (a.Hq + 2 * a.Hkv) + j) * D + lane + 32 * k];
+    if (is_q || is_k) {
+        const float* w = is_q ? a.qn_w : a.kn_w;
+        const float wv[4] = {w[lane], w[lane + 32], w[lane + 64], w[lane + 96]};
+        const float2* cs = a.rope + (size_t)pos * (D / 2);
+        const float2 rot[2] = {cs[lane], cs[lane + 32]};
+        head_norm_rope(wv, rot, a.eps, x);
+    }
+    if (is_q) {
+        float* dst = a.q_out + ((size_t)m * a.Hq + j) * D;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) dst[lane + 32 * k] = __fmul_rn(x[k], a.q_scale);
+        return;
+    }
+    const int h = is_k ? j - a.Hq : j - a.Hq - a.Hkv, part = is_k ? 0 : 1;
+    const int page = token_page(a.block_table, a.bt_stride, a.n_pages, a.slot[m], pos, a.err, lane == 0);
+    if (page < 0) return;
+    uint32_t amax = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) amax = max(amax, __float_as_uint(x[k]) & 0x7fffffffu);
+    amax = __reduce_max_sync(0xffffffffu, amax);
+    const float d = scale_of<FMT>(amax);
+    const uint32_t q = amax < 0x7f800000u ? pack4<FMT>(x, d, __frcp_rn(d)) : 0u;
+    unsigned char* tile = a.pool + ((size_t)page * a.Hkv + h) * kTileBytes;
+    const int t = pos % kPageTokens;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) tile[part * kPartBytes + t * D + lane + 32 * k] = (unsigned char)(q >> (8 * k));
+    if (lane == 0) reinterpret_cast<float*>(tile + kScaleOff)[part * kPageTokens + t] = d;
+}
+
+struct Kv8GatherArgs {
+    const unsigned char* pool;
+    int n_layers, n_pages, Hkv;
+    const int* block_table;
+    int bt_stride;
+    const int* slot;
+    const int* t0;           // [M] or nullptr: 0
+    const int* n_tok;        // [M]
+    const int* row0;         // [M]
+    int M, max_tokens, total_rows;
+    void* k_out;             // [n_layers][Hkv][total_rows][128]
+    void* v_out;
+    int* err;
+};
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]);
+template <>
+__device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+template <>
+__device__ __forceinline__ void store8<__half>(__half* p, const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <>
+__device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Gather: one CTA per page of one sequence in one layer; a thread 8 values of one token,
+// over the heads' K and V parts. The value d * q is formed in f32 and rounded once to the
+// output type.
+template <int FMT, typename T>
+__global__ void __launch_bounds__(256) kv8_gather_kernel(Kv8GatherArgs a) {
+    const int m = blockIdx.y, l = blockIdx.z;
+    const int t0 = a.t0 ? a.t0[m] : 0, n = a.n_tok[m], row0 = a.row0[m], slot = a.slot[m];
+    if (n == 0) return;
+    if (n < 0 || n > a.max_tokens || t0 < 0 || (long long)t0 + n > (long long)a.bt_stride * kPageTokens || row0 < 0 ||
+        (long long)row0 + n > a.total_rows || slot < 0) {
+        if (blockIdx.x == 0 && l == 0 && threadIdx.x == 0) record_error(a.err, kDevErrBadLen);
+        return;
+    }
+    const int pi = t0 / kPageTokens + blockIdx.x;
+    if (pi * kPageTokens >= t0 + n) return;
+    const int page = a.block_table[(size_t)slot * a.bt_stride + pi];
+    if (page < 0 || page >= a.n_pages) {
+        if (threadIdx.x == 0) record_error(a.err, kDevErrBadPage);
+        return;
+    }
+    const int t = threadIdx.x >> 4, c = threadIdx.x & 15;
+    const int token = pi * kPageTokens + t;
+    if (token < t0 || token >= t0 + n) return;
+    const unsigned char* tiles = a.pool + ((size_t)l * a.n_pages + page) * a.Hkv * kTileBytes;
+    const size_t row = (size_t)row0 + (token - t0);
+#pragma unroll 4
+    for (int j = 0; j < 2 * a.Hkv; ++j) {
+        const int h = j >> 1, part = j & 1;
+        const unsigned char* tile = tiles + (size_t)h * kTileBytes;
+        const uint2 w = *reinterpret_cast<const uint2*>(tile + part * kPartBytes + t * D + 8 * c);
+        const float d = reinterpret_cast<const float*>(tile + kScaleOff)[part * kPageTokens + t];
+        __half2 v[4];
+        expand4<FMT>(w.x, v[0], v[1]);
+        expand4<FMT>(w.y, v[2], v[3]);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(v[i]);
+            x[2 * i] = f.x * d;
+            x[2 * i + 1] = f.y * d;
+        }
+        T* out = reinterpret_cast<T*>(part ? a.v_out : a.k_out);
+        store8(out + (((size_t)l * a.Hkv + h) * a.total_rows + row) * D + 8 * c, x);
+    }
+}
+
+bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
+int launched(const char* what) {
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) return FA_OK;
+    return report_op_error(FA_ERR_CUDA, (std::string(what) + ": " + cudaGetErrorString(e)).c_str());
+}
+
+template <int FMT>
+void append_by_type(const Kv8AppendArgs& a, int type, unsigned blocks, cudaStream_t s) {
+    if (type == FA_TYPE_F32) kv8_append_kernel<FMT, float><<<blocks, 256, 0, s>>>(a);
+    else if (type == FA_TYPE_F16) kv8_append_kernel<FMT, __half><<<blocks, 256, 0, s>>>(a);
+    else kv8_append_kernel<FMT, __nv_bfloat16><<<blocks, 256, 0, s>>>(a);
+}
+
+template <int FMT>
+void gather_by_type(const Kv8GatherArgs& a, int type, dim3 grid, cudaStream_t s) {
+    if (type == FA_TYPE_F32) kv8_gather_kernel<FMT, float><<<grid, 256, 0, s>>>(a);
+    else if (type == FA_TYPE_F16) kv8_gather_kernel<FMT, __half><<<grid, 256, 0, s>>>(a);
+    else kv8_gather_kernel<FMT, __nv_bfloat16><<<grid, 256, 0, s>>>(a);
+}
+
+bool known_type(int type) { return type == FA_TYPE_F32 || type == FA_TYPE_F16 || type == FA_TYPE_BF16; }
+bool known_format(int format) { return format == FA_KV8_INT8 || format == FA_KV8_E4M3; }
+
+}  // namespace
+}  // namespace fa
+
+extern "C" FA_API size_t fa_op_kv8_page_bytes(int n_kv_heads) {
+    return n_kv_heads > 0 ? (size_t)n_kv_heads * fa::kv8::kTileBytes : 0;
+}
+
+extern "C" FA_API int fa_op_kv8_append(const void* k, const void* v, int src_type, int64_t row_stride, int M,
+                                       int n_layers, int n_kv_heads, const int* pos, const int* slot, const int* bt,
+                                       int bt_stride, int n_pages, int format, void* pool, int* err, void* stream) {
+    using namespace fa;
+    if (!k || !v || !pos || !slot || !bt || !pool || M <= 0 || n_layers <= 0 || n_kv_heads <= 0 || bt_stride <= 0 ||
+        n_pages <= 0)
+        return report_op_error(FA_ERR_INVALID_ARG, "fa_op_kv8_append: null or non-positive argument");
+    if (!known_format(format) || !known_type(src_type))
+        return report_op_error(FA_ERR_INVALID_ARG, "fa_op_kv8_append: unknown format or source type");
+    const int per16 = src_type == FA_TYPE_F32 ? 4 : 8;
+    if (row_stride < (int64_t)n_layers * n_kv_heads * kv8::D || row_stride % per16)
+        return report_op_error(FA_ERR_INVALID_ARG,
+                               "fa_op_kv8_append: row_stride must cover a row and be a multiple of 16 bytes");
+    if (misaligned(k, 16) || misaligned(v, 16) || misaligned(pool, 128))
+        return report_op_error(FA_ERR_INVALID_ARG, "fa_op_kv8_append: k and v must be 16-byte, pool 128-byte aligned");
+    const long long blocks = ((long long)M * n_layers * n_kv_heads + 7) / 8;
+    if ((long long)n_layers * n_kv_heads > (1 << 20) || blocks > 0x7fffffffll)
+        return report_op_error(FA_ERR_CAPACITY, "fa_op_kv8_append: too many vectors for one call");
+    Kv8AppendArgs a{k, v, row_stride, M, n_layers, n_kv_heads, pos, slot, bt, bt_stride, n_pages,
+                    static_cast<unsigned char*>(pool), err};
+    if (format == FA_KV8_INT8) append_by_type<kv8::kInt8>(a, src_type, (unsigned)blocks, (cudaStream_t)stream);
+    else append_by_type<kv8::kE4m3>(a, src_type, (unsigned)blocks, (cudaStream_t)stream);
+    return launched("fa_op_kv8_append");
+}
+
+extern "C" FA_API int fa_op_qknorm_rope_append_kv8(const float* qkv, int M, int n_heads, int n_kv_heads,
+                                                   const int* pos, const int* slot, const int* bt, int bt_stride,
+                                                   int n_pages, const float* qn, const float* kn, float eps,
+                                                   const float* rope, int max_pos, int format, void* pool_layer,
+                                                   float* q_out, int* err, void* stream) {
+    using namespace fa;
+    if (!qkv || !pos || !slot || !bt || !qn || !kn || !rope || !pool_layer || !q_out || M <= 0 || n_heads <= 0 ||
+        n_kv_heads <= 0 || bt_stride <= 0 || n_pages <= 0 || max_pos <= 0)
+        return report_op_error(FA_ERR_INVALID_ARG, "fa_op_qknorm_rope_append_kv8: null or non-positive argument");
+    if (!known_format(format))
+        return report_op_error(FA_ERR_INVALID_ARG, "fa_op_qknorm_rope_append_kv8: unknown format");
+    if (misaligned(qkv, 16) || misaligned(q_out, 16) || misaligned(rope, 16) || misaligned(pool_layer, 128))
+        return report_op_error(FA_ERR_INVALID_ARG,
+                               "fa_op_qknorm_rope_append_kv8: qkv, rope and q_out must be 16-byte, pool 128-byte aligned");
+    if ((long long)n_heads + 2ll * n_kv_heads > 65535)
+        return report_op_error(FA_ERR_CAPACITY, "fa_op_qknorm_rope_append_kv8: too many heads");
+    Kv8QkvArgs a{qkv, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages, qn, kn, eps,
+                 1.0f / std::sqrt((float)kv8::D), reinterpret_cast<const float2*>(rope), max_pos,
+                 static_cast<unsigned char*>(pool_layer), q_out, err};
+    const dim3 grid(M, (n_heads + 2 * n_kv_heads + 7) / 8);
+    if (format == FA_KV8_INT8) kv8_qkv_kernel<kv8::kInt8><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
+    else kv8_qkv_kernel<kv8::kE4m3><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
+    return launched("fa_op_qknorm_rope_append_kv8");
+}
+
+extern "C" FA_API int fa_op_kv8_gather(const void* pool, int format, int n_layers, int n_pages, int n_kv_heads,
+                                       const int* bt, int bt_stride, const int* slot, const int* t0, const int* n_tok,
+                                       const int* row0, int M, int max_tokens, int total_rows, int out_type,
+                                       void* k_out, void* v_out, int* err, void* stream) {
+    using namespace fa;
+    if (!pool || !bt || !slot || !n_tok || !row0 || !k_out || !v_out || M <= 0 || n_layers <= 0 || n_pages <= 0 ||
+        n_kv_heads <= 0 || bt_stride <= 0 || max_tokens <= 0 || total_rows <= 0)
+        return report_op_error(FA_ERR_INVALID_ARG, "fa_op_kv8_gather: null or non-positive argument");
+    if (!known_format(format) || !known_type(out_type))
+        return report_op_error(FA_ERR_INVALID_ARG, "fa_op_kv8_gather: unknown format or output type");
+    if (M > 65535 || n_layers > 65535)
+        return report_op_error(FA_ERR_INVALID_ARG, "fa_op_kv8_gather: M and n_layers are limited to 65535");
+    if (misaligned(k_out, 16) || misaligned(v_out, 16) || misaligned(pool, 128))
+        return report_op_error(FA_ERR_INVALID_ARG, "fa_op_kv8_gather: outputs must be 16-byte, pool 128-byte aligned");
+    if ((long long)bt_stride * kPageTokens > 0x7fffffffll)
+        return report_op_error(FA_ERR_CAPACITY, "fa_op_kv8_gather: bt_stride * 16 must fit in 31 bits");
+    Kv8GatherArgs a{static_cast<const unsigned char*>(pool), n_layers, n_pages, n_kv_heads, bt, bt_stride, slot, t0,
+                    n_tok, row0, M, max_tokens, total_rows, k_out, v_out, err};
+    // a range that does not start on a page boundary spans one page more
+    const int pages = (int)std::min<long long>((max_tokens + 2ll * (kPageTokens - 1)) / kPageTokens, bt_stride);
+    const dim3 grid(pages, M, n_layers);
+    if (format == FA_KV8_INT8) gather_by_type<kv8::kInt8>(a, out_type, grid, (cudaStream_t)stream);
+    else gather_by_type<kv8::kE4m3>(a, out_type, grid, (cudaStream_t)stream);
+    return launched("fa_op_kv8_gather");
+}

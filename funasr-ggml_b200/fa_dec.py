@@ -33,6 +33,8 @@ FA_ERR_WEIGHTS = -7
 
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_BF16 = 0, 1, 8, 30
 PAGE_TOKENS = 16
+KV8_INT8, KV8_E4M3 = 0, 1
+KV8_TILE_BYTES = 4224
 
 
 class FaError(RuntimeError):
@@ -170,6 +172,17 @@ def lib():
         "fa_op_q8p_gemm": ([_P, _P, _I, _I, _P, _I, _I, _P, _I, _P], _I),
         "fa_op_q8p_gemm_argmax": ([_P, _P, _I, _I, _P, _I, _P, _P, _P, _I, _P], _I),
         "fa_op_q8p_gemm_swiglu": ([_P, _P, _I, _I, _P, _I, _P, _P, _P], _I),
+        "fa_op_kv8_page_bytes": ([_I], ctypes.c_size_t),
+        "fa_op_kv8_append": ([_P, _P, _I, ctypes.c_int64, _I, _I, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P], _I),
+        "fa_op_qknorm_rope_append_kv8": ([_P, _I, _I, _I, _P, _P, _P, _I, _I, _P, _P, ctypes.c_float, _P, _I, _I, _P,
+                                          _P, _P, _P], _I),
+        "fa_op_kv8_gather": ([_P, _I, _I, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P], _I),
+        "fa_op_attention_kv8_scratch_bytes": ([_I, _I, _I], ctypes.c_size_t),
+        "fa_op_paged_attention_kv8": ([_P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _P, _P, ctypes.c_size_t, _P, _P, _P,
+                                       _P, _P], _I),
+        "fa_op_prefill_attention_kv8_scratch_bytes": ([_I, _I, _I], ctypes.c_size_t),
+        "fa_op_prefill_attention_kv8": ([_P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _P, _P, _I, _P, ctypes.c_size_t, _P,
+                                         _P, _P, _P, _P], _I),
         "fa_palloc_create": ([_I], _P),
         "fa_palloc_destroy": ([_P], None),
         "fa_palloc_alloc": ([_P], _I),
@@ -565,6 +578,61 @@ def op_q8p_gemm_swiglu(a16, a16_lo, M, K, planes, N, h16, h_lo, stream=0):
 def op_q8p_gemm_argmax(a16, a16_lo, M, K, planes, N, scratch, nxt, logits=0, variant=0, stream=0):
     _check(lib().fa_op_q8p_gemm_argmax(a16, a16_lo or None, M, K, planes, N, scratch, nxt, logits or None, variant,
                                        stream or None))
+
+
+# ------------------------------------------------------- 8-bit page pool --
+def op_kv8_page_bytes(n_kv_heads) -> int:
+    """Bytes of one page of one layer: n_kv_heads tiles of K, V [16][128] and their scales."""
+    return int(lib().fa_op_kv8_page_bytes(n_kv_heads))
+
+
+def op_kv8_append(k, v, src_type, row_stride, M, n_layers, n_kv_heads, pos, slot, bt, bt_stride, n_pages, fmt, pool,
+                  err=0, stream=0):
+    """K / V rows of src_type (TYPE_F32, TYPE_F16, TYPE_BF16), row_stride elements apart,
+    quantised into the 8-bit pages of every layer."""
+    _check(lib().fa_op_kv8_append(k, v, src_type, row_stride, M, n_layers, n_kv_heads, pos, slot, bt, bt_stride,
+                                  n_pages, fmt, pool, err or None, stream or None))
+
+
+def op_qknorm_rope_append_kv8(qkv, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages, qn, kn, eps, rope,
+                              max_pos, fmt, pool, q_out, err=0, stream=0):
+    """Kernel (1) whose K / V go to the 8-bit pages of one layer."""
+    _check(lib().fa_op_qknorm_rope_append_kv8(qkv, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages, qn, kn,
+                                              eps, rope, max_pos, fmt, pool, q_out, err or None, stream or None))
+
+
+def op_kv8_gather(pool, fmt, n_layers, n_pages, n_kv_heads, bt, bt_stride, slot, t0, n_tok, row0, M, max_tokens,
+                  total_rows, out_type, k_out, v_out, err=0, stream=0):
+    """Tokens [t0[m], t0[m] + n_tok[m]) of sequences slot[m] read back into head-major slabs
+    [n_layers][n_kv_heads][total_rows][128] of out_type (t0 = 0: from the first token)."""
+    _check(lib().fa_op_kv8_gather(pool, fmt, n_layers, n_pages, n_kv_heads, bt, bt_stride, slot, t0 or None, n_tok,
+                                  row0, M, max_tokens, total_rows, out_type, k_out, v_out, err or None,
+                                  stream or None))
+
+
+def op_attention_kv8_scratch_bytes(M, n_heads, n_kv_heads) -> int:
+    return int(lib().fa_op_attention_kv8_scratch_bytes(M, n_heads, n_kv_heads))
+
+
+def op_paged_attention_kv8(q, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages, fmt, pool, scratch,
+                           scratch_bytes, out16=0, out32=0, err=0, stream=0, out16_lo=0):
+    """Decode attention over the 8-bit pages of one layer."""
+    _check(lib().fa_op_paged_attention_kv8(q, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages, fmt, pool,
+                                           scratch or None, scratch_bytes, out16 or None, out16_lo or None,
+                                           out32 or None, err or None, stream or None))
+
+
+def op_prefill_attention_kv8_scratch_bytes(n_tiles, n_heads, n_kv_heads) -> int:
+    return int(lib().fa_op_prefill_attention_kv8_scratch_bytes(n_tiles, n_heads, n_kv_heads))
+
+
+def op_prefill_attention_kv8(q, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages, fmt, pool, tiles, n_tiles,
+                             scratch, scratch_bytes, out16=0, out32=0, err=0, stream=0, out16_lo=0):
+    """Causal attention of prefill tiles (first row, rows <= 128 * n_kv_heads // n_heads) over
+    the 8-bit pages of one layer."""
+    _check(lib().fa_op_prefill_attention_kv8(q, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages, fmt, pool,
+                                             tiles, n_tiles, scratch or None, scratch_bytes, out16 or None,
+                                             out16_lo or None, out32 or None, err or None, stream or None))
 
 
 # ---------------------------------------------------------------- encoder --

@@ -384,6 +384,78 @@ FA_API int fa_op_q8p_gemm_argmax(const uint16_t* a16_dev, const uint16_t* a16_lo
                                  const void* planes_dev, int N, void* scratch_dev, int* next_dev, float* logits_dev,
                                  int variant, void* stream);
 
+/* ---- 8-bit page pool: kernel-level entry points (device pointers, caller's stream) ----
+ * The f16 pool's ops above over a pool of half the bytes. No counterpart in the reference
+ * (its cache is f32, compute/kv_cache.hpp:38-60). One page of one layer holds 16 tokens in
+ * n_kv_heads tiles of 4224 bytes:
+ *   [K 16 tokens x 128 values][V 16 x 128][K scales 16 x f32][V scales 16 x f32]
+ * so a layer's pool is [n_pages][n_kv_heads][4224] (fa_op_kv8_page_bytes per page), 128-byte
+ * aligned, with the f16 pool's block tables. A vector x (one token, one KV head, K or V) is
+ * stored as a scale d and 128 values x / d:
+ *   FA_KV8_INT8: d = max(amax / 127, 2^-126) rounded to f32; x / d rounded to the nearest
+ *     integer, ties to even (exactly: the bytes depend on x alone).
+ *   FA_KV8_E4M3: d = the smallest power of two >= 2^-126 with amax <= 448 d; x / d rounded to
+ *     e4m3, ties to even.
+ * A vector that holds a NaN or an infinity is stored as d = NaN and zeros and reads back as
+ * NaN. The bytes of a token do not depend on how tokens are cut into calls.
+ * n_heads is 1 to 8 times n_kv_heads (query head H uses KV head H * n_kv_heads / n_heads),
+ * head_dim 128. A row with pos -1 is padding (its slot is not looked at): it appends nothing,
+ * its q_out row is left as it was, and its attention output is zero. All of these calls can
+ * be captured into a CUDA graph; positions, lengths and block tables are read on the device
+ * when it runs. */
+#define FA_KV8_INT8 0
+#define FA_KV8_E4M3 1
+FA_API size_t fa_op_kv8_page_bytes(int n_kv_heads); /* one page of one layer; 0 for n_kv_heads <= 0 */
+/* Raw append (fa_op_kv_append's 8-bit form). k, v: M rows of [n_layers][n_kv_heads][128]
+ * values of src_type (FA_TYPE_F32, F16 or BF16), row_stride elements apart (so K and V may be
+ * slices of one projection), 16-byte aligned; pool [n_layers][n_pages][n_kv_heads][4224].
+ * Rows of one call go to distinct (slot, pos). A position below -1 or past the block-table row
+ * sets error bit 4 and a page outside the pool bit 2; such a row appends nothing. */
+FA_API int fa_op_kv8_append(const void* k_dev, const void* v_dev, int src_type, int64_t row_stride, int M,
+                            int n_layers, int n_kv_heads, const int* pos_dev, const int* slot_dev,
+                            const int* block_table_dev, int bt_stride, int n_pages, int format, void* pool_dev,
+                            int* err_dev, void* stream);
+/* Kernel (1) with an 8-bit end: fa_op_qknorm_rope_append with qkv [M][n_heads + 2 n_kv_heads][128],
+ * q_out [M][n_heads][128] (the same bits), K (normed and rotated) and V quantised from f32. */
+FA_API int fa_op_qknorm_rope_append_kv8(const float* qkv_dev, int M, int n_heads, int n_kv_heads, const int* pos_dev,
+                                        const int* slot_dev, const int* block_table_dev, int bt_stride, int n_pages,
+                                        const float* q_norm_dev, const float* k_norm_dev, float eps,
+                                        const float* rope_dev, int max_pos, int format, void* pool_layer_dev,
+                                        float* q_out_dev, int* err_dev, void* stream);
+/* Reading the pool back (fa_op_kv_gather's 8-bit form): tokens [t0[m], t0[m] + n_tok[m]) of
+ * sequence slot[m] (t0_dev NULL: from 0), in every layer, as d * q rounded once to out_type,
+ * into k_out / v_out [n_layers][n_kv_heads][total_rows][128] at rows [row0[m], row0[m] +
+ * n_tok[m]) of each head plane; other rows are left as they are. n_tok[m] is 0 to max_tokens.
+ * Bad lengths or row ranges set error bit 8, bad pages bit 2; those tokens are not written. */
+FA_API int fa_op_kv8_gather(const void* pool_dev, int format, int n_layers, int n_pages, int n_kv_heads,
+                            const int* block_table_dev, int bt_stride, const int* slot_dev, const int* t0_dev,
+                            const int* n_tok_dev, const int* row0_dev, int M, int max_tokens, int total_rows,
+                            int out_type, void* k_out_dev, void* v_out_dev, int* err_dev, void* stream);
+/* Decode attention (fa_op_paged_attention's 8-bit form): row m attends to tokens [0, pos[m]]
+ * of sequence slot[m]. q [M][n_heads][128] f32 (pre-scaled); output [M][n_heads * 128] as f32
+ * and / or as an f16 pair. Nothing is planned on the host: the work is split on the device by
+ * the rows' lengths. scratch_dev: fa_op_attention_kv8_scratch_bytes(...) bytes, 16-byte
+ * aligned, of any content; calls that overlap on the GPU (captured graphs that run at the same
+ * time among them) need scratch of their own. A position below -1 or past the block-table row
+ * sets error bit 8 and that row is not written; a page outside the pool sets bit 2 and its
+ * tokens are left out. */
+FA_API size_t fa_op_attention_kv8_scratch_bytes(int M, int n_heads, int n_kv_heads);
+FA_API int fa_op_paged_attention_kv8(const float* q_dev, int M, int n_heads, int n_kv_heads, const int* pos_dev,
+                                     const int* slot_dev, const int* block_table_dev, int bt_stride, int n_pages,
+                                     int format, const void* pool_layer_dev, void* scratch_dev, size_t scratch_bytes,
+                                     uint16_t* out16_dev, uint16_t* out16_lo_dev, float* out32_dev, int* err_dev,
+                                     void* stream);
+/* Causal attention of prefill tiles (fa_op_prefill_attention's 8-bit form). tiles_dev holds
+ * n_tiles pairs (first row, rows): up to 128 * n_kv_heads / n_heads (rounded down) consecutive
+ * rows of one sequence with non-decreasing positions; each row attends to tokens [0, pos[m]].
+ * A bad tile sets error bit 4 and writes nothing; rows, pages and scratch as above. */
+FA_API size_t fa_op_prefill_attention_kv8_scratch_bytes(int n_tiles, int n_heads, int n_kv_heads);
+FA_API int fa_op_prefill_attention_kv8(const float* q_dev, int M, int n_heads, int n_kv_heads, const int* pos_dev,
+                                       const int* slot_dev, const int* block_table_dev, int bt_stride, int n_pages,
+                                       int format, const void* pool_layer_dev, const int* tiles_dev, int n_tiles,
+                                       void* scratch_dev, size_t scratch_bytes, uint16_t* out16_dev,
+                                       uint16_t* out16_lo_dev, float* out32_dev, int* err_dev, void* stream);
+
 /* ---- host-only page allocator (no GPU needed): the policy behind fa_seq_* ----
  * Lowest free page id first; compaction moves the highest live page into the lowest
  * free id until the live pages are [0, n_live). */

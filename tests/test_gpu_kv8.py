@@ -1,0 +1,733 @@
+"""The 8-bit cache on the GPU against tests/kv8_plain.py: byte identity for the writes,
+one rounding for the reads, derived bounds for the attention."""
+import numpy as np
+import pytest
+
+import fa_dec
+import kv8_plain as P
+import oracle
+from helpers import dev, rel_rms
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = [P.INT8, P.E4M3]
+IDS = ["int8", "e4m3"]
+F16_NAN = 0x7fff
+
+
+def _stream(torch):
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _err(torch):
+    return torch.zeros(1, dtype=torch.int32, device="cuda")
+
+
+def _src(torch, x, src_type):
+    """x (f32) on the device in src_type, and the same values as f32."""
+    t = dev(torch, x).to({P.F32: torch.float32, P.F16: torch.float16, P.BF16: torch.bfloat16}[src_type])
+    return t, t.float().cpu().numpy()
+
+
+def _vectors(rng, *shape):
+    """Head vectors of different sizes with a few large channels."""
+    x = rng.standard_normal((*shape, 128)) * np.exp(0.5 * rng.standard_normal((*shape, 1)))
+    x[..., ::37] *= 4
+    return x.astype(np.float32)
+
+
+def _table(rng, lens, n_pages, stride=None):
+    stride = stride or max(-(-max(lens) // 16), 1)
+    pages = rng.permutation(n_pages)
+    bt, used = np.zeros((len(lens), stride), np.int32), 0
+    for i, n in enumerate(lens):
+        need = -(-n // 16)
+        bt[i, :need] = pages[used:used + need]
+        used += need
+    return bt
+
+
+def _garbage_pool(rng, layers, n_pages, hkv):
+    """Random bytes: among them e4m3 NaN, and scales that are NaN, infinite or huge."""
+    pool = rng.integers(0, 256, (layers, n_pages, hkv, P.TILE), dtype=np.uint8)
+    pool[:, ::2, :, -128:] = 0xff
+    return pool
+
+
+def _append(torch, k, v, src_type, row_stride, M, layers, hkv, pos, slot, bt, n_pages, fmt, pool, err):
+    fa_dec.op_kv8_append(k.data_ptr(), v.data_ptr(), src_type, row_stride, M, layers, hkv, pos.data_ptr(),
+                         slot.data_ptr(), bt.data_ptr(), bt.shape[1], n_pages, fmt, pool.data_ptr(), err.data_ptr(),
+                         _stream(torch))
+
+
+# ------------------------------------------------------------------ append --
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("src_type,layers,hkv,M", [(P.F16, 1, 8, 1), (P.F32, 3, 8, 77), (P.BF16, 2, 5, 33),
+                                                   (P.F16, 28, 8, 3), (P.F32, 1, 1, 19), (P.F32, 1, 64, 5)])
+def test_append_bytes_are_exact(torch_cuda, fmt, src_type, layers, hkv, M):
+    torch = torch_cuda
+    rng = np.random.default_rng(M)
+    lens = [M + 16, 40]
+    n_pages = 2 * (-(-(M + 16) // 16) + 3) + 1
+    bt = _table(rng, lens, n_pages)
+    slot = np.where(np.arange(M) % 3 == 2, 1, 0).astype(np.int32)
+    pos = np.where(slot == 1, np.arange(M) // 3, np.arange(M) + 7).astype(np.int32)
+    pos[np.arange(M) % 5 == 4] = -1                              # padding rows
+    order = rng.permutation(M)
+    slot, pos = slot[order], pos[order]
+    keep = (pos < 0) | (pos < np.where(slot == 1, 40, M + 16))
+    pos[~keep] = -1
+    # K and V as slices of one projection row with a gap behind them
+    ld = 2 * layers * hkv * 128 + 64
+    x = np.zeros((M, ld), np.float32)
+    kv = _vectors(rng, 2, M, layers, hkv)
+    kv[0, 0, 0, 0] = 0                                           # a zero vector
+    kv[1, M // 2, -1, -1, 5] = 1000
+    n = layers * hkv * 128
+    x[:, :n], x[:, n:2 * n] = kv[0].reshape(M, n), kv[1].reshape(M, n)
+    d_x, x = _src(torch, x, src_type)
+    k, v = (x[:, i * n:(i + 1) * n].reshape(M, layers, hkv, 128) for i in (0, 1))
+    pool = _garbage_pool(rng, layers, n_pages, hkv)
+    d_pool, d_err = dev(torch, pool), _err(torch)
+    _append(torch, d_x, d_x[:, n:], src_type, ld, M, layers, hkv, dev(torch, pos), dev(torch, slot), dev(torch, bt),
+            n_pages, fmt, d_pool, d_err)
+    slot_of = np.where(pos < 0, 0, slot)
+    P.write(pool, bt, slot_of, pos, k, v, fmt)
+    assert np.array_equal(d_pool.cpu().numpy(), pool)
+    assert int(d_err) == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_append_edge_vectors(torch_cuda, fmt):
+    """Ties, the smallest and the largest f32, subnormals, infinities and NaN."""
+    torch = torch_cuda
+    rng = np.random.default_rng(5)
+    M = 64
+    x = _vectors(rng, 2, M, 1, 1)
+    for i, scale in enumerate([1e-38, 1e-41, 1e-45, 1e30, 2e37, 1.0]):
+        x[0, i] *= np.float32(scale)
+    ties = (np.arange(128) - 64 + 0.5).astype(np.float32)
+    ties[0] = 127
+    x[0, 8, 0, 0] = ties                                          # d = 1 in int8: all ties
+    x[0, 9, 0, 0] = ties * np.float32(1.7)                        # near ties of a rounded d
+    x[0, 10, 0, 0] = np.where(np.arange(128) % 2, 1, -1) * np.float32(448 * 2.0 ** -5)
+    x[0, 11, 0, 0] = np.concatenate([[448], np.arange(127) + 0.5]).astype(np.float32)
+    x[0, 12, 0, 0, 7], x[0, 13, 0, 0, 127], x[0, 14, 0, 0, 0] = np.nan, np.inf, -np.inf
+    x[0, 15] = np.finfo(np.float32).max
+    x[0, 16] = 0
+    x[0, 17] = -0.0
+    # quotients next to a border: the neighbours of (k + 1/2) d for random d
+    for m in range(20, M):
+        amax = np.float32(rng.uniform(1, 2) * 2.0 ** rng.integers(-20, 20))
+        d = np.float32(np.float64(amax) / 127)
+        border = ((rng.integers(0, 127, 127) + 0.5) * np.float64(d)).astype(np.float32)
+        step = rng.integers(-1, 2, 127)
+        near = np.where(step < 0, np.nextafter(border, 0), np.where(step > 0, np.nextafter(border, np.inf), border))
+        x[:, m, 0, 0] = np.concatenate([[amax], np.minimum(near.astype(np.float32), amax)])
+    pos = np.arange(M, dtype=np.int32)
+    bt = np.arange(4, dtype=np.int32)[None]
+    pool = np.zeros((1, 4, 1, P.TILE), np.uint8)
+    d_pool, d_err = dev(torch, pool), _err(torch)
+    _append(torch, dev(torch, x[0]), dev(torch, x[1]), P.F32, 128, M, 1, 1, dev(torch, pos),
+            dev(torch, np.zeros(M, np.int32)), dev(torch, bt), 4, fmt, d_pool, d_err)
+    P.write(pool, bt, np.zeros(M, np.int32), pos, x[0], x[1], fmt)
+    got, want = d_pool.cpu().numpy(), pool
+    (q, d), (qw, dw) = P.parts(got), P.parts(want)
+    assert np.array_equal(np.isnan(d), np.isnan(dw)) and np.array_equal(d[~np.isnan(d)], dw[~np.isnan(dw)])
+    assert np.array_equal(q, qw)
+
+
+@pytest.mark.parametrize("bad", ["pos", "past_table", "page", "page_negative", "slot"])
+def test_append_flags_bad_rows_and_writes_the_others(torch_cuda, bad):
+    torch = torch_cuda
+    rng = np.random.default_rng(6)
+    M, hkv, n_pages = 6, 8, 8
+    k, v = _vectors(rng, M, 1, hkv), _vectors(rng, M, 1, hkv)
+    bt = np.arange(8, dtype=np.int32).reshape(2, 4)[:, ::-1].copy()
+    slot, pos = np.array([0, 0, 1, 1, 0, 1], np.int32), np.array([0, 17, 33, 5, 40, 63], np.int32)
+    kb, want = bt.copy(), pos.copy()
+    if bad == "pos": pos[2] = -2
+    elif bad == "past_table": pos[2] = 64
+    elif bad == "page": kb[1, 2] = n_pages
+    elif bad == "page_negative": kb[1, 2] = -1
+    else: slot[2] = -1
+    want[2] = -1
+    pool = _garbage_pool(rng, 1, n_pages, hkv)
+    d_pool, d_err = dev(torch, pool), _err(torch)
+    _append(torch, dev(torch, k), dev(torch, v), P.F32, 1024, M, 1, hkv, dev(torch, pos), dev(torch, slot),
+            dev(torch, kb), n_pages, P.INT8, d_pool, d_err)
+    P.write(pool, bt, np.maximum(slot, 0), want, k, v, P.INT8)
+    assert np.array_equal(d_pool.cpu().numpy(), pool)
+    assert int(d_err) == (2 if bad.startswith("page") else 4)
+
+
+def test_append_reaches_pages_behind_2_gib(torch_cuda):
+    torch = torch_cuda
+    rng = np.random.default_rng(7)
+    hkv, n_pages = 8, 70000                                       # 2.4 GB
+    pool = torch.zeros((1, n_pages, hkv, P.TILE), dtype=torch.uint8, device="cuda")
+    bt = np.array([[69999, 3, 65000]], np.int32)
+    M = 48
+    k, v = _vectors(rng, M, 1, hkv), _vectors(rng, M, 1, hkv)
+    pos, slot, d_err = np.arange(M, dtype=np.int32), np.zeros(M, np.int32), _err(torch)
+    d = [dev(torch, a) for a in (k, v, pos, slot, bt)]
+    _append(torch, d[0], d[1], P.F32, 1024, M, 1, hkv, d[2], d[3], d[4], n_pages, P.INT8, pool, d_err)
+    small = np.zeros((1, 3, hkv, P.TILE), np.uint8)
+    P.write(small, np.array([[0, 1, 2]]), slot, pos, k, v, P.INT8)
+    assert np.array_equal(pool[:, bt[0].tolist()].cpu().numpy(), small)
+    q = dev(torch, (rng.standard_normal((1, 16, 128)) * 0.1).astype(np.float32))
+    out = _decode(torch, q, 16, hkv, dev(torch, np.array([47], np.int32)), d[3][:1], d[4], n_pages, P.INT8, pool, d_err)
+    want = P.attention(q.cpu().numpy()[0], *[x[0] for x in P.read(small, np.array([0, 1, 2]), 0, 48, P.INT8)])
+    assert rel_rms(out.cpu().numpy()[0], want.reshape(-1)) < 5e-6
+    assert int(d_err) == 0
+
+
+# ------------------------------------------------------------ kernel 1 form --
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,M", [(16, 8, 1), (16, 8, 130), (5, 5, 17), (12, 4, 9), (16, 2, 33), (1, 1, 3)])
+def test_qknorm_rope_append_matches_definition(torch_cuda, fmt, hq, hkv, M):
+    torch = torch_cuda
+    rng = np.random.default_rng(hq * 100 + M)
+    max_pos, n_pages = 512, 40
+    qkv = _vectors(rng, M, hq + 2 * hkv) * 2
+    qkv[0, hq] = 0
+    qn, kn = (rng.uniform(0.8, 1.2, 128).astype(np.float32) for _ in range(2))
+    rope = np.asarray(oracle.rope_table(max_pos), np.float32).reshape(max_pos, 64, 2)
+    bt = _table(rng, [max_pos], n_pages)
+    pos = rng.permutation(max_pos)[:M].astype(np.int32)
+    if M > 2:
+        pos[1] = -1
+    slot = np.where(pos < 0, 10 ** 6, 0).astype(np.int32)         # a padding row's slot is not looked at
+    pool = _garbage_pool(rng, 1, n_pages, hkv)
+    d_pool, d_err = dev(torch, pool), _err(torch)
+    q_out = torch.full((M, hq, 128), 7.0, device="cuda")
+    d = [dev(torch, a) for a in (qkv, pos, slot, bt, qn, kn, rope)]
+    fa_dec.op_qknorm_rope_append_kv8(d[0].data_ptr(), M, hq, hkv, d[1].data_ptr(), d[2].data_ptr(), d[3].data_ptr(),
+                                     bt.shape[1], n_pages, d[4].data_ptr(), d[5].data_ptr(), 1e-5, d[6].data_ptr(),
+                                     max_pos, fmt, d_pool.data_ptr(), q_out.data_ptr(), d_err.data_ptr(),
+                                     _stream(torch))
+    live = pos >= 0
+    rot = rope[np.maximum(pos, 0)]
+    q = P.norm_rotate(qkv[:, :hq], qn, rot) * np.float32(1 / np.sqrt(np.float32(128)))
+    q[~live] = 7
+    k = P.norm_rotate(qkv[:, hq:hq + hkv], kn, rot)
+    P.write(pool, bt, np.zeros(M, np.int32), pos, k[:, None], qkv[:, hq + hkv:][:, None], fmt)
+    assert np.array_equal(q_out.cpu().numpy(), q)
+    assert np.array_equal(d_pool.cpu().numpy(), pool)
+    assert int(d_err) == 0
+
+
+def test_qknorm_rope_append_q_equals_the_f16_pools_op(torch_cuda):
+    torch = torch_cuda
+    rng = np.random.default_rng(21)
+    M, max_pos = 37, 256
+    qkv, pos = _vectors(rng, M, 32), rng.permutation(max_pos)[:M].astype(np.int32)
+    d = [dev(torch, a) for a in (qkv, pos, np.zeros(M, np.int32), np.arange(16, dtype=np.int32)[None],
+                                 np.ones(128, np.float32), np.ones(128, np.float32),
+                                 np.asarray(oracle.rope_table(max_pos), np.float32))]
+    p = [x.data_ptr() for x in d]
+    q16, q8 = (torch.zeros((M, 16, 128), device="cuda") for _ in range(2))
+    pool16 = torch.zeros((16, 8 * 2 * 16 * 128), dtype=torch.int16, device="cuda")
+    pool8 = torch.zeros((16, 8, P.TILE), dtype=torch.uint8, device="cuda")
+    err = _err(torch)
+    fa_dec.op_qknorm_rope_append(p[0], M, p[1], p[2], p[3], 16, 16, p[4], p[5], 1e-5, p[6], max_pos, pool16.data_ptr(),
+                                 q16.data_ptr(), err.data_ptr(), _stream(torch))
+    fa_dec.op_qknorm_rope_append_kv8(p[0], M, 16, 8, p[1], p[2], p[3], 16, 16, p[4], p[5], 1e-5, p[6], max_pos, P.INT8,
+                                     pool8.data_ptr(), q8.data_ptr(), err.data_ptr(), _stream(torch))
+    assert torch.equal(q16, q8)
+    # the f16 cache rounds a value by 2^-11 of it at most, the 8-bit one by half a step
+    f16 = pool16.view(torch.float16).reshape(16, 8, 2, 16, 128).float().cpu().numpy()
+    raw, d8 = P.parts(pool8.cpu().numpy())
+    off = np.abs(P.values(raw, P.INT8) * d8[..., None] - f16)
+    assert (off <= d8[..., None] * 0.5 * (1 + 1e-6) + np.abs(f16) * 2.0 ** -11).all()
+    assert int(err) == 0
+
+
+def test_qknorm_rope_append_flags_bad_rows(torch_cuda):
+    torch = torch_cuda
+    rng = np.random.default_rng(22)
+    for pos, page, bits in ((-2, 0, 4), (64, 0, 4), (40, 0, 4), (3, 9, 2), (3, -1, 2)):
+        d = [dev(torch, a) for a in (_vectors(rng, 1, 32), np.array([pos], np.int32), np.zeros(1, np.int32),
+                                     np.array([[page, 1]], np.int32), np.ones(128, np.float32),
+                                     np.asarray(oracle.rope_table(64), np.float32))]
+        p = [x.data_ptr() for x in d]
+        q, err = torch.zeros((1, 16, 128), device="cuda"), _err(torch)
+        pool = torch.full((4, 8, P.TILE), 77, dtype=torch.uint8, device="cuda")
+        fa_dec.op_qknorm_rope_append_kv8(p[0], 1, 16, 8, p[1], p[2], p[3], 2, 4, p[4], p[4], 1e-5, p[5], 64, P.INT8,
+                                         pool.data_ptr(), q.data_ptr(), err.data_ptr(), _stream(torch))
+        assert int(err) == bits and bool((pool == 77).all())
+
+
+# ------------------------------------------------------------------ gather --
+def _filled(rng, lens, layers, hkv, fmt, n_pages=None, spread=0.5):
+    """A pool of garbage with these sequences written into it, the table and the read-back."""
+    n_pages = n_pages or sum(-(-n // 16) for n in lens) + 3
+    bt = _table(rng, lens, n_pages)
+    pool = _garbage_pool(rng, layers, n_pages, hkv)
+    raw, scales = P.parts(pool)
+    for i, n in enumerate(lens):
+        if not n:
+            continue
+        x = rng.standard_normal((2, n, layers, hkv, 128)) * np.exp(spread * rng.standard_normal((2, n, layers, hkv, 1)))
+        q, d = P.quantise(x.astype(np.float32), fmt)
+        t = np.arange(n)
+        for part in (0, 1):
+            raw[:, bt[i, t // 16], :, part, t % 16] = q[part]
+            scales[:, bt[i, t // 16], :, part, t % 16] = d[part]
+    return pool, bt, n_pages
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("out_type,layers,hkv", [(P.F16, 3, 8), (P.BF16, 1, 5), (P.F32, 2, 1), (P.F16, 1, 11)])
+def test_gather_ragged_ranges(torch_cuda, fmt, out_type, layers, hkv):
+    torch = torch_cuda
+    rng = np.random.default_rng(hkv)
+    lens = [1, 16, 17, 320, 47, 33, 5]
+    pool, bt, n_pages = _filled(rng, lens, layers, hkv, fmt)
+    t0 = np.array([0, 0, 16, 3, 31, 0, 2], np.int32)
+    n_tok = np.array([1, 16, 1, 301, 2, 0, 3], np.int32)
+    slot = np.arange(7, dtype=np.int32)
+    order = rng.permutation(7)
+    row0 = np.zeros(7, np.int32)
+    at = 2
+    for m in order:
+        row0[m] = at
+        at += n_tok[m] + 1                                        # gaps
+    total = at + 3
+    dt = {P.F32: torch.float32, P.F16: torch.float16, P.BF16: torch.bfloat16}[out_type]
+    k_out, v_out = (torch.full((layers, hkv, total, 128), 9.0, dtype=dt, device="cuda") for _ in range(2))
+    d = [dev(torch, a) for a in (pool, bt, slot[order], t0[order], n_tok[order], row0[order])]
+    p, err = [x.data_ptr() for x in d], _err(torch)
+    fa_dec.op_kv8_gather(p[0], fmt, layers, n_pages, hkv, p[1], bt.shape[1], p[2], p[3], p[4], p[5], 7, 301, total,
+                         out_type, k_out.data_ptr(), v_out.data_ptr(), err.data_ptr(), _stream(torch))
+    want = np.full((2, layers, hkv, total, 128), 9.0)
+    for m in range(7):
+        kv = P.read(pool, bt[m], t0[m], t0[m] + n_tok[m], fmt)
+        for part in (0, 1):
+            want[part, :, :, row0[m]:row0[m] + n_tok[m]] = kv[part]
+    for part, got in ((0, k_out), (1, v_out)):
+        # d q is formed in f32 and rounded to the type: the f32 product of the definition, rounded once
+        w = torch.from_numpy(want[part].astype(np.float32)).to(dt)
+        assert torch.equal(got.cpu(), w)
+    assert int(err) == 0
+    if not t0[0]:                                                 # NULL t0: from the first token
+        one = torch.zeros((layers, hkv, 1, 128), dtype=dt, device="cuda")
+        two = torch.zeros_like(one)
+        z = dev(torch, np.zeros(1, np.int32))
+        fa_dec.op_kv8_gather(p[0], fmt, layers, n_pages, hkv, p[1], bt.shape[1], z.data_ptr(), 0,
+                             dev(torch, np.ones(1, np.int32)).data_ptr(), z.data_ptr(), 1, 1, 1, out_type,
+                             one.data_ptr(), two.data_ptr(), err.data_ptr(), _stream(torch))
+        assert torch.equal(one.cpu(), torch.from_numpy(want[0][:, :, row0[0]:row0[0] + 1].astype(np.float32)).to(dt))
+
+
+@pytest.mark.parametrize("over,bits", [(dict(n_tok=17), 8), (dict(n_tok=-1), 8), (dict(t0=-1), 8), (dict(t0=20), 8),
+                                       (dict(row0=-1), 8), (dict(row0=17), 8), (dict(slot=-1), 8),
+                                       (dict(page=3), 2), (dict(page=-1), 2), (dict(t0=2 ** 31 - 8), 8),
+                                       (dict(row0=2 ** 31 - 1), 8)], ids=str)
+def test_gather_flags_bad_ranges(torch_cuda, over, bits):
+    torch = torch_cuda
+    a = dict(slot=0, t0=0, n_tok=16, row0=0, page=1)
+    a.update(over)
+    pool = torch.zeros((1, 3, 8, P.TILE), dtype=torch.uint8, device="cuda")
+    d = {k: dev(torch, np.array([a[k]], np.int32)) for k in ("slot", "t0", "n_tok", "row0")}
+    bt = dev(torch, np.array([[a["page"], 2]], np.int32))
+    k_out, v_out = (torch.full((1, 8, 32, 128), 9.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    err = _err(torch)
+    fa_dec.op_kv8_gather(pool.data_ptr(), P.INT8, 1, 3, 8, bt.data_ptr(), 2, d["slot"].data_ptr(), d["t0"].data_ptr(),
+                         d["n_tok"].data_ptr(), d["row0"].data_ptr(), 1, 16, 32, P.F16, k_out.data_ptr(),
+                         v_out.data_ptr(), err.data_ptr(), _stream(torch))
+    assert int(err) == bits
+    assert bool((k_out == 9).all()) and bool((v_out == 9).all())
+
+
+# --------------------------------------------------------------- attention --
+def _scratch(torch, size):
+    return torch.full((max(size, 16),), 0xff, dtype=torch.uint8, device="cuda")      # NaN bytes: nothing is read unwritten
+
+
+def _decode(torch, q, hq, hkv, pos, slot, bt, n_pages, fmt, pool, err, out16=None, out16_lo=None, out=None):
+    M = q.shape[0]
+    out = torch.full((M, hq * 128), 5.0, device="cuda") if out is None else out
+    size = fa_dec.op_attention_kv8_scratch_bytes(M, hq, hkv)
+    scratch = _scratch(torch, size)
+    fa_dec.op_paged_attention_kv8(q.data_ptr(), M, hq, hkv, pos.data_ptr(), slot.data_ptr(), bt.data_ptr(),
+                                  bt.shape[1], n_pages, fmt, pool.data_ptr(), scratch.data_ptr(), size,
+                                  out32=out.data_ptr(), err=err.data_ptr(), stream=_stream(torch),
+                                  out16=0 if out16 is None else out16.data_ptr(),
+                                  out16_lo=0 if out16_lo is None else out16_lo.data_ptr())
+    return out
+
+
+def _tiles(rows, step):
+    """(first row, rows) pairs covering runs of rows (first, count)."""
+    return np.array([(f + i, min(step, n - i)) for f, n in rows for i in range(0, n, step)], np.int32)
+
+
+def _prefill(torch, q, hq, hkv, pos, slot, bt, n_pages, fmt, pool, tiles, err, out16=None, out16_lo=None, out=None):
+    M = q.shape[0]
+    out = torch.full((M, hq * 128), 5.0, device="cuda") if out is None else out
+    size = fa_dec.op_prefill_attention_kv8_scratch_bytes(len(tiles), hq, hkv)
+    scratch, d_tiles = _scratch(torch, size), dev(torch, tiles)
+    fa_dec.op_prefill_attention_kv8(q.data_ptr(), M, hq, hkv, pos.data_ptr(), slot.data_ptr(), bt.data_ptr(),
+                                    bt.shape[1], n_pages, fmt, pool.data_ptr(), d_tiles.data_ptr(), len(tiles),
+                                    scratch.data_ptr(), size, out32=out.data_ptr(), err=err.data_ptr(),
+                                    stream=_stream(torch), out16=0 if out16 is None else out16.data_ptr(),
+                                    out16_lo=0 if out16_lo is None else out16_lo.data_ptr())
+    return out
+
+
+def _bound(q, k, v):
+    """Largest error of an output of a row: a score is off by 2^-18 of sum |q k| at most (f32
+    sums of 128 products that carry 22 bits: 128 x 2^-24 + 2^-22 < 2^-16.9 if every rounding
+    went the same way, 2^-20 as they fall; an eighth of the former), a weight by that times ln 2
+    relative, and the weighted sum by 2^-18 of the largest |v|."""
+    g = len(q) // len(k)
+    s = max(float((np.abs(k[h // g]) @ np.abs(q[h].astype(np.float64))).max()) for h in range(len(q)))
+    return 2 * (2.0 ** -18 * s + 2.0 ** -18) * float(np.abs(v).max())
+
+
+LENS = [1, 2, 15, 16, 17, 31, 33, 64, 65, 255, 256, 257, 640, 1000]
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("hq,hkv", [(16, 8), (8, 8), (12, 4), (16, 2), (32, 8), (5, 5), (5, 1), (1, 1), (7, 1)])
+def test_decode_attention_ragged(torch_cuda, fmt, hq, hkv):
+    torch = torch_cuda
+    rng = np.random.default_rng(hq * 10 + hkv)
+    pool, bt, n_pages = _filled(rng, LENS, 1, hkv, fmt)
+    order = rng.permutation(len(LENS))
+    slot = np.concatenate([order, [10 ** 6, 3]]).astype(np.int32)
+    pos = np.array([LENS[i] - 1 for i in order] + [-1, 4], np.int32)      # a padding row; a second row of sequence 3
+    M = len(slot)
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    err = _err(torch)
+    out16, lo = (torch.zeros((M, hq * 128), dtype=torch.float16, device="cuda") for _ in range(2))
+    got = _decode(torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, slot), dev(torch, bt), n_pages, fmt,
+                  dev(torch, pool), err, out16, lo)
+    o32, pair = got.cpu().numpy(), (out16.float() + lo.float()).cpu().numpy()
+    assert int(err) == 0
+    for m in range(M):
+        if pos[m] < 0:
+            assert not o32[m].any() and not pair[m].any()
+            continue
+        k, v = (x[0] for x in P.read(pool, bt[slot[m]], 0, pos[m] + 1, fmt))
+        want = P.attention(q[m], k, v).reshape(-1)
+        assert np.abs(o32[m] - want).max() <= _bound(q[m], k, v)
+        assert rel_rms(o32[m], want) <= 5e-6, (m, pos[m])
+        # the pair keeps 22 bits of the f32 output, its low part down to the f16 subnormals
+        assert np.abs(pair[m] - o32[m]).max() <= np.abs(o32[m]).max() * 2.0 ** -21 + 2.0 ** -24
+    assert np.array_equal(out16.cpu().numpy(), got.cpu().numpy().astype(np.float16))
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("n,hq,hkv,M", [(4001, 16, 8, 1), (20000, 16, 8, 2), (40960, 8, 1, 1), (9999, 32, 4, 3)])
+def test_decode_attention_long(torch_cuda, fmt, n, hq, hkv, M):
+    torch = torch_cuda
+    rng = np.random.default_rng(n)
+    lens = [n - 37 * i for i in range(M)]
+    pool, bt, n_pages = _filled(rng, lens, 1, hkv, fmt)
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    err = _err(torch)
+    got = _decode(torch, dev(torch, q), hq, hkv, dev(torch, np.array(lens, np.int32) - 1),
+                  dev(torch, np.arange(M, dtype=np.int32)), dev(torch, bt), n_pages, fmt, dev(torch, pool), err)
+    for m in range(M):
+        k, v = (x[0] for x in P.read(pool, bt[m], 0, lens[m], fmt))
+        want = P.attention(q[m], k, v).reshape(-1)
+        assert rel_rms(got[m].cpu().numpy(), want) <= 5e-6
+    assert int(err) == 0
+
+
+@pytest.mark.parametrize("kind", ["sharp", "scales", "q_small", "q_large", "zeros"])
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_attention_value_ranges(torch_cuda, fmt, which, kind):
+    """Scores far apart, vectors whose sizes differ by many powers of ten, tiny and huge
+    queries, zero vectors."""
+    torch = torch_cuda
+    rng = np.random.default_rng(3)
+    hq, hkv, n, M = 16, 8, 300, 20
+    pool, bt, n_pages = _filled(rng, [n], 1, hkv, fmt)
+    raw, scales = P.parts(pool)
+    page, t = bt[0, np.arange(n) // 16], np.arange(n) % 16
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    if kind == "sharp":
+        q *= 20
+    elif kind == "scales":      # K and V sizes over many decades; the weight of a large V stays what it is
+        scales[0, page, :, 0, t] *= (10.0 ** rng.uniform(-6, 0, (n, hkv))).astype(np.float32)
+        scales[0, page, :, 1, t] *= (10.0 ** rng.uniform(-12, 12, (n, hkv))).astype(np.float32)
+    elif kind == "q_small":
+        q *= np.float32(1e-30)
+    elif kind == "q_large":     # scores of thousands over keys of 1e-3
+        q *= np.float32(1e6)
+        scales[0, page, :, 0, t] *= np.float32(1e-4)
+    else:
+        raw[0, page[::3], :, 1, t[::3]] = 0
+        scales[0, page[::3], :, 1, t[::3]] = P.TINY
+        q[:, 3] = 0
+    pos = np.arange(n - M, n).astype(np.int32)
+    args = (torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, np.zeros(M, np.int32)), dev(torch, bt), n_pages,
+            fmt, dev(torch, pool))
+    err = _err(torch)
+    got = _decode(*args, err) if which == "decode" else _prefill(*args, _tiles([(0, M)], 64), err)
+    got = got.cpu().numpy().reshape(M, hq, 128)
+    for m in range(M):
+        k, v = (x[0] for x in P.read(pool, bt[0], 0, pos[m] + 1, fmt))
+        want = P.attention(q[m], k, v)
+        for h in range(hq):
+            b = _bound(q[m, h:h + 1], k[h // 2:h // 2 + 1], v[h // 2:h // 2 + 1])
+            assert np.abs(got[m, h] - want[h]).max() <= b, (m, h)
+    assert int(err) == 0
+
+
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_nan_vectors_reach_their_own_rows_only(torch_cuda, fmt, which):
+    """A token whose K or V vector is NaN makes the rows that see it NaN, on its head alone;
+    rows before it, other sequences and masked places are untouched."""
+    torch = torch_cuda
+    rng = np.random.default_rng(4)
+    hq, hkv, lens = 16, 8, [70, 70]
+    pool, bt, n_pages = _filled(rng, lens, 1, hkv, fmt)
+    _, scales = P.parts(pool)
+    scales[0, bt[0, 50 // 16], 2, 0, 50 % 16] = np.nan            # K of token 50, KV head 2
+    scales[0, bt[0, 60 // 16], 5, 1, 60 % 16] = np.nan            # V of token 60, KV head 5
+    M = 140
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    pos, slot = np.tile(np.arange(70), 2).astype(np.int32), np.repeat([0, 1], 70).astype(np.int32)
+    args = (torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, slot), dev(torch, bt), n_pages, fmt,
+            dev(torch, pool))
+    err = _err(torch)
+    got = _decode(*args, err) if which == "decode" else _prefill(*args, _tiles([(0, 70), (70, 70)], 64), err)
+    nan = np.isnan(got.cpu().numpy().reshape(M, hq, 128))
+    want = np.zeros_like(nan)
+    want[50:70, 4:6] = True
+    want[60:70, 10:12] = True
+    assert np.array_equal(nan, want)
+
+
+@pytest.mark.parametrize("bad", ["pos", "past_table", "slot", "page", "page_negative"])
+def test_decode_attention_flags_bad_rows(torch_cuda, bad):
+    torch = torch_cuda
+    rng = np.random.default_rng(8)
+    hq, hkv, lens = 16, 8, [40, 200, 64]
+    pool, bt, n_pages = _filled(rng, lens, 1, hkv, P.INT8)
+    pos, slot = np.array([39, 199, 63], np.int32), np.array([0, 1, 2], np.int32)
+    q = (rng.standard_normal((3, hq, 128)) * 0.3).astype(np.float32)
+    kb = bt.copy()
+    if bad == "pos": pos[1] = -2
+    elif bad == "past_table": pos[1] = 16 * bt.shape[1]
+    elif bad == "slot": slot[1] = -1
+    elif bad == "page": kb[1, 3] = n_pages
+    else: kb[1, 3] = -1
+    err = _err(torch)
+    got = _decode(torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, slot), dev(torch, kb), n_pages, P.INT8,
+                  dev(torch, pool), err).cpu().numpy()
+    assert int(err) == (2 if bad.startswith("page") else 8)
+    for m in (0, 1, 2):
+        k, v = (x[0] for x in P.read(pool, bt[m], 0, lens[m], P.INT8))
+        if m == 1 and bad.startswith("page"):                     # the bad page's tokens are left out
+            keep = np.r_[0:48, 64:200]
+            k, v = k[:, keep], v[:, keep]
+        elif m == 1:
+            assert (got[1] == 5).all()
+            continue
+        assert rel_rms(got[m], P.attention(q[m], k, v).reshape(-1)) <= 5e-6
+
+
+# ----------------------------------------------------------------- prefill --
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,chunks", [
+    (16, 8, [(0, 112)]), (16, 8, [(0, 1), (5, 1), (63, 2), (64, 65)]), (16, 8, [(700, 130), (0, 64), (15, 17)]),
+    (8, 8, [(33, 200)]), (12, 4, [(100, 90)]), (16, 2, [(70, 40), (0, 16)]), (5, 1, [(20, 60)]), (32, 8, [(250, 70)]),
+    (7, 1, [(3, 37)]), (1, 1, [(0, 129)])])
+def test_prefill_attention_ragged(torch_cuda, fmt, hq, hkv, chunks):
+    torch = torch_cuda
+    rng = np.random.default_rng(len(chunks) * 100 + hq)
+    lens = [b + n for b, n in chunks]
+    pool, bt, n_pages = _filled(rng, lens, 1, hkv, fmt)
+    pos = np.concatenate([np.arange(b, b + n) for b, n in chunks]).astype(np.int32)
+    slot = np.repeat(np.arange(len(chunks)), [n for _, n in chunks]).astype(np.int32)
+    first = np.concatenate([[0], np.cumsum([n for _, n in chunks])[:-1]])
+    tiles = _tiles([(int(f), n) for f, (_, n) in zip(first, chunks)], 128 * hkv // hq)
+    M = len(pos)
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    err = _err(torch)
+    out16, lo = (torch.zeros((M, hq * 128), dtype=torch.float16, device="cuda") for _ in range(2))
+    got = _prefill(torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, slot), dev(torch, bt), n_pages, fmt,
+                   dev(torch, pool), tiles, err, out16, lo).cpu().numpy()
+    pair = (out16.float() + lo.float()).cpu().numpy()
+    assert int(err) == 0
+    for m in range(M):
+        k, v = (x[0] for x in P.read(pool, bt[slot[m]], 0, pos[m] + 1, fmt))
+        want = P.attention(q[m], k, v).reshape(-1)
+        assert np.abs(got[m] - want).max() <= _bound(q[m], k, v)
+        assert rel_rms(got[m], want) <= 5e-6, m
+        assert np.abs(pair[m] - got[m]).max() <= np.abs(got[m]).max() * 2.0 ** -21 + 2.0 ** -24
+
+
+def test_prefill_attention_repeated_and_padded_rows(torch_cuda):
+    """Positions that repeat within a tile, rows of no tile, and a tile that begins with padding."""
+    torch = torch_cuda
+    rng = np.random.default_rng(9)
+    hq, hkv = 16, 8
+    pool, bt, n_pages = _filled(rng, [90], 1, hkv, P.INT8)
+    pos = np.array([-1, -1, 40, 40, 41, 89, 89, 7], np.int32)
+    M = len(pos)
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    err = _err(torch)
+    got = _prefill(torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, np.zeros(M, np.int32)), dev(torch, bt),
+                   n_pages, P.INT8, dev(torch, pool), np.array([[0, 7]], np.int32), err).cpu().numpy()
+    assert not got[:2].any() and (got[7] == 5).all() and int(err) == 0
+    for m in range(2, 7):
+        k, v = (x[0] for x in P.read(pool, bt[0], 0, pos[m] + 1, P.INT8))
+        assert rel_rms(got[m], P.attention(q[m], k, v).reshape(-1)) <= 5e-6
+
+
+@pytest.mark.parametrize("tile,pos,page,bits", [
+    ((0, 0), None, None, 4), ((0, 65), None, None, 4), ((-1, 4), None, None, 4), ((70, 64), None, None, 4),
+    ((2 ** 31 - 1, 4), None, None, 4), ((64, 64), -2, None, 8), ((64, 64), 10 ** 6, None, 8), ((64, 64), None, 99, 2),
+    ((64, 64), None, -1, 2)])
+def test_prefill_attention_flags_bad_tiles(torch_cuda, tile, pos, page, bits):
+    """The tile beside the bad one is computed; a bad tile or row writes nothing."""
+    torch = torch_cuda
+    rng = np.random.default_rng(10)
+    hq, hkv = 16, 8
+    pool, bt, n_pages = _filled(rng, [128], 1, hkv, P.INT8)
+    p = np.arange(128, dtype=np.int32)
+    if pos is not None:
+        p[127] = pos
+    kb = bt.copy()
+    if page is not None:
+        kb[0, 5] = page                                           # tokens 80..95
+    q = (rng.standard_normal((128, hq, 128)) * 0.3).astype(np.float32)
+    err = _err(torch)
+    got = _prefill(torch, dev(torch, q), hq, hkv, dev(torch, p), dev(torch, np.zeros(128, np.int32)), dev(torch, kb),
+                   n_pages, P.INT8, dev(torch, pool), np.array([[0, 64], tile], np.int32), err).cpu().numpy()
+    assert int(err) == bits
+    if tile[0] != 0:
+        k, v = (x[0] for x in P.read(pool, bt[0], 0, 128, P.INT8))
+        for m in range(64):
+            assert rel_rms(got[m], P.attention(q[m], k[:, :m + 1], v[:, :m + 1]).reshape(-1)) <= 5e-6
+        if pos is not None:
+            assert (got[127] == 5).all()
+        if page is not None:                                      # the bad page's tokens are left out
+            keep = np.r_[0:80, 96:128]
+            assert rel_rms(got[127], P.attention(q[127], k[:, keep], v[:, keep]).reshape(-1)) <= 5e-6
+        elif bits == 4:
+            assert (got[64:] == 5).all()
+
+
+# ---------------------------------------------------------------- together --
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_a_layers_steps_together_and_from_a_graph(torch_cuda, fmt):
+    """A prompt chunk through kernel (1) and the prefill attention, then decode steps (one row
+    per sequence, one of them padding) from ONE captured graph whose positions advance on the
+    device, on a stream of its own; every output against the read-back of the pages."""
+    torch = torch_cuda
+    rng = np.random.default_rng(11)
+    hq, hkv, max_pos, lens = 16, 8, 256, [45, 16, 70]
+    n_steps, n_pages = 20, 24
+    rope = np.asarray(oracle.rope_table(max_pos), np.float32).reshape(max_pos, 64, 2)
+    bt = _table(rng, [n + n_steps for n in lens], n_pages)
+    qn, kn = (rng.uniform(0.8, 1.2, 128).astype(np.float32) for _ in range(2))
+    pool, err = dev(torch, _garbage_pool(rng, 1, n_pages, hkv)), _err(torch)
+    d_bt, d_rope, d_qn, d_kn = (dev(torch, a) for a in (bt, rope, qn, kn))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def kernel1(qkv, pos, slot, q):
+        fa_dec.op_qknorm_rope_append_kv8(qkv.data_ptr(), len(pos), hq, hkv, pos.data_ptr(), slot.data_ptr(),
+                                         d_bt.data_ptr(), bt.shape[1], n_pages, d_qn.data_ptr(), d_kn.data_ptr(), 1e-5,
+                                         d_rope.data_ptr(), max_pos, fmt, pool.data_ptr(), q.data_ptr(),
+                                         err.data_ptr(), _stream(torch))
+
+    def check(out, q, pos, slot):
+        host = pool.cpu().numpy()
+        for m in range(len(pos)):
+            if pos[m] < 0:
+                assert not out[m].any()
+                continue
+            k, v = (x[0] for x in P.read(host, bt[slot[m]], 0, pos[m] + 1, fmt))
+            assert rel_rms(out[m], P.attention(q[m], k, v).reshape(-1)) <= 5e-6, (m, pos[m])
+
+    with torch.cuda.stream(side):
+        pos = np.concatenate([np.arange(n) for n in lens]).astype(np.int32)
+        slot = np.repeat([0, 1, 2], lens).astype(np.int32)
+        qkv = dev(torch, _vectors(rng, len(pos), hq + 2 * hkv))
+        q = torch.zeros((len(pos), hq, 128), device="cuda")
+        d_pos, d_slot = dev(torch, pos), dev(torch, slot)
+        kernel1(qkv, d_pos, d_slot, q)
+        first = np.concatenate([[0], np.cumsum(lens)[:-1]])
+        out = _prefill(torch, q, hq, hkv, d_pos, d_slot, d_bt, n_pages, fmt, pool,
+                       _tiles([(int(f), n) for f, n in zip(first, lens)], 64), err)
+        side.synchronize()
+        check(out.cpu().numpy(), q.cpu().numpy(), pos, slot)
+
+        M = 4
+        d_pos = dev(torch, np.array(lens + [-1], np.int32))
+        d_slot = dev(torch, np.array([0, 1, 2, 0], np.int32))
+        step = dev(torch, np.array([1, 1, 1, 0], np.int32))
+        qkv = torch.zeros((M, hq + 2 * hkv, 128), device="cuda")
+        q, out = torch.zeros((M, hq, 128), device="cuda"), torch.zeros((M, hq * 128), device="cuda")
+        size = fa_dec.op_attention_kv8_scratch_bytes(M, hq, hkv)
+        scratch = _scratch(torch, size)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            kernel1(qkv, d_pos, d_slot, q)
+            fa_dec.op_paged_attention_kv8(q.data_ptr(), M, hq, hkv, d_pos.data_ptr(), d_slot.data_ptr(),
+                                          d_bt.data_ptr(), bt.shape[1], n_pages, fmt, pool.data_ptr(),
+                                          scratch.data_ptr(), size, out32=out.data_ptr(), err=err.data_ptr(),
+                                          stream=_stream(torch))
+            d_pos += step
+        for i in range(n_steps):
+            qkv.copy_(dev(torch, _vectors(rng, M, hq + 2 * hkv)))
+            graph.replay()
+            side.synchronize()
+            if i % 6 == 0 or i == n_steps - 1:
+                check(out.cpu().numpy(), q.cpu().numpy(), np.array([n + i for n in lens] + [-1]), [0, 1, 2, 0])
+    assert int(err) == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_bytes_do_not_depend_on_how_tokens_are_cut_into_calls(torch_cuda, fmt):
+    torch = torch_cuda
+    rng = np.random.default_rng(12)
+    M, hkv = 50, 8
+    k, v = dev(torch, _vectors(rng, M, 2, hkv)), dev(torch, _vectors(rng, M, 2, hkv))
+    pos, slot = dev(torch, np.arange(M, dtype=np.int32)), dev(torch, np.zeros(M, np.int32))
+    bt = dev(torch, np.array([[3, 0, 2, 1]], np.int32))
+    pools = []
+    for cuts in ([0, 50], [0, 1, 2, 17, 18, 40, 50]):
+        pool, err = torch.zeros((2, 4, hkv, P.TILE), dtype=torch.uint8, device="cuda"), _err(torch)
+        for a, b in zip(cuts, cuts[1:]):
+            _append(torch, k[a:b], v[a:b], P.F32, 2 * hkv * 128, b - a, 2, hkv, pos[a:b].contiguous(), slot, bt, 4,
+                    fmt, pool, err)
+        pools.append(pool)
+        assert int(err) == 0
+    assert torch.equal(*pools)
+
+
+def test_two_decode_calls_on_two_streams(torch_cuda):
+    """Calls with scratch of their own may overlap; results repeat bit for bit."""
+    torch = torch_cuda
+    rng = np.random.default_rng(13)
+    hq, hkv, lens = 16, 8, [900, 1200, 3]
+    pool, bt, n_pages = _filled(rng, lens, 1, hkv, P.INT8)
+    d_pool, d_bt = dev(torch, pool), dev(torch, bt)
+    pos, slot = dev(torch, np.array(lens, np.int32) - 1), dev(torch, np.arange(3, dtype=np.int32))
+    qs = [dev(torch, (rng.standard_normal((3, hq, 128)) * 0.3).astype(np.float32)) for _ in range(2)]
+    err = _err(torch)
+    alone = [_decode(torch, q, hq, hkv, pos, slot, d_bt, n_pages, P.INT8, d_pool, err) for q in qs]
+    outs = [torch.zeros((3, hq * 128), device="cuda") for _ in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    keep = []
+    for _ in range(20):
+        for s, q, o in zip(streams, qs, outs):
+            with torch.cuda.stream(s):
+                keep.append(_decode(torch, q, hq, hkv, pos, slot, d_bt, n_pages, P.INT8, d_pool, err, out=o))
+    torch.cuda.synchronize()
+    for a, b in zip(alone, outs):
+        assert torch.equal(a, b)
+    assert int(err) == 0
