@@ -6,8 +6,10 @@
 // with kq, vq the stored 8-bit values and dk, dv the scales of their vectors. The scales
 // multiply a score and a weight, never the 128 values.
 #include "k_kv8.cuh"
+#include "tc_common.cuh"
 #include "funasr_dec.h"
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -93,10 +95,538 @@ __device__ void attend_row(const Kv8AttnArgs& a, int m, int H, int lane) {
     for (int i = 0; i < 4; ++i) store_out(a, o + i, sum == 0.0f ? 0.0f : acc[i] / sum);
 }
 
+// ------------------------------------------------------------------ decode --
+// The pages of every (row, KV head), in that order, are one list of T pages; CTA c takes the
+// chunk [c, c + 1) * ceil(T / CTAs) of it, whatever rows that covers, so every CTA streams the
+// same number of pages however ragged the rows are. The part of a chunk that lies in one (row,
+// KV head) is a segment. A segment that holds all of its row's pages writes the output; any
+// other writes its un-normalised partial to scratch: at most two a CTA (a chunk's first and
+// last segment), and kv8_merge_kernel joins them.
+//
+// A CTA's four warps take its pages in turn, each through a ring of its own: lane 0 issues one
+// TMA box (32 rows of 128 B: K and V of the head in that page, 128 B swizzle) and one bulk copy
+// (their scales) per page. Per page of 16 tokens, on the tensor cores with the keys as the
+// 16-row operand (m16n8k16, f16 in, f32 sums):
+//   S[16 tokens][8 columns] = K . q     K expanded to f16 exactly; a query head is two columns,
+//                                       hi = f16(q') and lo = f16(q' - hi), q' = q scaled by a
+//                                       power of two to [2^10, 2^11): 22 bits of q
+//   softmax: lane (g, t) = (lane / 4, lane % 4) holds tokens g and g + 8 of head t; running
+//            maximum per head, sums per lane
+//   O[16 dims x 8][8 columns] += V^T . w   w = p dv as a hi / lo pair, scaled by a power of two
+//                                       that takes the page's largest dv to [2^10, 2^11)
+// The page's product starts from zero and is added to the running output by one f32 fma per
+// value, so the sum over pages is rounded to nearest.
+constexpr int kWarps = 4;
+constexpr int kCtasPerSm = 3;
+constexpr int kMaxCtas = 148 * kCtasPerSm;     // one resident wave of a B200
+
+template <int NT>
+constexpr int kStages = NT == 1 ? 4 : 3;
+
+template <int NT>
+struct DecodeSmem {
+    unsigned char tiles[kWarps][kStages<NT>][2 * kPartBytes];   // K then V, 128 B swizzle
+    float scales[kWarps][kStages<NT>][2 * kPageTokens];         // K then V
+    float acc[kWarps][4 * NT][D];
+    float2 ml[kWarps][4 * NT];                                  // running maximum (log2 units), sum
+    uint64_t bars[kWarps][kStages<NT>];
+    long long scan[kWarps];
+    int start[3];                                               // the chunk's first row, KV head, page
+};
+
+// Scratch: per CTA the place where its chunk begins, and two partials of every query head.
+struct Partials {
+    int4* begin;             // [CTAs] (row, KV head, page, pages of the row), row -1: no work
+    float2* ml;              // [CTAs][2][G]
+    float* o;                // [CTAs][2][G][128]
+    int* chunk;              // [1] pages of a chunk
+};
+__host__ __device__ inline size_t partial_bytes(int G) {
+    return (size_t)kMaxCtas * (sizeof(int4) + 2 * G * (sizeof(float2) + D * sizeof(float))) + 16;
+}
+__host__ __device__ inline Partials partials(void* scratch, int G) {
+    Partials p;
+    p.o = static_cast<float*>(scratch);
+    p.begin = reinterpret_cast<int4*>(p.o + (size_t)kMaxCtas * 2 * G * D);
+    p.ml = reinterpret_cast<float2*>(p.begin + kMaxCtas);
+    p.chunk = reinterpret_cast<int*>(p.ml + (size_t)kMaxCtas * 2 * G);
+    return p;
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+__device__ __forceinline__ uint32_t hi_lo(float x) {
+    const __half h = __float2half_rn(x);
+    const __half l = __float2half_rn(__fsub_rn(x, __half2float(h)));
+    return (uint32_t)__half_as_ushort(h) | ((uint32_t)__half_as_ushort(l) << 16);
+}
+
+// 2^10 / (the power of two at or below x), and its inverse, for finite x > 0.
+__device__ __forceinline__ float pow2_floor(float x) {
+    return __uint_as_float(max(__float_as_uint(x) & 0x7f800000u, 0x00800000u));
+}
+__device__ __forceinline__ float pow2_inverse(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
+
+// Stored values of two tokens (words a, b: four dims each) as f16 pairs (a_i, b_i).
 template <int FMT>
-__global__ void __launch_bounds__(128) kv8_decode_kernel(Kv8AttnArgs a) {
-    const int H = blockIdx.y * 4 + (threadIdx.x >> 5);
-    if (H < a.Hq) attend_row<FMT>(a, blockIdx.x, H, threadIdx.x & 31);
+__device__ __forceinline__ void expand_pairs(uint32_t a, uint32_t b, uint32_t (&v)[4]) {
+    if (FMT == kInt8) {
+        const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1152
+        const uint32_t lo = __byte_perm(a, b, 0x5140) ^ 0x80808080u, hi = __byte_perm(a, b, 0x7362) ^ 0x80808080u;
+        const uint32_t e[4] = {__byte_perm(lo, 0x64646464u, 0x4140), __byte_perm(lo, 0x64646464u, 0x4342),
+                               __byte_perm(hi, 0x64646464u, 0x4140), __byte_perm(hi, 0x64646464u, 0x4342)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = as_u32(__hsub2(*reinterpret_cast<const __half2*>(&e[i]), off));
+    } else {
+        __half2 x, y;
+        expand4<FMT>(__byte_perm(a, b, 0x5140), x, y);
+        v[0] = as_u32(x);
+        v[1] = as_u32(y);
+        expand4<FMT>(__byte_perm(a, b, 0x7362), x, y);
+        v[2] = as_u32(x);
+        v[3] = as_u32(y);
+    }
+}
+
+// Pages of row m; 0 for padding and for a row that cannot be served (flagged elsewhere).
+__device__ __forceinline__ bool row_bad(const Kv8AttnArgs& a, int m) {
+    const int pos = a.pos[m];
+    return pos < -1 || pos / kPageTokens >= a.bt_stride || (pos >= 0 && a.slot[m] < 0);
+}
+__device__ __forceinline__ int row_pages(const Kv8AttnArgs& a, int m) {
+    return row_bad(a, m) ? 0 : (a.pos[m] + kPageTokens) / kPageTokens;
+}
+
+// A place in the list of pages.
+struct Place {
+    int m, h, p, np;
+};
+__device__ __forceinline__ void next_item(const Kv8AttnArgs& a, Place& x) {
+    x.p = 0;
+    if (++x.h < a.Hkv) return;
+    x.h = 0;
+    do {
+        ++x.m;
+        x.np = x.m < a.M ? row_pages(a, x.m) : 1;
+    } while (x.np == 0);
+}
+__device__ __forceinline__ void advance(const Kv8AttnArgs& a, Place& x, int n) {
+    while (n >= x.np - x.p) {
+        n -= x.np - x.p;
+        next_item(a, x);
+        if (x.m >= a.M) return;
+    }
+    x.p += n;
+}
+
+template <int FMT, int NT>
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
+    kv8_decode_kernel(const __grid_constant__ CUtensorMap tm_pool, const Kv8AttnArgs a, void* scratch) {
+    constexpr int ST = kStages<NT>;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    DecodeSmem<NT>& S = *reinterpret_cast<DecodeSmem<NT>*>(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int g = lane >> 2, t = lane & 3;
+    const int G = a.Hq / a.Hkv;
+    const Partials part = partials(scratch, G);
+    pdl_trigger();
+
+    // the list's length, and where this CTA's chunk begins
+    if (tid == 0) {
+        tma_prefetch_desc(&tm_pool);
+        for (int w = 0; w < kWarps; ++w)
+            for (int s = 0; s < ST; ++s) mbar_init(&S.bars[w][s], 1);
+        fence_mbar_init();
+    }
+    const int per = (a.M + kWarps * 32 - 1) / (kWarps * 32);
+    const int r0 = min(tid * per, a.M), r1 = min(r0 + per, a.M);
+    long long mine = 0;
+    for (int m = r0; m < r1; ++m) mine += row_pages(a, m);
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) S.scan[warp] = incl;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) incl += S.scan[w];
+        total += S.scan[w];
+    }
+    total *= a.Hkv;
+    const int chunk = (int)((total + gridDim.x - 1) / gridDim.x);
+    const long long begin = (long long)blockIdx.x * chunk;
+    const int n = (int)min((long long)chunk, total - begin);      // <= 0: no work
+    long long before = (incl - mine) * a.Hkv;
+    if (n > 0 && before <= begin && begin < incl * a.Hkv) {
+        for (int m = r0; m < r1; ++m) {
+            const int np = row_pages(a, m);
+            if (begin < before + (long long)np * a.Hkv) {
+                S.start[0] = m;
+                S.start[1] = (int)((begin - before) / np);
+                S.start[2] = (int)((begin - before) % np);
+                break;
+            }
+            before += (long long)np * a.Hkv;
+        }
+    }
+    // rows without pages: padding is zeroed, a row that cannot be served is flagged and left
+    for (int m = blockIdx.x; m < a.M; m += gridDim.x) {
+        if (a.pos[m] == -1)
+            for (int d = tid; d < a.Hq * D; d += kWarps * 32) store_out(a, (size_t)m * a.Hq * D + d, 0.0f);
+        else if (tid == 0 && row_bad(a, m)) record_error(a.err, kDevErrBadLen);
+    }
+    __syncthreads();
+    Place at{-1, 0, 0, 0};
+    if (n > 0) {
+        at = Place{S.start[0], S.start[1], S.start[2], 0};
+        at.np = row_pages(a, at.m);
+    }
+    if (tid == 0) {
+        part.begin[blockIdx.x] = make_int4(at.m, at.h, at.p, at.np);
+        if (blockIdx.x == 0) *part.chunk = chunk;
+    }
+    if (n <= 0) return;
+
+    // the warp's pages: chunk indices warp, warp + 4, ...; lane l looks up its pages 32 b + l
+    // of batch b, a batch ahead
+    const int nw = n > warp ? (n - warp + kWarps - 1) / kWarps : 0;
+    Place ahead = at;
+    advance(a, ahead, warp + kWarps * lane);     // may run past the list: never looked up then
+    auto look_up = [&](int first, int& row, int& valid) {
+        row = 0;
+        valid = 0;
+        if (first + lane < nw) {
+            const int page = a.block_table[(size_t)a.slot[ahead.m] * a.bt_stride + ahead.p];
+            if (page >= 0 && page < a.n_pages) {
+                row = (page * a.Hkv + ahead.h) * (kTileBytes / 128);
+                valid = min(kPageTokens, a.pos[ahead.m] + 1 - ahead.p * kPageTokens);
+            } else {
+                record_error(a.err, kDevErrBadPage);             // its tokens are left out
+            }
+            if (first + 32 + lane < nw) advance(a, ahead, 32 * kWarps);
+        }
+    };
+    int row_a, valid_a, row_b, valid_b;
+    look_up(0, row_a, valid_a);
+    look_up(32, row_b, valid_b);
+    auto issue = [&](int i, int row) {           // lane 0
+        const int s = i % ST;
+        mbar_arrive_expect_tx(&S.bars[warp][s], kTileBytes);
+        tma_load_2d(S.tiles[warp][s], &tm_pool, 0, row, &S.bars[warp][s]);
+        bulk_copy_g2s(S.scales[warp][s], a.pool + (size_t)row * 128 + kScaleOff, 2 * kPageTokens * sizeof(float),
+                      &S.bars[warp][s]);
+    };
+#pragma unroll
+    for (int i = 0; i < ST; ++i) {
+        const int row = __shfl_sync(0xffffffffu, row_a, i);
+        if (lane == 0 && i < nw) issue(i, row);
+    }
+
+    bool ok = true;
+    int i = 0;                                   // the warp's pages done
+    for (int j = 0; j < n;) {
+        const int seg = min(at.np - at.p, n - j);                 // pages of this segment
+        // this warp's pages of it: chunk indices in [j, j + seg) that are warp mod 4
+        const int i_end = j + seg > warp ? (j + seg - warp + kWarps - 1) / kWarps : 0;
+
+        // the queries of the KV head: lane (g, t) holds column g = 2 * head + (lo part), dims
+        // [32 t, 32 t + 32) as the pairs of the MMA's rows 2t, 2t+1 and 2t+8, 2t+9 in eight steps
+        uint32_t qb[NT][8][2];
+        float qs[NT];                            // score of head t (+ 4): acc * qs in log2 units
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            const int head = 4 * c + (g >> 1);
+            float x[32];
+            float amax = 0.0f;
+            if (head < G && i < i_end) {
+                const float4* src =
+                    reinterpret_cast<const float4*>(a.q + ((size_t)at.m * a.Hq + at.h * G + head) * D + 32 * t);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float4 v = src[k];
+                    x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) x[k] = 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 32; ++k) amax = fmaxf(amax, fabsf(x[k]));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const float p2 = pow2_floor(amax);
+            const float up = pow2_inverse(p2);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = hi_lo(x[4 * k + e] * up * 1024.0f);
+                const uint32_t sel = (g & 1) ? 0x7632 : 0x5410;
+                qb[c][k][0] = __byte_perm(w[0], w[1], sel);
+                qb[c][k][1] = __byte_perm(w[2], w[3], sel);
+            }
+            // the factor of head t is with the lanes of columns 2t, 2t + 1
+            qs[c] = __shfl_sync(0xffffffffu, p2, 8 * t) * (kLog2e / 1024.0f);
+        }
+        float mx[NT], sum[NT], o[NT][16];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            mx[c] = -INFINITY;
+            sum[c] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[c][k] = 0.0f;
+        }
+
+        for (; i < i_end && ok; ++i) {
+            const int s = i % ST;
+            const int valid = __shfl_sync(0xffffffffu, valid_a, i & 31);
+            const bool got = mbar_wait_bounded(&S.bars[warp][s], (uint32_t)(i / ST) & 1u);
+            if (!__all_sync(0xffffffffu, got)) {
+                ok = false;
+                break;
+            }
+            const unsigned char* Kt = S.tiles[warp][s];
+            const unsigned char* Vt = Kt + kPartBytes;
+            // scores: K rows g and g + 8, dims 32 t .. (16 B chunks 2t, 2t + 1, swizzled by the row)
+            float sc[NT][4];
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[c][e] = 0.0f;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int off = ((2 * t + hf) ^ g) * 16;
+                const uint4 x = lds128(Kt + g * 128 + off), y = lds128(Kt + (g + 8) * 128 + off);
+                const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    __half2 x0, x1, y0, y1;
+                    expand4<FMT>(xw[e], x0, x1);
+                    expand4<FMT>(yw[e], y0, y1);
+                    const uint32_t fa[4] = {as_u32(x0), as_u32(y0), as_u32(x1), as_u32(y1)};
+#pragma unroll
+                    for (int c = 0; c < NT; ++c) mma16816(sc[c], fa, qb[c][4 * hf + e][0], qb[c][4 * hf + e][1]);
+                }
+            }
+            const float* scale = S.scales[warp][s];
+            const float k0 = scale[g], k1 = scale[g + 8];
+            const bool in0 = g < valid, in1 = g + 8 < valid;
+            const float v0 = in0 ? scale[kPageTokens + g] : 0.0f, v1 = in1 ? scale[kPageTokens + g + 8] : 0.0f;
+            // the power of two at the page's largest V scale
+            const float p2 = __uint_as_float(max(
+                __reduce_max_sync(0xffffffffu, max(__float_as_uint(v0), __float_as_uint(v1)) & 0x7f800000u),
+                0x00800000u));
+            const float inv = pow2_inverse(p2);
+            const float u0 = v0 * inv, u1 = v1 * inv, back = p2 * (1.0f / 1024.0f);
+            uint32_t w0[NT], w1[NT];
+            float alpha[NT];
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const float s0 = in0 ? (sc[c][0] + sc[c][1]) * (k0 * qs[c]) : -INFINITY;
+                const float s1 = in1 ? (sc[c][2] + sc[c][3]) * (k1 * qs[c]) : -INFINITY;
+                float top = fmaxf(s0, s1);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                top = fmaxf(top, mx[c]);
+                alpha[c] = mx[c] == top ? 1.0f : exp2f(mx[c] - top);
+                mx[c] = top;
+                const float p0 = in0 ? exp2f(s0 - top) : 0.0f, p1 = in1 ? exp2f(s1 - top) : 0.0f;
+                sum[c] = sum[c] * alpha[c] + (p0 + p1);
+                w0[c] = hi_lo(in0 ? p0 * u0 * 1024.0f : 0.0f);
+                w1[c] = hi_lo(in1 ? p1 * u1 * 1024.0f : 0.0f);
+            }
+            // weights as the second operand: column g = 2 * head + (lo part), tokens 2t, 2t+1, 2t+8, 2t+9
+            uint32_t wb[NT][2];
+            const uint32_t sel = (g & 1) ? 0x7632 : 0x5410;
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const int from = 8 * t + (g >> 1);
+                const uint32_t x0 = __shfl_sync(0xffffffffu, w0[c], from), y0 = __shfl_sync(0xffffffffu, w0[c], from + 4);
+                const uint32_t x1 = __shfl_sync(0xffffffffu, w1[c], from), y1 = __shfl_sync(0xffffffffu, w1[c], from + 4);
+                wb[c][0] = __byte_perm(x0, y0, sel);
+                wb[c][1] = __byte_perm(x1, y1, sel);
+            }
+            // V rows of those tokens, dims 16 g ..
+            uint32_t vw[4][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int tok = 2 * t + (e & 1) + 8 * (e >> 1);
+                const uint4 x = lds128(Vt + tok * 128 + ((g ^ (tok & 7)) * 16));
+                // bytes behind the last token may be e4m3 NaN, which a zero weight does not cancel
+                const bool live = FMT == kInt8 || tok < valid;
+                vw[e][0] = live ? x.x : 0u;
+                vw[e][1] = live ? x.y : 0u;
+                vw[e][2] = live ? x.z : 0u;
+                vw[e][3] = live ? x.w : 0u;
+            }
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {        // dims 16 g + 4 d ..
+                uint32_t lo[4], hi[4];
+                expand_pairs<FMT>(vw[0][d], vw[1][d], lo);
+                expand_pairs<FMT>(vw[2][d], vw[3][d], hi);
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const uint32_t fa[4] = {lo[e], lo[e + 1], hi[e], hi[e + 1]};
+#pragma unroll
+                    for (int c = 0; c < NT; ++c) {
+                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma16816(acc, fa, wb[c][0], wb[c][1]);
+                        float& oa = o[c][4 * d + e];
+                        float& ob = o[c][4 * d + e + 1];
+                        oa = fmaf(acc[0] + acc[1], back, oa * alpha[c]);
+                        ob = fmaf(acc[2] + acc[3], back, ob * alpha[c]);
+                    }
+                }
+            }
+            __syncwarp();
+            {
+                const int k = i + ST;
+                const int row = __shfl_sync(0xffffffffu, (k >> 5) == (i >> 5) ? row_a : row_b, k & 31);
+                if (lane == 0 && k < nw) {
+                    fence_proxy_async_smem();
+                    issue(k, row);
+                }
+            }
+            if ((i & 31) == 31) {
+                row_a = row_b;
+                valid_a = valid_b;
+                look_up(i + 33, row_b, valid_b);
+            }
+        }
+        if (!ok) {
+            // A wait gave up: flag it, wait (bounded again) for the warp's copies in flight and
+            // leave its part out.
+            if (lane == 0) record_error(a.err, kDevErrTimeout);
+            for (int k = i; k < min(i + ST, nw); ++k) {
+                const bool done = mbar_wait_bounded(&S.bars[warp][k % ST], (uint32_t)(k / ST) & 1u);
+                (void)__all_sync(0xffffffffu, done);
+            }
+            i = nw;
+        }
+        // the warps' parts of the segment, joined by 128 threads, one dim each
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            float l = sum[c];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            if (g == 0) S.ml[warp][4 * c + t] = ok ? make_float2(mx[c], l) : make_float2(-INFINITY, 0.0f);
+            float4* dst = reinterpret_cast<float4*>(&S.acc[warp][4 * c + t][16 * g]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                dst[k] = make_float4(o[c][4 * k], o[c][4 * k + 1], o[c][4 * k + 2], o[c][4 * k + 3]);
+        }
+        __syncthreads();
+        const bool whole = seg == at.np;
+        const int slot = 2 * blockIdx.x + (j == 0 ? 0 : 1);
+        for (int head = 0; head < G; ++head) {
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, S.ml[w][head].x);
+            float L = 0.0f, O = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float2 ml = S.ml[w][head];
+                // a part without a token (maximum -inf) holds zeros; one whose scores are all NaN, NaN
+                const float f = ml.x == M ? 1.0f : exp2f(ml.x - M);
+                L = fmaf(ml.y, f, L);
+                O = fmaf(S.acc[w][head][tid], f, O);
+            }
+            if (whole) {
+                store_out(a, ((size_t)at.m * a.Hq + at.h * G + head) * D + tid, L == 0.0f ? 0.0f : O / L);
+            } else {
+                part.o[((size_t)slot * G + head) * D + tid] = O;
+                if (tid == 0) part.ml[(size_t)slot * G + head] = make_float2(M, L);
+            }
+        }
+        __syncthreads();
+        j += seg;
+        if (j < n) next_item(a, at);
+    }
+}
+
+// Joins the partials of the (row, KV head)s that several chunks share: CTA c the one that
+// chunk c + 1 begins inside, if that is the first chunk to do so. Warp w of query head y takes
+// the chunks w, w + 8, ...; the warps' sums meet in shared memory.
+constexpr int kMergeWarps = 8;
+__global__ void __launch_bounds__(kMergeWarps * 32) kv8_merge_kernel(const Kv8AttnArgs a, void* scratch) {
+    __shared__ float4 s_o[kMergeWarps][32];
+    __shared__ float2 s_ml[kMergeWarps];
+    pdl_wait();
+    const int G = a.Hq / a.Hkv, head = blockIdx.y;
+    const Partials part = partials(scratch, G);
+    const int c = blockIdx.x + 1;
+    const int chunk = *part.chunk;
+    const int4 at = part.begin[c];
+    // pages [0, at.z) of the item lie before chunk c; the first chunk that begins inside it?
+    if (at.x < 0 || at.z == 0 || at.z > chunk) return;
+    const int n = 1 + (at.w - at.z + chunk - 1) / chunk;          // chunks that hold a part
+    const int first = 2 * (c - 1) + (at.z == chunk ? 0 : 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float M = -INFINITY;
+    for (int k = lane; k < n; k += 32) M = fmaxf(M, part.ml[(size_t)(k ? 2 * (c + k - 1) : first) * G + head].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float L = 0.0f;
+    float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int k = warp; k < n; k += kMergeWarps) {
+        const size_t i = (size_t)(k ? 2 * (c + k - 1) : first) * G + head;
+        const float2 ml = part.ml[i];
+        const float4 v = reinterpret_cast<const float4*>(part.o + i * D)[lane];
+        const float f = ml.x == M ? 1.0f : exp2f(ml.x - M);
+        L = fmaf(ml.y, f, L);
+        O.x = fmaf(v.x, f, O.x);
+        O.y = fmaf(v.y, f, O.y);
+        O.z = fmaf(v.z, f, O.z);
+        O.w = fmaf(v.w, f, O.w);
+    }
+    s_o[warp][lane] = O;
+    if (lane == 0) s_ml[warp].y = L;
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    L = 0.0f;
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) {
+        L += s_ml[w].y;
+        v += reinterpret_cast<const float*>(s_o[w])[threadIdx.x];
+    }
+    store_out(a, ((size_t)at.x * a.Hq + at.y * G + head) * D + threadIdx.x, L == 0.0f ? 0.0f : v / L);
+}
+
+template <int FMT, int NT>
+cudaError_t launch_decode(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scratch, int grid, cudaStream_t s) {
+    auto kern = kv8_decode_kernel<FMT, NT>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DecodeSmem<NT>));
+    if (e != cudaSuccess) return e;
+    kern<<<grid, kWarps * 32, sizeof(DecodeSmem<NT>), s>>>(tm, a, scratch);
+    if (grid == 1) return cudaGetLastError();
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    // launched while the decode kernel runs; it waits for that kernel's end before it reads
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid - 1, a.Hq / a.Hkv);
+    cfg.blockDim = dim3(kMergeWarps * 32);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv8_merge_kernel, a, scratch);
 }
 
 template <int FMT>
@@ -131,10 +661,17 @@ int check(const std::string& what, const Kv8AttnArgs& a, int format, const void*
                                (what + ": q, outputs and scratch must be 16-byte, pool 128-byte aligned").c_str());
     if (a.Hq > 65535 || (long long)a.bt_stride * kPageTokens > 0x7fffffffll)
         return report_op_error(FA_ERR_CAPACITY, (what + ": n_heads or bt_stride too large").c_str());
+    if ((long long)a.n_pages * a.Hkv * (kTileBytes / 128) > 0x7fffffffll)
+        return report_op_error(FA_ERR_CAPACITY, (what + ": the pool has too many pages").c_str());
     if (need && (!scratch || scratch_bytes < need))
         return report_op_error(FA_ERR_INVALID_ARG, (what + ": scratch of " + std::to_string(need) +
                                                     " bytes required").c_str());
     return FA_OK;
+}
+
+// The pool as rows of 128 bytes (33 a tile: 16 of K, 16 of V, the scales); a box is K and V.
+bool make_tile_map(CUtensorMap* tm, const void* pool, long long rows) {
+    return make_map(tm, pool, 64, rows, 64, 2 * kPageTokens, true);
 }
 
 int launched(const char* what) {
@@ -147,7 +684,8 @@ int launched(const char* what) {
 }  // namespace fa
 
 extern "C" FA_API size_t fa_op_attention_kv8_scratch_bytes(int M, int n_heads, int n_kv_heads) {
-    return M > 0 && n_heads > 0 && n_kv_heads > 0 ? 16 : 0;
+    if (M <= 0 || n_kv_heads <= 0 || n_heads < n_kv_heads || n_heads % n_kv_heads) return 0;
+    return fa::partial_bytes(n_heads / n_kv_heads);
 }
 
 extern "C" FA_API size_t fa_op_prefill_attention_kv8_scratch_bytes(int n_tiles, int n_heads, int n_kv_heads) {
@@ -166,10 +704,19 @@ extern "C" FA_API int fa_op_paged_attention_kv8(const float* q, int M, int n_hea
     if (int rc = check("fa_op_paged_attention_kv8", a, format, scratch, scratch_bytes,
                        fa_op_attention_kv8_scratch_bytes(M, n_heads, n_kv_heads)))
         return rc;
-    const dim3 grid(M, (n_heads + 3) / 4);
-    if (format == FA_KV8_INT8) kv8_decode_kernel<kInt8><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
-    else kv8_decode_kernel<kE4m3><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
-    return launched("fa_op_paged_attention_kv8");
+    CUtensorMap tm;
+    if (!make_tile_map(&tm, pool_layer, (long long)n_pages * n_kv_heads * (kTileBytes / 128)))
+        return report_op_error(FA_ERR_CUDA, "fa_op_paged_attention_kv8: cannot build the page-pool tensor map");
+    // no more CTAs than there can be pages
+    const int grid = (int)std::min<long long>((long long)M * n_kv_heads * bt_stride, kMaxCtas);
+    const bool wide = n_heads / n_kv_heads > 4;
+    const cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e;
+    if (format == FA_KV8_INT8) e = wide ? launch_decode<kInt8, 2>(tm, a, scratch, grid, st) : launch_decode<kInt8, 1>(tm, a, scratch, grid, st);
+    else e = wide ? launch_decode<kE4m3, 2>(tm, a, scratch, grid, st) : launch_decode<kE4m3, 1>(tm, a, scratch, grid, st);
+    if (e != cudaSuccess) cudaGetLastError();
+    return e == cudaSuccess ? FA_OK
+                            : report_op_error(FA_ERR_CUDA, (std::string("fa_op_paged_attention_kv8: ") + cudaGetErrorString(e)).c_str());
 }
 
 extern "C" FA_API int fa_op_prefill_attention_kv8(const float* q, int M, int n_heads, int n_kv_heads, const int* pos,
