@@ -49,6 +49,43 @@ __device__ __forceinline__ void store_out(const Kv8AttnArgs& a, size_t o, float 
     if (a.out32) a.out32[o] = v;
 }
 
+// N consecutive outputs x / l from offset o (a multiple of 4; of 8 for N = 16): 0 where no
+// token takes part (l = 0).
+template <int N>
+__device__ __forceinline__ void store_quotients(const Kv8AttnArgs& a, size_t o, const float (&x)[N], float l) {
+    float v[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = l == 0.0f ? 0.0f : x[k] / l;
+    if (a.out32) {
+#pragma unroll
+        for (int k = 0; k < N; k += 4)
+            *reinterpret_cast<float4*>(a.out32 + o + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+    }
+    if (a.out16) {
+#pragma unroll
+        for (int k = 0; k < N; k += 4) {
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const __half2 h = __floats2half2_rn(v[k + 2 * e], v[k + 2 * e + 1]);
+                const float2 f = __half22float2(h);
+                const __half2 r = __floats2half2_rn(__fsub_rn(v[k + 2 * e], f.x), __fsub_rn(v[k + 2 * e + 1], f.y));
+                hi[e] = *reinterpret_cast<const uint32_t*>(&h);
+                lo[e] = *reinterpret_cast<const uint32_t*>(&r);
+            }
+            *reinterpret_cast<uint2*>(a.out16 + o + k) = make_uint2(hi[0], hi[1]);
+            if (a.out16_lo) *reinterpret_cast<uint2*>(a.out16_lo + o + k) = make_uint2(lo[0], lo[1]);
+        }
+    }
+}
+__device__ __forceinline__ void store16(const Kv8AttnArgs& a, size_t o, const float (&x)[16], float l) {
+    store_quotients<16>(a, o, x, l);
+}
+__device__ __forceinline__ void store4(const Kv8AttnArgs& a, size_t o, float4 x, float l) {
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    store_quotients<4>(a, o, v, l);
+}
+
 // One query vector of one row by a warp, lane l holding dims 4l .. 4l+3.
 template <int FMT>
 __device__ void attend_row(const Kv8AttnArgs& a, int m, int H, int lane) {
@@ -96,15 +133,15 @@ __device__ void attend_row(const Kv8AttnArgs& a, int m, int H, int lane) {
 }
 
 // ------------------------------------------------------------------ decode --
-// The pages of every (row, KV head), in that order, are one list of T pages; CTA c takes the
-// chunk [c, c + 1) * ceil(T / CTAs) of it, whatever rows that covers, so every CTA streams the
-// same number of pages however ragged the rows are. The part of a chunk that lies in one (row,
-// KV head) is a segment. A segment that holds all of its row's pages writes the output; any
-// other writes its un-normalised partial to scratch: at most two a CTA (a chunk's first and
-// last segment), and kv8_merge_kernel joins them.
+// The (row, KV head)s, in that order, are one list of units, a unit per page and kItemUnits
+// more for the cost of beginning one; every warp of the grid takes ceil(units / warps) of them,
+// whatever rows they cover, so all warps stream the same number of pages however ragged the
+// rows are. The part of a warp's range in one (row, KV head) is a segment; one that holds all
+// of its row's pages writes the output. The others are at most two a warp (its first and its
+// last): the CTA joins those of its four warps, and what it shares with other CTAs, again at
+// most two partials, goes to scratch un-normalised and is joined by kv8_merge_kernel.
 //
-// A CTA's four warps take its pages in turn, each through a ring of its own: lane 0 issues one
-// TMA box (32 rows of 128 B: K and V of the head in that page, 128 B swizzle) and one bulk copy
+// A warp streams its pages through a ring of its own: lane 0 issues one TMA box (32 rows of 128 B: K and V of the head in that page, 128 B swizzle) and one bulk copy
 // (their scales) per page. Per page of 16 tokens, on the tensor cores with the keys as the
 // 16-row operand (m16n8k16, f16 in, f32 sums):
 //   S[16 tokens][8 columns] = K . q     K expanded to f16 exactly; a query head is two columns,
@@ -119,6 +156,7 @@ __device__ void attend_row(const Kv8AttnArgs& a, int m, int H, int lane) {
 constexpr int kWarps = 4;
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 148 * kCtasPerSm;     // one resident wave of a B200
+constexpr int kItemUnits = 2;
 
 template <int NT>
 constexpr int kStages = NT == 1 ? 4 : 3;
@@ -127,19 +165,22 @@ template <int NT>
 struct DecodeSmem {
     unsigned char tiles[kWarps][kStages<NT>][2 * kPartBytes];   // K then V, 128 B swizzle
     float scales[kWarps][kStages<NT>][2 * kPageTokens];         // K then V
+    // the warps' first partials; their last ones go over the warp's ring once it is drained
     float acc[kWarps][4 * NT][D];
-    float2 ml[kWarps][4 * NT];                                  // running maximum (log2 units), sum
+    float2 ml[kWarps][2][4 * NT];                               // running maximum (log2 units), sum
+    int4 item[kWarps][2];                                       // (row, KV head, first page, pages), row -1: none
     uint64_t bars[kWarps][kStages<NT>];
     long long scan[kWarps];
-    int start[3];                                               // the chunk's first row, KV head, page
+    int np[kWarps][2];
+    int start[3];                                               // the CTA's first row, KV head, unit
 };
 
-// Scratch: per CTA the place where its chunk begins, and two partials of every query head.
+// Scratch: per CTA the place where its units begin, and two partials of every query head.
 struct Partials {
-    int4* begin;             // [CTAs] (row, KV head, page, pages of the row), row -1: no work
+    int4* begin;             // [CTAs] (row, KV head, unit, pages of the row), row -1: no work
     float2* ml;              // [CTAs][2][G]
     float* o;                // [CTAs][2][G][128]
-    int* chunk;              // [1] pages of a chunk
+    int* chunk;              // [1] units of a CTA
 };
 __host__ __device__ inline size_t partial_bytes(int G) {
     return (size_t)kMaxCtas * (sizeof(int4) + 2 * G * (sizeof(float2) + D * sizeof(float))) + 16;
@@ -204,12 +245,12 @@ __device__ __forceinline__ int row_pages(const Kv8AttnArgs& a, int m) {
     return row_bad(a, m) ? 0 : (a.pos[m] + kPageTokens) / kPageTokens;
 }
 
-// A place in the list of pages.
+// A place in the list: unit u of (row m, KV head h), whose first np units are its pages.
 struct Place {
-    int m, h, p, np;
+    int m, h, u, np;
 };
 __device__ __forceinline__ void next_item(const Kv8AttnArgs& a, Place& x) {
-    x.p = 0;
+    x.u = 0;
     if (++x.h < a.Hkv) return;
     x.h = 0;
     do {
@@ -217,13 +258,21 @@ __device__ __forceinline__ void next_item(const Kv8AttnArgs& a, Place& x) {
         x.np = x.m < a.M ? row_pages(a, x.m) : 1;
     } while (x.np == 0);
 }
-__device__ __forceinline__ void advance(const Kv8AttnArgs& a, Place& x, int n) {
-    while (n >= x.np - x.p) {
-        n -= x.np - x.p;
+// n units on (past the list's end: m >= M)
+__device__ __forceinline__ void skip_units(const Kv8AttnArgs& a, Place& x, int n) {
+    while (x.m < a.M && n >= x.np + kItemUnits - x.u) {
+        n -= x.np + kItemUnits - x.u;
         next_item(a, x);
-        if (x.m >= a.M) return;
     }
-    x.p += n;
+    x.u += n;
+}
+// n pages on; x is a page, and at least n more follow
+__device__ __forceinline__ void skip_pages(const Kv8AttnArgs& a, Place& x, int n) {
+    while (n >= x.np - x.u) {
+        n -= x.np - x.u;
+        next_item(a, x);
+    }
+    x.u += n;
 }
 
 template <int FMT, int NT>
@@ -248,7 +297,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     const int per = (a.M + kWarps * 32 - 1) / (kWarps * 32);
     const int r0 = min(tid * per, a.M), r1 = min(r0 + per, a.M);
     long long mine = 0;
-    for (int m = r0; m < r1; ++m) mine += row_pages(a, m);
+    for (int m = r0; m < r1; ++m) {
+        const int np = row_pages(a, m);
+        mine += np ? np + kItemUnits : 0;
+    }
     long long incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -264,20 +316,20 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
         total += S.scan[w];
     }
     total *= a.Hkv;
-    const int chunk = (int)((total + gridDim.x - 1) / gridDim.x);
-    const long long begin = (long long)blockIdx.x * chunk;
-    const int n = (int)min((long long)chunk, total - begin);      // <= 0: no work
+    const int per_warp = (int)((total + gridDim.x * kWarps - 1) / (gridDim.x * kWarps));
+    const long long begin = (long long)blockIdx.x * kWarps * per_warp;
+    const bool work = begin < total;
     long long before = (incl - mine) * a.Hkv;
-    if (n > 0 && before <= begin && begin < incl * a.Hkv) {
+    if (work && before <= begin && begin < incl * a.Hkv) {
         for (int m = r0; m < r1; ++m) {
-            const int np = row_pages(a, m);
-            if (begin < before + (long long)np * a.Hkv) {
+            const int np = row_pages(a, m), units = np ? np + kItemUnits : 0;
+            if (begin < before + (long long)units * a.Hkv) {
                 S.start[0] = m;
-                S.start[1] = (int)((begin - before) / np);
-                S.start[2] = (int)((begin - before) % np);
+                S.start[1] = (int)((begin - before) / units);
+                S.start[2] = (int)((begin - before) % units);
                 break;
             }
-            before += (long long)np * a.Hkv;
+            before += (long long)units * a.Hkv;
         }
     }
     // rows without pages: padding is zeroed, a row that cannot be served is flagged and left
@@ -288,33 +340,42 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     }
     __syncthreads();
     Place at{-1, 0, 0, 0};
-    if (n > 0) {
+    if (work) {
         at = Place{S.start[0], S.start[1], S.start[2], 0};
         at.np = row_pages(a, at.m);
     }
     if (tid == 0) {
-        part.begin[blockIdx.x] = make_int4(at.m, at.h, at.p, at.np);
-        if (blockIdx.x == 0) *part.chunk = chunk;
+        part.begin[blockIdx.x] = make_int4(at.m, at.h, at.u, at.np);
+        if (blockIdx.x == 0) *part.chunk = kWarps * per_warp;
     }
-    if (n <= 0) return;
+    if (!work) return;
 
-    // the warp's pages: chunk indices warp, warp + 4, ...; lane l looks up its pages 32 b + l
-    // of batch b, a batch ahead
-    const int nw = n > warp ? (n - warp + kWarps - 1) / kWarps : 0;
+    // the warp's range: per_warp units from `at`, nw pages among them
+    skip_units(a, at, warp * per_warp);
+    int nw = 0;
+    {
+        Place x = at;
+        for (int left = per_warp; left > 0 && x.m < a.M; next_item(a, x)) {
+            nw += max(0, min(x.np - x.u, left));
+            left -= min(left, x.np + kItemUnits - x.u);
+        }
+    }
+    if (nw > 0 && at.u >= at.np) next_item(a, at);                // begins in the units behind an item's pages
+    // lane l looks up its pages 32 b + l of batch b, a batch ahead
     Place ahead = at;
-    advance(a, ahead, warp + kWarps * lane);     // may run past the list: never looked up then
+    if (lane < nw) skip_pages(a, ahead, lane);
     auto look_up = [&](int first, int& row, int& valid) {
         row = 0;
         valid = 0;
         if (first + lane < nw) {
-            const int page = a.block_table[(size_t)a.slot[ahead.m] * a.bt_stride + ahead.p];
+            const int page = a.block_table[(size_t)a.slot[ahead.m] * a.bt_stride + ahead.u];
             if (page >= 0 && page < a.n_pages) {
                 row = (page * a.Hkv + ahead.h) * (kTileBytes / 128);
-                valid = min(kPageTokens, a.pos[ahead.m] + 1 - ahead.p * kPageTokens);
+                valid = min(kPageTokens, a.pos[ahead.m] + 1 - ahead.u * kPageTokens);
             } else {
                 record_error(a.err, kDevErrBadPage);             // its tokens are left out
             }
-            if (first + 32 + lane < nw) advance(a, ahead, 32 * kWarps);
+            if (first + 32 + lane < nw) skip_pages(a, ahead, 32);
         }
     };
     int row_a, valid_a, row_b, valid_b;
@@ -332,13 +393,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
         const int row = __shfl_sync(0xffffffffu, row_a, i);
         if (lane == 0 && i < nw) issue(i, row);
     }
+    if (lane < 2) S.item[warp][lane] = make_int4(-1, 0, 0, 0);
+    __syncwarp();
 
     bool ok = true;
     int i = 0;                                   // the warp's pages done
-    for (int j = 0; j < n;) {
-        const int seg = min(at.np - at.p, n - j);                 // pages of this segment
-        // this warp's pages of it: chunk indices in [j, j + seg) that are warp mod 4
-        const int i_end = j + seg > warp ? (j + seg - warp + kWarps - 1) / kWarps : 0;
+    while (i < nw) {
+        const int seg = min(at.np - at.u, nw - i);                // pages of this segment
+        const int i_end = i + seg, p_begin = at.u;
 
         // the queries of the KV head: lane (g, t) holds column g = 2 * head + (lo part), dims
         // [32 t, 32 t + 32) as the pairs of the MMA's rows 2t, 2t+1 and 2t+8, 2t+9 in eight steps
@@ -349,7 +411,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
             const int head = 4 * c + (g >> 1);
             float x[32];
             float amax = 0.0f;
-            if (head < G && i < i_end) {
+            if (head < G) {
                 const float4* src =
                     reinterpret_cast<const float4*>(a.q + ((size_t)at.m * a.Hq + at.h * G + head) * D + 32 * t);
 #pragma unroll
@@ -514,52 +576,96 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
                 (void)__all_sync(0xffffffffu, done);
             }
             i = nw;
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                mx[c] = -INFINITY;
+                sum[c] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[c][k] = 0.0f;
+            }
         }
-        // the warps' parts of the segment, joined by 128 threads, one dim each
+        // lane (g, t): sum of head t, its dims [16 g, 16 g + 16)
+        const bool whole = seg == at.np;
+        const int which = i_end == seg ? 0 : 1;                   // the warp's first segment, or its last
+        float* to = which ? reinterpret_cast<float*>(S.tiles[warp][0]) : &S.acc[warp][0][0];
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
             float l = sum[c];
             l += __shfl_xor_sync(0xffffffffu, l, 4);
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);
-            if (g == 0) S.ml[warp][4 * c + t] = ok ? make_float2(mx[c], l) : make_float2(-INFINITY, 0.0f);
-            float4* dst = reinterpret_cast<float4*>(&S.acc[warp][4 * c + t][16 * g]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                dst[k] = make_float4(o[c][4 * k], o[c][4 * k + 1], o[c][4 * k + 2], o[c][4 * k + 3]);
-        }
-        __syncthreads();
-        const bool whole = seg == at.np;
-        const int slot = 2 * blockIdx.x + (j == 0 ? 0 : 1);
-        for (int head = 0; head < G; ++head) {
-            float M = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, S.ml[w][head].x);
-            float L = 0.0f, O = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float2 ml = S.ml[w][head];
-                // a part without a token (maximum -inf) holds zeros; one whose scores are all NaN, NaN
-                const float f = ml.x == M ? 1.0f : exp2f(ml.x - M);
-                L = fmaf(ml.y, f, L);
-                O = fmaf(S.acc[w][head][tid], f, O);
-            }
+            const int head = 4 * c + t;
             if (whole) {
-                store_out(a, ((size_t)at.m * a.Hq + at.h * G + head) * D + tid, L == 0.0f ? 0.0f : O / L);
+                if (head < G) store16(a, ((size_t)at.m * a.Hq + at.h * G + head) * D + 16 * g, o[c], l);
             } else {
-                part.o[((size_t)slot * G + head) * D + tid] = O;
-                if (tid == 0) part.ml[(size_t)slot * G + head] = make_float2(M, L);
+                if (g == 0) S.ml[warp][which][head] = make_float2(mx[c], l);
+                float4* dst = reinterpret_cast<float4*>(to + head * D + 16 * g);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    dst[k] = make_float4(o[c][4 * k], o[c][4 * k + 1], o[c][4 * k + 2], o[c][4 * k + 3]);
             }
         }
-        __syncthreads();
-        j += seg;
-        if (j < n) next_item(a, at);
+        if (!whole && lane == 0) {
+            S.item[warp][which] = make_int4(at.m, at.h, p_begin, seg);
+            S.np[warp][which] = at.np;
+        }
+        if (i < nw) next_item(a, at);
+    }
+
+    // the warps' partials in list order: those of one (row, KV head) are neighbours; warp w
+    // joins heads w, w + 4, lane l dims [4 l, 4 l + 4)
+    __syncthreads();
+    for (int head = warp; head < G; head += kWarps) {
+        int4 run = make_int4(-1, 0, 0, 0);
+        int np = 0;
+        float M = -INFINITY, L = 0.0f;
+        float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        auto flush = [&]() {
+            if (run.x < 0) return;
+            if (run.w == np) {
+                store4(a, ((size_t)run.x * a.Hq + run.y * G + head) * D + 4 * lane, O, L);
+                return;
+            }
+            // the CTA's own beginning goes to its first slot, an item that it begins and does not end to its second
+            const bool at_begin = run.z > 0 || (run.x == S.start[0] && run.y == S.start[1] && S.start[2] == 0);
+            const size_t slot = ((size_t)2 * blockIdx.x + (at_begin ? 0 : 1)) * G + head;
+            reinterpret_cast<float4*>(part.o + slot * D)[lane] = O;
+            if (lane == 0) part.ml[slot] = make_float2(M, L);
+        };
+#pragma unroll 1
+        for (int k = 0; k < 2 * kWarps; ++k) {
+            const int w = k >> 1, which = k & 1;
+            const int4 it = S.item[w][which];
+            if (it.x < 0) continue;
+            if (it.x != run.x || it.y != run.y) {
+                flush();
+                run = make_int4(it.x, it.y, it.z, 0);
+                np = S.np[w][which];
+                M = -INFINITY;
+                L = 0.0f;
+                O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+            run.w += it.w;
+            const float* from = which ? reinterpret_cast<const float*>(S.tiles[w][0]) : &S.acc[w][0][0];
+            const float4 v = reinterpret_cast<const float4*>(from + head * D)[lane];
+            const float2 ml = S.ml[w][which][head];
+            // a part without a token (maximum -inf) holds zeros; one whose scores are all NaN, NaN
+            const float top = fmaxf(M, ml.x);
+            const float f0 = M == top ? 1.0f : exp2f(M - top), f1 = ml.x == top ? 1.0f : exp2f(ml.x - top);
+            M = top;
+            L = fmaf(ml.y, f1, L * f0);
+            O.x = fmaf(v.x, f1, O.x * f0);
+            O.y = fmaf(v.y, f1, O.y * f0);
+            O.z = fmaf(v.z, f1, O.z * f0);
+            O.w = fmaf(v.w, f1, O.w * f0);
+        }
+        flush();
     }
 }
 
-// Joins the partials of the (row, KV head)s that several chunks share: CTA c the one that
-// chunk c + 1 begins inside, if that is the first chunk to do so. Warp w of query head y takes
-// the chunks w, w + 8, ...; the warps' sums meet in shared memory.
+// Joins the partials of the (row, KV head)s that several CTAs of the decode kernel share: CTA
+// c - 1 the one among whose pages CTA c began, if c is the first to do so. Warp w of query head
+// y takes the partials w, w + 8, ...; the warps' sums meet in shared memory.
 constexpr int kMergeWarps = 8;
 __global__ void __launch_bounds__(kMergeWarps * 32) kv8_merge_kernel(const Kv8AttnArgs a, void* scratch) {
     __shared__ float4 s_o[kMergeWarps][32];
@@ -570,9 +676,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv8_merge_kernel(const Kv8At
     const int c = blockIdx.x + 1;
     const int chunk = *part.chunk;
     const int4 at = part.begin[c];
-    // pages [0, at.z) of the item lie before chunk c; the first chunk that begins inside it?
-    if (at.x < 0 || at.z == 0 || at.z > chunk) return;
-    const int n = 1 + (at.w - at.z + chunk - 1) / chunk;          // chunks that hold a part
+    // units [0, at.z) of the item lie before CTA c; the first CTA that begins among its pages?
+    if (at.x < 0 || at.z == 0 || at.z > chunk || at.z >= at.w) return;
+    const int n = 1 + (at.w - at.z + chunk - 1) / chunk;          // CTAs that hold a part
     const int first = 2 * (c - 1) + (at.z == chunk ? 0 : 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float M = -INFINITY;
