@@ -146,7 +146,7 @@ __device__ void attend_row(const Kv8AttnArgs& a, int m, int H, int lane) {
 // 16-row operand (m16n8k16, f16 in, f32 sums):
 //   S[16 tokens][8 columns] = K . q     K expanded to f16 exactly; a query head is two columns,
 //                                       hi = f16(q') and lo = f16(q' - hi), q' = q scaled by a
-//                                       power of two to [2^10, 2^11): 22 bits of q
+//                                       power of two to [1, 2): 22 bits of q
 //   softmax: lane (g, t) = (lane / 4, lane % 4) holds tokens g and g + 8 of head t; running
 //            maximum per head, sums per lane
 //   O[16 dims x 8][8 columns] += V^T . w   w = p dv as a hi / lo pair, scaled by a power of two
@@ -209,9 +209,9 @@ __device__ __forceinline__ uint32_t hi_lo(float x) {
     return (uint32_t)__half_as_ushort(h) | ((uint32_t)__half_as_ushort(l) << 16);
 }
 
-// 2^10 / (the power of two at or below x), and its inverse, for finite x > 0.
+// The power of two at or below x, within 2^-126 .. 2^126, and the inverse of such a one.
 __device__ __forceinline__ float pow2_floor(float x) {
-    return __uint_as_float(max(__float_as_uint(x) & 0x7f800000u, 0x00800000u));
+    return __uint_as_float(min(max(__float_as_uint(x) & 0x7f800000u, 0x00800000u), 0x7e800000u));
 }
 __device__ __forceinline__ float pow2_inverse(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
 
@@ -245,6 +245,13 @@ __device__ __forceinline__ int row_pages(const Kv8AttnArgs& a, int m) {
     return row_bad(a, m) ? 0 : (a.pos[m] + kPageTokens) / kPageTokens;
 }
 
+// Quotients of non-negative numbers, in 32 bits where they fit (a 64-bit division is a call
+// of a few hundred cycles, on every CTA's way to its first load).
+__device__ __forceinline__ long long floor_div(long long x, int y) {
+    return x >> 32 ? x / y : (long long)((uint32_t)x / (uint32_t)y);
+}
+__device__ __forceinline__ long long ceil_div(long long x, int y) { return floor_div(x + y - 1, y); }
+
 // A place in the list: unit u of (row m, KV head h), whose first np units are its pages.
 struct Place {
     int m, h, u, np;
@@ -273,6 +280,41 @@ __device__ __forceinline__ void skip_pages(const Kv8AttnArgs& a, Place& x, int n
         next_item(a, x);
     }
     x.u += n;
+}
+
+// The queries of a KV head: lane (g, t) holds column g = 2 * head + (lo part), dims [32 t,
+// 32 t + 32) as the MMA's rows 2t, 2t+1 and 2t+8, 2t+9 in eight steps. Heads from G on: zeros.
+__device__ __forceinline__ void load_query(const Kv8AttnArgs& a, const Place& at, int G, int head, int t,
+                                           float (&x)[32]) {
+    const float4* src = reinterpret_cast<const float4*>(a.q + ((size_t)at.m * a.Hq + at.h * G + head) * D + 32 * t);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float4 v = head < G ? src[k] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        x[4 * k] = v.x;
+        x[4 * k + 1] = v.y;
+        x[4 * k + 2] = v.z;
+        x[4 * k + 3] = v.w;
+    }
+}
+// The f16 pair of a query scaled by a power of two to [1, 2): hi rounds to 11 bits, lo to
+// 2^-25 of the largest value; a column keeps one of the two. Returns the factor that takes
+// head t's scores to log2 units.
+__device__ __forceinline__ float split_query(const float (&x)[32], int g, int t, uint32_t (&b)[8][2]) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) amax = fmaxf(amax, fabsf(x[k]));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const float p2 = pow2_floor(amax), up = pow2_inverse(p2);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const float y0 = x[2 * k] * up, y1 = x[2 * k + 1] * up;
+        const __half2 hi = __floats2half2_rn(y0, y1);
+        const float2 f = __half22float2(hi);
+        const __half2 lo = __floats2half2_rn(__fsub_rn(y0, f.x), __fsub_rn(y1, f.y));
+        b[k >> 1][k & 1] = (g & 1) ? as_u32(lo) : as_u32(hi);
+    }
+    return __shfl_sync(0xffffffffu, p2, 8 * t) * kLog2e;          // held by the lanes of columns 2t, 2t + 1
 }
 
 template <int FMT, int NT>
@@ -316,7 +358,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
         total += S.scan[w];
     }
     total *= a.Hkv;
-    const int per_warp = (int)((total + gridDim.x * kWarps - 1) / (gridDim.x * kWarps));
+    const int per_warp = (int)ceil_div(total, gridDim.x * kWarps);
     const long long begin = (long long)blockIdx.x * kWarps * per_warp;
     const bool work = begin < total;
     long long before = (incl - mine) * a.Hkv;
@@ -324,9 +366,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
         for (int m = r0; m < r1; ++m) {
             const int np = row_pages(a, m), units = np ? np + kItemUnits : 0;
             if (begin < before + (long long)units * a.Hkv) {
+                const int h = (int)floor_div(begin - before, units);
                 S.start[0] = m;
-                S.start[1] = (int)((begin - before) / units);
-                S.start[2] = (int)((begin - before) % units);
+                S.start[1] = h;
+                S.start[2] = (int)(begin - before - (long long)h * units);
                 break;
             }
             before += (long long)units * a.Hkv;
@@ -361,6 +404,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
         }
     }
     if (nw > 0 && at.u >= at.np) next_item(a, at);                // begins in the units behind an item's pages
+    float qx[NT][32];                            // the first item's queries, under way while its pages are looked up
+#pragma unroll
+    for (int c = 0; c < NT; ++c) load_query(a, at, nw > 0 ? G : 0, 4 * c + (g >> 1), t, qx[c]);
     // lane l looks up its pages 32 b + l of batch b, a batch ahead
     Place ahead = at;
     if (lane < nw) skip_pages(a, ahead, lane);
@@ -402,44 +448,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
         const int seg = min(at.np - at.u, nw - i);                // pages of this segment
         const int i_end = i + seg, p_begin = at.u;
 
-        // the queries of the KV head: lane (g, t) holds column g = 2 * head + (lo part), dims
-        // [32 t, 32 t + 32) as the pairs of the MMA's rows 2t, 2t+1 and 2t+8, 2t+9 in eight steps
         uint32_t qb[NT][8][2];
         float qs[NT];                            // score of head t (+ 4): acc * qs in log2 units
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
-            const int head = 4 * c + (g >> 1);
-            float x[32];
-            float amax = 0.0f;
-            if (head < G) {
-                const float4* src =
-                    reinterpret_cast<const float4*>(a.q + ((size_t)at.m * a.Hq + at.h * G + head) * D + 32 * t);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float4 v = src[k];
-                    x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 32; ++k) x[k] = 0.0f;
-            }
-#pragma unroll
-            for (int k = 0; k < 32; ++k) amax = fmaxf(amax, fabsf(x[k]));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const float p2 = pow2_floor(amax);
-            const float up = pow2_inverse(p2);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = hi_lo(x[4 * k + e] * up * 1024.0f);
-                const uint32_t sel = (g & 1) ? 0x7632 : 0x5410;
-                qb[c][k][0] = __byte_perm(w[0], w[1], sel);
-                qb[c][k][1] = __byte_perm(w[2], w[3], sel);
-            }
-            // the factor of head t is with the lanes of columns 2t, 2t + 1
-            qs[c] = __shfl_sync(0xffffffffu, p2, 8 * t) * (kLog2e / 1024.0f);
+            if (i > 0) load_query(a, at, G, 4 * c + (g >> 1), t, qx[c]);
+            qs[c] = split_query(qx[c], g, t, qb[c]);
         }
         float mx[NT], sum[NT], o[NT][16];
 #pragma unroll
@@ -485,12 +499,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
             const float k0 = scale[g], k1 = scale[g + 8];
             const bool in0 = g < valid, in1 = g + 8 < valid;
             const float v0 = in0 ? scale[kPageTokens + g] : 0.0f, v1 = in1 ? scale[kPageTokens + g + 8] : 0.0f;
-            // the power of two at the page's largest V scale
-            const float p2 = __uint_as_float(max(
-                __reduce_max_sync(0xffffffffu, max(__float_as_uint(v0), __float_as_uint(v1)) & 0x7f800000u),
-                0x00800000u));
-            const float inv = pow2_inverse(p2);
-            const float u0 = v0 * inv, u1 = v1 * inv, back = p2 * (1.0f / 1024.0f);
+            // the power of two at the page's largest V scale, over 2^10
+            const float back = __uint_as_float(
+                max(__reduce_max_sync(0xffffffffu, max(__float_as_uint(v0), __float_as_uint(v1)) & 0x7f800000u),
+                    11u << 23) - (10u << 23));
+            const float inv = pow2_inverse(back);
+            const float u0 = v0 * inv, u1 = v1 * inv;
             uint32_t w0[NT], w1[NT];
             float alpha[NT];
 #pragma unroll
@@ -506,8 +520,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
                 mx[c] = top;
                 const float p0 = in0 ? exp2f(s0 - top) : 0.0f, p1 = in1 ? exp2f(s1 - top) : 0.0f;
                 sum[c] = sum[c] * alpha[c] + (p0 + p1);
-                w0[c] = hi_lo(in0 ? p0 * u0 * 1024.0f : 0.0f);
-                w1[c] = hi_lo(in1 ? p1 * u1 * 1024.0f : 0.0f);
+                w0[c] = hi_lo(in0 ? p0 * u0 : 0.0f);
+                w1[c] = hi_lo(in1 ? p1 * u1 : 0.0f);
             }
             // weights as the second operand: column g = 2 * head + (lo part), tokens 2t, 2t+1, 2t+8, 2t+9
             uint32_t wb[NT][2];
@@ -612,105 +626,165 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
         if (i < nw) next_item(a, at);
     }
 
-    // the warps' partials in list order: those of one (row, KV head) are neighbours; warp w
-    // joins heads w, w + 4, lane l dims [4 l, 4 l + 4)
+    // The warps' partials in list order, lane k the k-th: those of one (row, KV head) are
+    // neighbours, a run. Warp w joins the runs of heads w, w + kWarps, ..., lane l dims 4 l ..
     __syncthreads();
+    static_assert(2 * kWarps <= 32, "a lane per partial");
+    int4 it = make_int4(-1, 0, 0, 0);
+    int np = 0;
+    if (lane < 2 * kWarps) {
+        it = S.item[lane >> 1][lane & 1];
+        np = S.np[lane >> 1][lane & 1];
+    }
+    const uint32_t parts = __ballot_sync(0xffffffffu, it.x >= 0);
     for (int head = warp; head < G; head += kWarps) {
-        int4 run = make_int4(-1, 0, 0, 0);
-        int np = 0;
-        float M = -INFINITY, L = 0.0f;
-        float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        auto flush = [&]() {
-            if (run.x < 0) return;
-            if (run.w == np) {
-                store4(a, ((size_t)run.x * a.Hq + run.y * G + head) * D + 4 * lane, O, L);
-                return;
-            }
-            // the CTA's own beginning goes to its first slot, an item that it begins and does not end to its second
-            const bool at_begin = run.z > 0 || (run.x == S.start[0] && run.y == S.start[1] && S.start[2] == 0);
-            const size_t slot = ((size_t)2 * blockIdx.x + (at_begin ? 0 : 1)) * G + head;
-            reinterpret_cast<float4*>(part.o + slot * D)[lane] = O;
-            if (lane == 0) part.ml[slot] = make_float2(M, L);
-        };
-#pragma unroll 1
-        for (int k = 0; k < 2 * kWarps; ++k) {
-            const int w = k >> 1, which = k & 1;
-            const int4 it = S.item[w][which];
-            if (it.x < 0) continue;
-            if (it.x != run.x || it.y != run.y) {
-                flush();
-                run = make_int4(it.x, it.y, it.z, 0);
-                np = S.np[w][which];
-                M = -INFINITY;
-                L = 0.0f;
-                O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            }
-            run.w += it.w;
-            const float* from = which ? reinterpret_cast<const float*>(S.tiles[w][0]) : &S.acc[w][0][0];
-            const float4 v = reinterpret_cast<const float4*>(from + head * D)[lane];
-            const float2 ml = S.ml[w][which][head];
+        const float2 ml = it.x >= 0 ? S.ml[lane >> 1][lane & 1][head] : make_float2(-INFINITY, 0.0f);
+        for (uint32_t todo = parts; todo;) {
+            const int k0 = __ffs(todo) - 1;
+            const int m = __shfl_sync(0xffffffffu, it.x, k0), h = __shfl_sync(0xffffffffu, it.y, k0);
+            const int p0 = __shfl_sync(0xffffffffu, it.z, k0), pages = __shfl_sync(0xffffffffu, np, k0);
+            const bool in_run = it.x == m && it.y == h;
+            const uint32_t run = __ballot_sync(0xffffffffu, in_run);
+            todo &= ~run;
+            const int sum_pages = __reduce_add_sync(0xffffffffu, in_run ? it.w : 0);
+            float M = in_run ? ml.x : -INFINITY;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
             // a part without a token (maximum -inf) holds zeros; one whose scores are all NaN, NaN
-            const float top = fmaxf(M, ml.x);
-            const float f0 = M == top ? 1.0f : exp2f(M - top), f1 = ml.x == top ? 1.0f : exp2f(ml.x - top);
-            M = top;
-            L = fmaf(ml.y, f1, L * f0);
-            O.x = fmaf(v.x, f1, O.x * f0);
-            O.y = fmaf(v.y, f1, O.y * f0);
-            O.z = fmaf(v.z, f1, O.z * f0);
-            O.w = fmaf(v.w, f1, O.w * f0);
+            const float f = ml.x == M ? 1.0f : exp2f(ml.x - M);
+            float L = in_run ? ml.y * f : 0.0f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+            float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+            for (uint32_t r = run; r; r &= r - 1) {
+                const int k = __ffs(r) - 1;
+                const float* from =
+                    (k & 1) ? reinterpret_cast<const float*>(S.tiles[k >> 1][0]) : &S.acc[k >> 1][0][0];
+                const float4 v = reinterpret_cast<const float4*>(from + head * D)[lane];
+                const float fk = __shfl_sync(0xffffffffu, f, k);
+                O.x = fmaf(v.x, fk, O.x);
+                O.y = fmaf(v.y, fk, O.y);
+                O.z = fmaf(v.z, fk, O.z);
+                O.w = fmaf(v.w, fk, O.w);
+            }
+            if (sum_pages == pages) {
+                store4(a, ((size_t)m * a.Hq + h * G + head) * D + 4 * lane, O, L);
+            } else {
+                // the item that the CTA begins inside (or with) goes to its first slot, one that it does not
+                // end to its second
+                const bool first = p0 > 0 || (m == S.start[0] && h == S.start[1] && S.start[2] == 0);
+                const size_t slot = ((size_t)2 * blockIdx.x + (first ? 0 : 1)) * G + head;
+                reinterpret_cast<float4*>(part.o + slot * D)[lane] = O;
+                if (lane == 0) part.ml[slot] = make_float2(M, L);
+            }
         }
-        flush();
     }
 }
 
-// Joins the partials of the (row, KV head)s that several CTAs of the decode kernel share: CTA
-// c - 1 the one among whose pages CTA c began, if c is the first to do so. Warp w of query head
-// y takes the partials w, w + 8, ...; the warps' sums meet in shared memory.
+// Joins the partials of the (row, KV head)s that several CTAs of the decode kernel share: for
+// each CTA c that begins among the pages of one, if c is the first to do so. A block looks at
+// eight such c and one query head of each: a warp joins up to eight partials alone, and the
+// block's warps together those of an item with more.
 constexpr int kMergeWarps = 8;
-__global__ void __launch_bounds__(kMergeWarps * 32) kv8_merge_kernel(const Kv8AttnArgs a, void* scratch) {
+
+struct MergeItem {
+    int4 at;                 // where CTA c begins
+    int c, n, first;         // n partials: slot `first`, then slots 2 c, 2 (c + 1), ...
+};
+__device__ __forceinline__ MergeItem merge_item(const Partials& part, int c, int n_ctas, int chunk) {
+    MergeItem x;
+    x.c = c;
+    x.n = 0;
+    if (c >= n_ctas) return x;
+    x.at = part.begin[c];
+    // units [0, at.z) of the item lie before CTA c; is c the first CTA that begins among its pages?
+    if (x.at.x < 0 || x.at.z == 0 || x.at.z > chunk || x.at.z >= x.at.w) return x;
+    x.n = 1 + (x.at.w - x.at.z + chunk - 1) / chunk;
+    x.first = 2 * (c - 1) + (x.at.z == chunk ? 0 : 1);
+    return x;
+}
+
+// Partials k0, k0 + step, ... (at most eight) of an item joined to (M, L, O), lane l dims 4 l ..
+__device__ __forceinline__ void merge_eight(const Partials& part, const MergeItem& x, int G, int head, int k0, int step,
+                                            int lane, float& M, float& L, float4& O) {
+    float2 ml[8];
+    float4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int k = k0 + j * step;
+        ml[j] = make_float2(-INFINITY, 0.0f);
+        v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (k < x.n) {
+            const size_t slot = (size_t)(k ? 2 * (x.c + k - 1) : x.first) * G + head;
+            ml[j] = part.ml[slot];
+            v[j] = reinterpret_cast<const float4*>(part.o + slot * D)[lane];
+        }
+    }
+    float top = M;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, ml[j].x);
+    const float f = M == top ? 1.0f : exp2f(M - top);
+    M = top;
+    L *= f;
+    O = make_float4(O.x * f, O.y * f, O.z * f, O.w * f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float fj = ml[j].x == top ? 1.0f : exp2f(ml[j].x - top);
+        L = fmaf(ml[j].y, fj, L);
+        O.x = fmaf(v[j].x, fj, O.x);
+        O.y = fmaf(v[j].y, fj, O.y);
+        O.z = fmaf(v[j].z, fj, O.z);
+        O.w = fmaf(v[j].w, fj, O.w);
+    }
+}
+
+__global__ void __launch_bounds__(kMergeWarps * 32) kv8_merge_kernel(const Kv8AttnArgs a, void* scratch, int n_ctas) {
     __shared__ float4 s_o[kMergeWarps][32];
     __shared__ float2 s_ml[kMergeWarps];
-    pdl_wait();
+    __shared__ MergeItem s_item[kMergeWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.Hq / a.Hkv, head = blockIdx.y;
     const Partials part = partials(scratch, G);
-    const int c = blockIdx.x + 1;
-    const int chunk = *part.chunk;
-    const int4 at = part.begin[c];
-    // units [0, at.z) of the item lie before CTA c; the first CTA that begins among its pages?
-    if (at.x < 0 || at.z == 0 || at.z > chunk || at.z >= at.w) return;
-    const int n = 1 + (at.w - at.z + chunk - 1) / chunk;          // CTAs that hold a part
-    const int first = 2 * (c - 1) + (at.z == chunk ? 0 : 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float M = -INFINITY;
-    for (int k = lane; k < n; k += 32) M = fmaxf(M, part.ml[(size_t)(k ? 2 * (c + k - 1) : first) * G + head].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float L = 0.0f;
-    float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int k = warp; k < n; k += kMergeWarps) {
-        const size_t i = (size_t)(k ? 2 * (c + k - 1) : first) * G + head;
-        const float2 ml = part.ml[i];
-        const float4 v = reinterpret_cast<const float4*>(part.o + i * D)[lane];
-        const float f = ml.x == M ? 1.0f : exp2f(ml.x - M);
-        L = fmaf(ml.y, f, L);
-        O.x = fmaf(v.x, f, O.x);
-        O.y = fmaf(v.y, f, O.y);
-        O.z = fmaf(v.z, f, O.z);
-        O.w = fmaf(v.w, f, O.w);
+    pdl_wait();
+    const MergeItem mine = merge_item(part, blockIdx.x * kMergeWarps + warp + 1, n_ctas, *part.chunk);
+    if (lane == 0) s_item[warp] = mine;
+    if (mine.n > 0 && mine.n <= 8) {
+        float M = -INFINITY, L = 0.0f;
+        float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        merge_eight(part, mine, G, head, 0, 1, lane, M, L, O);
+        store4(a, ((size_t)mine.at.x * a.Hq + mine.at.y * G + head) * D + 4 * lane, O, L);
     }
-    s_o[warp][lane] = O;
-    if (lane == 0) s_ml[warp].y = L;
-    __syncthreads();
-    if (threadIdx.x >= D) return;
-    L = 0.0f;
-    float v = 0.0f;
+    if (!__syncthreads_or(mine.n > 8)) return;
+    for (int j = 0; j < kMergeWarps; ++j) {
+        const MergeItem x = s_item[j];
+        if (x.n <= 8) continue;
+        float M = -INFINITY, L = 0.0f;
+        float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = warp; k < x.n; k += 8 * kMergeWarps) merge_eight(part, x, G, head, k, kMergeWarps, lane, M, L, O);
+        s_o[warp][lane] = O;
+        if (lane == 0) s_ml[warp] = make_float2(M, L);
+        __syncthreads();
+        if (warp == 0) {
+            float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) {
-        L += s_ml[w].y;
-        v += reinterpret_cast<const float*>(s_o[w])[threadIdx.x];
+            for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, s_ml[w].x);
+            L = 0.0f;
+            O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kMergeWarps; ++w) {
+                const float f = s_ml[w].x == top ? 1.0f : exp2f(s_ml[w].x - top);
+                const float4 v = s_o[w][lane];
+                L = fmaf(s_ml[w].y, f, L);
+                O.x = fmaf(v.x, f, O.x);
+                O.y = fmaf(v.y, f, O.y);
+                O.z = fmaf(v.z, f, O.z);
+                O.w = fmaf(v.w, f, O.w);
+            }
+            store4(a, ((size_t)x.at.x * a.Hq + x.at.y * G + head) * D + 4 * lane, O, L);
+        }
+        __syncthreads();
     }
-    store_out(a, ((size_t)at.x * a.Hq + at.y * G + head) * D + threadIdx.x, L == 0.0f ? 0.0f : v / L);
 }
 
 template <int FMT, int NT>
@@ -724,7 +798,7 @@ cudaError_t launch_decode(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scr
     if (e != cudaSuccess) return e;
     // launched while the decode kernel runs; it waits for that kernel's end before it reads
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid - 1, a.Hq / a.Hkv);
+    cfg.gridDim = dim3((grid - 1 + kMergeWarps - 1) / kMergeWarps, a.Hq / a.Hkv);
     cfg.blockDim = dim3(kMergeWarps * 32);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -732,7 +806,7 @@ cudaError_t launch_decode(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scr
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv8_merge_kernel, a, scratch);
+    return cudaLaunchKernelEx(&cfg, kv8_merge_kernel, a, scratch, grid);
 }
 
 template <int FMT>
