@@ -121,17 +121,6 @@ __host__ __device__ constexpr uint32_t tmem_cols() {
     return Q8 ? 512u : (2 * BNA < 32 ? 32u : (uint32_t)(2 * BNA));
 }
 
-// tcgen05.mma with the A operand (M = 128 rows, K = 16: 8 columns of f16 pairs) in TMEM.
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc,
-                                              uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
 // Half a row (32 of the stage's 64 K values, half h) of a raw stage -> the f16 pair of those
 // weights in TMEM slot columns [col + 16h, col + 16h + 16) (hi) and [col + 32 + 16h, ...)
 // (lo). The q row is read with the 64 B swizzle its TMA box was written with: chunk c of

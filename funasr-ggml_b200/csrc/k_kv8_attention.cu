@@ -1,13 +1,5 @@
-// Attention over the 8-bit page pool (k_kv8.cuh): decode rows and causal prefill tiles.
-//
-// Row m attends to tokens t in [0, pos[m]] of its sequence; query head H uses KV head
-// H / (n_heads / n_kv_heads):
-//   s_t = dk_t (q . kq_t),  o = sum_t exp(s_t - max s) dv_t vq_t / sum_t exp(s_t - max s)
-// with kq, vq the stored 8-bit values and dk, dv the scales of their vectors. The scales
-// multiply a score and a weight, never the 128 values.
-#include "k_kv8.cuh"
-#include "tc_common.cuh"
-#include "funasr_dec.h"
+// Decode attention over the 8-bit page pool (formulas in k_kv8_attn.cuh).
+#include "k_kv8_attn.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -15,122 +7,47 @@
 
 namespace fa {
 
-int report_op_error(int code, const char* msg);   // fa_api.cu
+using namespace kv8;
 
 namespace {
 
-using namespace kv8;
+bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 
-constexpr float kLog2e = 1.4426950408889634f;
+}  // namespace
 
-struct Kv8AttnArgs {
-    const float* q;          // [M][Hq][128], pre-scaled
-    int M, Hq, Hkv;
-    const int* pos;
-    const int* slot;
-    const int* block_table;
-    int bt_stride;
-    int n_pages;
-    const unsigned char* pool;   // one layer
-    const int2* tiles;       // prefill: (first row, rows)
-    int n_tiles;
-    __half* out16;
-    __half* out16_lo;
-    float* out32;
-    int* err;
-};
-
-__device__ __forceinline__ void store_out(const Kv8AttnArgs& a, size_t o, float v) {
-    if (a.out16) {
-        const __half h = __float2half_rn(v);
-        a.out16[o] = h;
-        if (a.out16_lo) a.out16_lo[o] = __float2half_rn(__fsub_rn(v, __half2float(h)));
-    }
-    if (a.out32) a.out32[o] = v;
+// The arguments that decode and prefill share, checked; FA_OK or the recorded error.
+int kv8_attention_check(const std::string& what, const Kv8AttnArgs& a, int format, const void* scratch,
+                        size_t scratch_bytes, size_t need) {
+    if (!a.q || !a.pos || !a.slot || !a.block_table || !a.pool || (!a.out16 && !a.out32) || a.M <= 0 || a.Hq <= 0 ||
+        a.Hkv <= 0 || a.bt_stride <= 0 || a.n_pages <= 0)
+        return report_op_error(FA_ERR_INVALID_ARG, (what + ": null or non-positive argument").c_str());
+    if (a.out16_lo && !a.out16)
+        return report_op_error(FA_ERR_INVALID_ARG, (what + ": out16_lo needs out16").c_str());
+    if (format != FA_KV8_INT8 && format != FA_KV8_E4M3)
+        return report_op_error(FA_ERR_INVALID_ARG, (what + ": unknown format").c_str());
+    if (a.Hq % a.Hkv || a.Hq / a.Hkv > 8)
+        return report_op_error(FA_ERR_INVALID_ARG,
+                               (what + ": n_heads must be 1 to 8 times n_kv_heads").c_str());
+    if (misaligned(a.q, 16) || misaligned(a.pool, 128) || misaligned(a.out16, 16) || misaligned(a.out16_lo, 16) ||
+        misaligned(a.out32, 16) || misaligned(scratch, 16))
+        return report_op_error(FA_ERR_INVALID_ARG,
+                               (what + ": q, outputs and scratch must be 16-byte, pool 128-byte aligned").c_str());
+    if (a.Hq > 65535 || (long long)a.bt_stride * kPageTokens > 0x7fffffffll)
+        return report_op_error(FA_ERR_CAPACITY, (what + ": n_heads or bt_stride too large").c_str());
+    if ((long long)a.n_pages * a.Hkv * (kTileBytes / 128) > 0x7fffffffll)
+        return report_op_error(FA_ERR_CAPACITY, (what + ": the pool has too many pages").c_str());
+    if (need && (!scratch || scratch_bytes < need))
+        return report_op_error(FA_ERR_INVALID_ARG, (what + ": scratch of " + std::to_string(need) +
+                                                    " bytes required").c_str());
+    return FA_OK;
 }
 
-// N consecutive outputs x / l from offset o (a multiple of 4; of 8 for N = 16): 0 where no
-// token takes part (l = 0).
-template <int N>
-__device__ __forceinline__ void store_quotients(const Kv8AttnArgs& a, size_t o, const float (&x)[N], float l) {
-    float v[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = l == 0.0f ? 0.0f : x[k] / l;
-    if (a.out32) {
-#pragma unroll
-        for (int k = 0; k < N; k += 4)
-            *reinterpret_cast<float4*>(a.out32 + o + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-    }
-    if (a.out16) {
-#pragma unroll
-        for (int k = 0; k < N; k += 4) {
-            uint32_t hi[2], lo[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const __half2 h = __floats2half2_rn(v[k + 2 * e], v[k + 2 * e + 1]);
-                const float2 f = __half22float2(h);
-                const __half2 r = __floats2half2_rn(__fsub_rn(v[k + 2 * e], f.x), __fsub_rn(v[k + 2 * e + 1], f.y));
-                hi[e] = *reinterpret_cast<const uint32_t*>(&h);
-                lo[e] = *reinterpret_cast<const uint32_t*>(&r);
-            }
-            *reinterpret_cast<uint2*>(a.out16 + o + k) = make_uint2(hi[0], hi[1]);
-            if (a.out16_lo) *reinterpret_cast<uint2*>(a.out16_lo + o + k) = make_uint2(lo[0], lo[1]);
-        }
-    }
-}
-__device__ __forceinline__ void store16(const Kv8AttnArgs& a, size_t o, const float (&x)[16], float l) {
-    store_quotients<16>(a, o, x, l);
-}
-__device__ __forceinline__ void store4(const Kv8AttnArgs& a, size_t o, float4 x, float l) {
-    const float v[4] = {x.x, x.y, x.z, x.w};
-    store_quotients<4>(a, o, v, l);
+// The pool as rows of 128 bytes (33 a tile: 16 of K, 16 of V, the scales); a box is K and V.
+bool make_kv8_tile_map(CUtensorMap* tm, const void* pool, long long rows) {
+    return make_map(tm, pool, 64, rows, 64, 2 * kPageTokens, true);
 }
 
-// One query vector of one row by a warp, lane l holding dims 4l .. 4l+3.
-template <int FMT>
-__device__ void attend_row(const Kv8AttnArgs& a, int m, int H, int lane) {
-    const int pos = a.pos[m];
-    const size_t o = ((size_t)m * a.Hq + H) * D + 4 * lane;
-    if (pos < -1 || pos / kPageTokens >= a.bt_stride || (pos >= 0 && a.slot[m] < 0)) {
-        if (lane == 0 && H == 0) record_error(a.err, kDevErrBadLen);
-        return;
-    }
-    const int h = H / (a.Hq / a.Hkv);
-    const float4 q = *reinterpret_cast<const float4*>(a.q + o);
-    float mx = -INFINITY, sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = 0; p * kPageTokens <= pos; ++p) {
-        const int page = a.block_table[(size_t)a.slot[m] * a.bt_stride + p];
-        if (page < 0 || page >= a.n_pages) {
-            if (lane == 0) record_error(a.err, kDevErrBadPage);
-            continue;
-        }
-        const unsigned char* tile = a.pool + ((size_t)page * a.Hkv + h) * kTileBytes;
-        const float* scale = reinterpret_cast<const float*>(tile + kScaleOff);
-        const int n = min(kPageTokens, pos + 1 - p * kPageTokens);
-        for (int t = 0; t < n; ++t) {
-            __half2 x, y;
-            expand4<FMT>(*reinterpret_cast<const uint32_t*>(tile + t * D + 4 * lane), x, y);
-            const float2 k0 = __half22float2(x), k1 = __half22float2(y);
-            float s = q.x * k0.x + q.y * k0.y + q.z * k1.x + q.w * k1.y;
-#pragma unroll
-            for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
-            s *= scale[t] * kLog2e;
-            const float top = fmaxf(mx, s);
-            const float alpha = exp2f(mx - top), w = exp2f(s - top);
-            mx = top;
-            sum = sum * alpha + w;
-            expand4<FMT>(*reinterpret_cast<const uint32_t*>(tile + kPartBytes + t * D + 4 * lane), x, y);
-            const float2 v0 = __half22float2(x), v1 = __half22float2(y);
-            const float wv = w * scale[kPageTokens + t];
-            acc[0] = acc[0] * alpha + wv * v0.x;
-            acc[1] = acc[1] * alpha + wv * v0.y;
-            acc[2] = acc[2] * alpha + wv * v1.x;
-            acc[3] = acc[3] * alpha + wv * v1.y;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) store_out(a, o + i, sum == 0.0f ? 0.0f : acc[i] / sum);
-}
+namespace {
 
 // ------------------------------------------------------------------ decode --
 // The (row, KV head)s, in that order, are one list of units, a unit per page and kItemUnits
@@ -141,9 +58,10 @@ __device__ void attend_row(const Kv8AttnArgs& a, int m, int H, int lane) {
 // last): the CTA joins those of its four warps, and what it shares with other CTAs, again at
 // most two partials, goes to scratch un-normalised and is joined by kv8_merge_kernel.
 //
-// A warp streams its pages through a ring of its own: lane 0 issues one TMA box (32 rows of 128 B: K and V of the head in that page, 128 B swizzle) and one bulk copy
-// (their scales) per page. Per page of 16 tokens, on the tensor cores with the keys as the
-// 16-row operand (m16n8k16, f16 in, f32 sums):
+// A warp streams its pages through a ring of its own: lane 0 issues one TMA box (32 rows of
+// 128 B: K and V of the head in that page, 128 B swizzle, so that the reads below meet no bank
+// conflicts) and one bulk copy (their scales) per page. Per page of 16 tokens, on the tensor
+// cores with the keys as the 16-row operand (m16n8k16, f16 in, f32 sums):
 //   S[16 tokens][8 columns] = K . q     K expanded to f16 exactly; a query head is two columns,
 //                                       hi = f16(q') and lo = f16(q' - hi), q' = q scaled by a
 //                                       power of two to [1, 2): 22 bits of q
@@ -209,12 +127,6 @@ __device__ __forceinline__ uint32_t hi_lo(float x) {
     return (uint32_t)__half_as_ushort(h) | ((uint32_t)__half_as_ushort(l) << 16);
 }
 
-// The power of two at or below x, within 2^-126 .. 2^126, and the inverse of such a one.
-__device__ __forceinline__ float pow2_floor(float x) {
-    return __uint_as_float(min(max(__float_as_uint(x) & 0x7f800000u, 0x00800000u), 0x7e800000u));
-}
-__device__ __forceinline__ float pow2_inverse(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
-
 // Stored values of two tokens (words a, b: four dims each) as f16 pairs (a_i, b_i).
 template <int FMT>
 __device__ __forceinline__ void expand_pairs(uint32_t a, uint32_t b, uint32_t (&v)[4]) {
@@ -236,11 +148,6 @@ __device__ __forceinline__ void expand_pairs(uint32_t a, uint32_t b, uint32_t (&
     }
 }
 
-// Pages of row m; 0 for padding and for a row that cannot be served (flagged elsewhere).
-__device__ __forceinline__ bool row_bad(const Kv8AttnArgs& a, int m) {
-    const int pos = a.pos[m];
-    return pos < -1 || pos / kPageTokens >= a.bt_stride || (pos >= 0 && a.slot[m] < 0);
-}
 __device__ __forceinline__ int row_pages(const Kv8AttnArgs& a, int m) {
     return row_bad(a, m) ? 0 : (a.pos[m] + kPageTokens) / kPageTokens;
 }
@@ -378,7 +285,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     // rows without pages: padding is zeroed, a row that cannot be served is flagged and left
     for (int m = blockIdx.x; m < a.M; m += gridDim.x) {
         if (a.pos[m] == -1)
-            for (int d = tid; d < a.Hq * D; d += kWarps * 32) store_out(a, (size_t)m * a.Hq * D + d, 0.0f);
+            for (int d = 4 * tid; d < a.Hq * D; d += kWarps * 128)
+                store4(a, (size_t)m * a.Hq * D + d, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 1.0f);
         else if (tid == 0 && row_bad(a, m)) record_error(a.err, kDevErrBadLen);
     }
     __syncthreads();
@@ -809,67 +717,12 @@ cudaError_t launch_decode(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scr
     return cudaLaunchKernelEx(&cfg, kv8_merge_kernel, a, scratch, grid);
 }
 
-template <int FMT>
-__global__ void __launch_bounds__(128) kv8_prefill_kernel(Kv8AttnArgs a) {
-    const int2 tile = a.tiles[blockIdx.x];
-    if (tile.x < 0 || tile.y < 1 || tile.y > 128 / (a.Hq / a.Hkv) || tile.x > a.M - tile.y) {
-        if (blockIdx.y == 0 && threadIdx.x == 0) record_error(a.err, kDevErrBadPos);
-        return;
-    }
-    const int H = blockIdx.y;
-    for (int r = threadIdx.x >> 5; r < tile.y; r += 4) attend_row<FMT>(a, tile.x + r, H, threadIdx.x & 31);
-}
-
-bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
-
-// The arguments that decode and prefill share, checked; FA_OK or the recorded error.
-int check(const std::string& what, const Kv8AttnArgs& a, int format, const void* scratch, size_t scratch_bytes,
-          size_t need) {
-    if (!a.q || !a.pos || !a.slot || !a.block_table || !a.pool || (!a.out16 && !a.out32) || a.M <= 0 || a.Hq <= 0 ||
-        a.Hkv <= 0 || a.bt_stride <= 0 || a.n_pages <= 0)
-        return report_op_error(FA_ERR_INVALID_ARG, (what + ": null or non-positive argument").c_str());
-    if (a.out16_lo && !a.out16)
-        return report_op_error(FA_ERR_INVALID_ARG, (what + ": out16_lo needs out16").c_str());
-    if (format != FA_KV8_INT8 && format != FA_KV8_E4M3)
-        return report_op_error(FA_ERR_INVALID_ARG, (what + ": unknown format").c_str());
-    if (a.Hq % a.Hkv || a.Hq / a.Hkv > 8)
-        return report_op_error(FA_ERR_INVALID_ARG,
-                               (what + ": n_heads must be 1 to 8 times n_kv_heads").c_str());
-    if (misaligned(a.q, 16) || misaligned(a.pool, 128) || misaligned(a.out16, 16) || misaligned(a.out16_lo, 16) ||
-        misaligned(a.out32, 16) || misaligned(scratch, 16))
-        return report_op_error(FA_ERR_INVALID_ARG,
-                               (what + ": q, outputs and scratch must be 16-byte, pool 128-byte aligned").c_str());
-    if (a.Hq > 65535 || (long long)a.bt_stride * kPageTokens > 0x7fffffffll)
-        return report_op_error(FA_ERR_CAPACITY, (what + ": n_heads or bt_stride too large").c_str());
-    if ((long long)a.n_pages * a.Hkv * (kTileBytes / 128) > 0x7fffffffll)
-        return report_op_error(FA_ERR_CAPACITY, (what + ": the pool has too many pages").c_str());
-    if (need && (!scratch || scratch_bytes < need))
-        return report_op_error(FA_ERR_INVALID_ARG, (what + ": scratch of " + std::to_string(need) +
-                                                    " bytes required").c_str());
-    return FA_OK;
-}
-
-// The pool as rows of 128 bytes (33 a tile: 16 of K, 16 of V, the scales); a box is K and V.
-bool make_tile_map(CUtensorMap* tm, const void* pool, long long rows) {
-    return make_map(tm, pool, 64, rows, 64, 2 * kPageTokens, true);
-}
-
-int launched(const char* what) {
-    const cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess) return FA_OK;
-    return report_op_error(FA_ERR_CUDA, (std::string(what) + ": " + cudaGetErrorString(e)).c_str());
-}
-
 }  // namespace
 }  // namespace fa
 
 extern "C" FA_API size_t fa_op_attention_kv8_scratch_bytes(int M, int n_heads, int n_kv_heads) {
     if (M <= 0 || n_kv_heads <= 0 || n_heads < n_kv_heads || n_heads % n_kv_heads) return 0;
     return fa::partial_bytes(n_heads / n_kv_heads);
-}
-
-extern "C" FA_API size_t fa_op_prefill_attention_kv8_scratch_bytes(int n_tiles, int n_heads, int n_kv_heads) {
-    return n_tiles > 0 && n_heads > 0 && n_kv_heads > 0 ? 16 : 0;
 }
 
 extern "C" FA_API int fa_op_paged_attention_kv8(const float* q, int M, int n_heads, int n_kv_heads, const int* pos,
@@ -881,11 +734,11 @@ extern "C" FA_API int fa_op_paged_attention_kv8(const float* q, int M, int n_hea
     Kv8AttnArgs a{q, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages,
                   static_cast<const unsigned char*>(pool_layer), nullptr, 0, reinterpret_cast<__half*>(out16),
                   reinterpret_cast<__half*>(out16_lo), out32, err};
-    if (int rc = check("fa_op_paged_attention_kv8", a, format, scratch, scratch_bytes,
+    if (int rc = kv8_attention_check("fa_op_paged_attention_kv8", a, format, scratch, scratch_bytes,
                        fa_op_attention_kv8_scratch_bytes(M, n_heads, n_kv_heads)))
         return rc;
     CUtensorMap tm;
-    if (!make_tile_map(&tm, pool_layer, (long long)n_pages * n_kv_heads * (kTileBytes / 128)))
+    if (!make_kv8_tile_map(&tm, pool_layer, (long long)n_pages * n_kv_heads * (kTileBytes / 128)))
         return report_op_error(FA_ERR_CUDA, "fa_op_paged_attention_kv8: cannot build the page-pool tensor map");
     // no more CTAs than there can be pages
     const int grid = (int)std::min<long long>((long long)M * n_kv_heads * bt_stride, kMaxCtas);
@@ -897,24 +750,4 @@ extern "C" FA_API int fa_op_paged_attention_kv8(const float* q, int M, int n_hea
     if (e != cudaSuccess) cudaGetLastError();
     return e == cudaSuccess ? FA_OK
                             : report_op_error(FA_ERR_CUDA, (std::string("fa_op_paged_attention_kv8: ") + cudaGetErrorString(e)).c_str());
-}
-
-extern "C" FA_API int fa_op_prefill_attention_kv8(const float* q, int M, int n_heads, int n_kv_heads, const int* pos,
-                                                  const int* slot, const int* bt, int bt_stride, int n_pages,
-                                                  int format, const void* pool_layer, const int* tiles, int n_tiles,
-                                                  void* scratch, size_t scratch_bytes, uint16_t* out16,
-                                                  uint16_t* out16_lo, float* out32, int* err, void* stream) {
-    using namespace fa;
-    Kv8AttnArgs a{q, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages,
-                  static_cast<const unsigned char*>(pool_layer), reinterpret_cast<const int2*>(tiles), n_tiles,
-                  reinterpret_cast<__half*>(out16), reinterpret_cast<__half*>(out16_lo), out32, err};
-    if (!tiles || n_tiles <= 0 || misaligned(tiles, 8))
-        return report_op_error(FA_ERR_INVALID_ARG, "fa_op_prefill_attention_kv8: tiles missing or not 8-byte aligned");
-    if (int rc = check("fa_op_prefill_attention_kv8", a, format, scratch, scratch_bytes,
-                       fa_op_prefill_attention_kv8_scratch_bytes(n_tiles, n_heads, n_kv_heads)))
-        return rc;
-    const dim3 grid(n_tiles, n_heads);
-    if (format == FA_KV8_INT8) kv8_prefill_kernel<kInt8><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
-    else kv8_prefill_kernel<kE4m3><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
-    return launched("fa_op_prefill_attention_kv8");
 }

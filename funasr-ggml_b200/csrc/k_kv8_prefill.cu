@@ -1,0 +1,625 @@
+// Causal attention of prefill tiles over the 8-bit page pool on the 5th-generation tensor
+// cores (formulas in k_kv8_attn.cuh).
+//
+// A CTA takes one tile (up to R = 128 / G rows of one sequence, G query heads to a KV head), one
+// KV head and, where a call has few tiles, a part of the tile's keys: its up to 128 query
+// vectors (vector v = row v % R, head v / R) are the M side of every MMA, so a page is read and
+// expanded to f16 once for all of them. Per block of 64 keys (4 pages):
+//   S  = Q . K^T        tcgen05.mma kind::f16, M 128, N 64, K 128; Q in TMEM as the pair
+//                       hi = f16(q'), lo = f16(q' - hi), q' = q scaled by a power of two to [1, 2)
+//   p  = exp2(dk S - m) one query vector per thread; w = p dv / sigma, sigma a power of two at
+//                       the largest dv so far (times 2^-6): f16 pairs, written over S in TMEM
+//   O += w . V          M 128, N 128 (dims), K 64 (keys), V MN-major
+// Both A operands are in TMEM because shared memory would otherwise bound the kernel: a block
+// reads 128 KB of it for the MMAs with Q and w there, 64 KB (only K and V) without, against the
+// 1024 cycles that its MMAs take.
+// The running maximum is lazy (O is rescaled when a block exceeds it by 2^8 or sigma grows).
+//
+// Roles (320 threads): warp 0 issues the page copies (one TMA box and one bulk copy of scales
+// per page) into a ring of raw blocks; warps 6-9 expand a raw block into the f16 K / V tiles of
+// a second ring, with each key's factors; warp 1 holds TMEM and issues the MMAs; warps 2-5
+// load Q, run the softmax and write the outputs. Every mbarrier wait is bounded; on a timeout
+// the CTA records the error, drains its copies and MMAs and frees TMEM.
+#include "k_kv8_attn.cuh"
+
+#include <algorithm>
+
+namespace fa {
+
+using namespace kv8;
+
+namespace {
+
+constexpr int KB = 64;                        // keys per block
+constexpr int PAGES = KB / kPageTokens;
+constexpr int RAW = 3;                        // raw ring (8-bit blocks)
+constexpr int TILES = 4;                      // f16 ring
+constexpr int THREADS = 320;
+constexpr int kMaxParts = 16;                 // key ranges of one tile and head
+constexpr int kMinPartBlocks = 8;
+constexpr uint32_t TMEM_COLS = 512;           // S0 [0,64) S1 [64,128) O [128,256) Q hi [256,320) Q lo [320,384)
+constexpr uint32_t COL_O = 128, COL_Q = 256;
+constexpr float kLazy = 8.0f;                 // log2 units
+
+struct PfSmem {
+    __half k[TILES][2][KB * 64];              // [dim half][64 tokens][64 dims], 128 B swizzle
+    __half v[TILES][2][KB * 64];
+    unsigned char raw[RAW][PAGES][2 * kPartBytes];
+    float raw_scales[RAW][PAGES][2 * kPageTokens];
+    float dk[TILES][KB];                      // K scales
+    float dv[TILES][KB];                      // V scales / sigma
+    float sigma[TILES];
+    float ratio[TILES];                       // sigma before the block / sigma
+    int raw_pages[RAW];                       // bit q: page q of the block was copied
+    int pages[TILES];
+    uint64_t raw_full[RAW];
+    uint64_t raw_empty[RAW];
+    uint64_t kv_full[TILES];
+    uint64_t kv_empty[TILES];
+    uint64_t s_full[2];
+    uint64_t p_ready[2];
+    uint64_t q_ready;
+    uint64_t o_done;
+    uint64_t drain;
+    uint32_t tmem_base;
+    int pos_last;                             // last key any row of the tile attends to; -1: none
+    int slot;
+    int err;
+    int issued;                               // raw blocks issued, and waited for
+    int consumed;
+};
+
+// Byte offset of 16-byte chunk `chunk` (0..7) of row `row` in a [rows][128 B] tile with 128 B
+// swizzle.
+__device__ __forceinline__ uint32_t sw128(int row, int chunk) {
+    return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// f16 pair words of (a, b): high parts, and the rest
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack2(a, b);
+    const float2 f = h2_to_f2(hi);
+    lo = pack2(__fsub_rn(a, f.x), __fsub_rn(b, f.y));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The key blocks [first, last) of part `part` of an item of nb blocks cut into at most
+// max_parts, and the number of parts.
+__device__ __forceinline__ int part_blocks(int nb, int max_parts, int part, int& first, int& last) {
+    const int parts = max(1, min(max_parts, nb / kMinPartBlocks));
+    const int per = (nb + parts - 1) / parts;
+    first = min(part * per, nb);
+    last = min(first + per, nb);
+    return max(1, (nb + per - 1) / max(per, 1));
+}
+
+// By one warp: the last key that the rows of a tile attend to (-1: none) and their slot, the
+// one of the row that attends furthest.
+__device__ __forceinline__ int tile_extent(const Kv8AttnArgs& a, int2 tile, int lane, int& slot) {
+    int best = -1, row = 0;
+    for (int r = lane; r < tile.y; r += 32) {
+        const int m = tile.x + r;
+        if (!row_bad(a, m) && a.pos[m] > best) {
+            best = a.pos[m];
+            row = m;
+        }
+    }
+    const int last = __reduce_max_sync(0xffffffffu, best);
+    const int who = __ffs(__ballot_sync(0xffffffffu, best == last)) - 1;
+    slot = last >= 0 ? a.slot[__shfl_sync(0xffffffffu, row, who)] : 0;
+    return last;
+}
+__device__ __forceinline__ bool tile_bad(const Kv8AttnArgs& a, int2 tile) {
+    return tile.x < 0 || tile.y < 1 || tile.y > 128 / (a.Hq / a.Hkv) || tile.x > a.M - tile.y;
+}
+
+// Un-normalised partials of the parts: o [items][parts][128 vectors][128], ml (maximum in log2
+// units, sum) [items][parts][128]; item = tile * Hkv + KV head.
+__host__ __device__ inline size_t part_index(const Kv8AttnArgs& a, int tile, int h, int parts, int part) {
+    return (((size_t)tile * a.Hkv + h) * parts + part) * 128;
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(THREADS, 1)
+    kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm_pool, const Kv8AttnArgs a, float* part_o,
+                       float2* part_ml) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    PfSmem& S = *reinterpret_cast<PfSmem*>(smem_raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.x, max_parts = gridDim.z;
+    const int G = a.Hq / a.Hkv, R = 128 / G;
+    pdl_trigger();
+
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tm_pool);
+        for (int s = 0; s < RAW; ++s) {
+            mbar_init(&S.raw_full[s], 1);
+            mbar_init(&S.raw_empty[s], 4);
+        }
+        for (int s = 0; s < TILES; ++s) {
+            mbar_init(&S.kv_full[s], 4);
+            mbar_init(&S.kv_empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&S.s_full[s], 1);
+            mbar_init(&S.p_ready[s], 128);
+        }
+        mbar_init(&S.q_ready, 128);
+        mbar_init(&S.o_done, 1);
+        mbar_init(&S.drain, 1);
+        S.err = 0;
+        S.issued = 0;
+        S.consumed = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem_base)),
+                     "r"(TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    const int2 tile = a.tiles[blockIdx.y];
+    const bool bad = tile_bad(a, tile);
+    if (warp == 2) {
+        int slot = 0;
+        const int last = bad ? -1 : tile_extent(a, tile, lane, slot);
+        if (lane == 0) {
+            S.pos_last = last;
+            S.slot = slot;
+        }
+    }
+    if (bad && threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.z == 0) record_error(a.err, kDevErrBadPos);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = S.tmem_base;
+    const int pos_last = S.pos_last, slot = S.slot;
+    int first = 0, last = 0;
+    const int parts = part_blocks((pos_last + KB) / KB, max_parts, blockIdx.z, first, last);
+    const int n_blocks = bad || blockIdx.z >= parts ? 0 : last - first;
+
+    if (bad || (int)blockIdx.z >= parts) {
+        // nothing issued: fall through to the TMEM release
+    } else if (warp == 0) {
+        const int* bt = a.block_table + (size_t)slot * a.bt_stride;
+        const int last_page = pos_last / kPageTokens;
+        bool ok = true;
+        int ids = 0;                                   // lane l: page 32 b + l of the part
+        for (int j = 0; ok && j < n_blocks; ++j) {
+            if ((j & 7) == 0) {
+                const int p = (first + j) * PAGES + lane;
+                ids = p <= last_page ? bt[p] : -1;
+                if (p <= last_page && (ids < 0 || ids >= a.n_pages)) {
+                    ids = -1;                          // its tokens are left out
+                    record_error(a.err, kDevErrBadPage);
+                }
+            }
+            const int s = j % RAW;
+            if (j >= RAW) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.raw_empty[s], (uint32_t)(j / RAW - 1) & 1u));
+            if (!ok) break;
+            int id[PAGES], have = 0;
+#pragma unroll
+            for (int q = 0; q < PAGES; ++q) {
+                id[q] = __shfl_sync(0xffffffffu, ids, (j & 7) * PAGES + q);
+                have |= (id[q] >= 0) << q;
+            }
+            if (lane == 0) {
+                S.raw_pages[s] = have;
+                mbar_arrive_expect_tx(&S.raw_full[s], __popc(have) * kTileBytes);
+#pragma unroll
+                for (int q = 0; q < PAGES; ++q) {
+                    if (id[q] < 0) continue;
+                    const int row = (id[q] * a.Hkv + h) * (kTileBytes / 128);
+                    tma_load_2d(S.raw[s][q], &tm_pool, 0, row, &S.raw_full[s]);
+                    bulk_copy_g2s(S.raw_scales[s][q], a.pool + (size_t)row * 128 + kScaleOff,
+                                  2 * kPageTokens * sizeof(float), &S.raw_full[s]);
+                }
+                S.issued = j + 1;
+            }
+            __syncwarp();
+        }
+        if (!ok && lane == 0) S.err = 1;
+    } else if (warp == 1) {
+        if (lane == 0 && n_blocks > 0) {
+            constexpr uint32_t kIdS = idesc_f16(128, KB, false, false);
+            constexpr uint32_t kIdPV = idesc_f16(128, D, false, true);
+            bool ok = mbar_wait_bounded(&S.q_ready, 0);
+            tc_fence_after();
+            for (int j = 0; ok && j <= n_blocks; ++j) {
+                if (j < n_blocks) {
+                    const int s = j % TILES;
+                    if (!mbar_wait_bounded(&S.kv_full[s], (uint32_t)(j / TILES) & 1u)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t d_s = tmem + (uint32_t)((j & 1) * KB);
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk) {
+                        const uint64_t db = smem_desc_k128(S.k[s][kk >> 2]) + ((uint32_t)((kk & 3) * 32) >> 4);
+                        tc_mma_f16_ts(d_s, tmem + COL_Q + 8 * kk, db, kIdS, kk > 0 ? 1u : 0u);
+                        tc_mma_f16_ts(d_s, tmem + COL_Q + 64 + 8 * kk, db, kIdS, 1u);
+                    }
+                    tc_commit(&S.s_full[j & 1]);
+                }
+                if (j >= 1) {
+                    const int jp = j - 1, sp = jp % TILES;
+                    if (!mbar_wait_bounded(&S.p_ready[jp & 1], (uint32_t)(jp >> 1) & 1u)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t d_p = tmem + (uint32_t)((jp & 1) * KB);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint64_t db = smem_desc_mn128(&S.v[sp][0][kk * 16 * 64], KB * 64 * 2);
+                        tc_mma_f16_ts(tmem + COL_O, d_p + 8 * kk, db, kIdPV, (jp > 0 || kk > 0) ? 1u : 0u);
+                        tc_mma_f16_ts(tmem + COL_O, d_p + 32 + 8 * kk, db, kIdPV, 1u);
+                    }
+                    tc_commit(&S.kv_empty[sp]);
+                    tc_commit(&S.o_done);
+                }
+            }
+            if (!ok) S.err = 1;
+            tc_commit(&S.drain);
+            if (!mbar_wait_bounded(&S.drain, 0)) S.err = 1;
+        }
+        __syncwarp();
+    } else if (warp >= 6) {
+        // expansion: thread c takes 16-byte chunk c % 8 of tokens c / 8, c / 8 + 16, ..., K and V
+        const int ct = threadIdx.x - 192, cw = warp - 6;
+        const int chunk = ct & 7;
+        uint32_t run = 0;                              // exponent field of sigma
+        bool ok = true;
+        for (int j = 0; j < n_blocks; ++j) {
+            const int s = j % RAW, d = j % TILES;
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.raw_full[s], (uint32_t)(j / RAW) & 1u));
+            if (ok && j >= TILES)
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.kv_empty[d], (uint32_t)(j / TILES - 1) & 1u));
+            if (!ok) break;
+            if (ct == 0) S.consumed = j + 1;
+            const int have = S.raw_pages[s];
+            const int key0 = (first + j) * KB;
+            // the keys' factors: sigma covers the finite V scales of the block's tokens
+            float dv[2];
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int t = lane + 32 * e;
+                const bool in = ((have >> (t >> 4)) & 1) && key0 + t <= pos_last;
+                dv[e] = in ? S.raw_scales[s][t >> 4][kPageTokens + (t & 15)] : 0.0f;
+                const uint32_t x = __float_as_uint(dv[e]) & 0x7f800000u;
+                top = max(top, x == 0x7f800000u ? 0u : x);
+            }
+            top = max(__reduce_max_sync(0xffffffffu, top), 11u << 23);
+            const uint32_t old = run;
+            run = max(run, top);
+            if (cw == 0) {
+                const float sigma = __uint_as_float(run - (6u << 23)), inv = pow2_inverse(sigma);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int t = lane + 32 * e;
+                    S.dk[d][t] = S.raw_scales[s][t >> 4][t & 15];
+                    S.dv[d][t] = dv[e] * inv;
+                }
+                if (lane == 0) {
+                    S.sigma[d] = sigma;
+                    S.ratio[d] = j == 0 ? 1.0f : __uint_as_float(old - (6u << 23)) * inv;
+                    S.pages[d] = have;
+                }
+            }
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                unsigned char* out = reinterpret_cast<unsigned char*>(part ? S.v[d][chunk >> 2] : S.k[d][chunk >> 2]);
+#pragma unroll
+                for (int i = 0; i < PAGES; ++i) {
+                    const int r = ct >> 3;             // token 16 i + r
+                    const int t = i * kPageTokens + r;
+                    uint4 x = lds128(S.raw[s][i] + part * kPartBytes + r * 128 + ((chunk ^ (r & 7)) << 4));
+                    // tokens of pages left out, and V behind the last token (unwritten bytes may be e4m3 NaN)
+                    if (!((have >> i) & 1) || (part && key0 + t > pos_last)) x = make_uint4(0, 0, 0, 0);
+                    __half2 y[8];
+                    expand4<FMT>(x.x, y[0], y[1]);
+                    expand4<FMT>(x.y, y[2], y[3]);
+                    expand4<FMT>(x.z, y[4], y[5]);
+                    expand4<FMT>(x.w, y[6], y[7]);
+                    const uint4* w = reinterpret_cast<const uint4*>(y);
+                    // dims 16 chunk ..: chunks 2 (chunk % 4), + 1 of the half's row; the upper half's threads
+                    // write them in the other order, which spreads a row's stores over all banks
+                    const int up = chunk >> 2, c2 = 2 * (chunk & 3);
+                    *reinterpret_cast<uint4*>(out + sw128(t, c2 + up)) = up ? w[1] : w[0];
+                    *reinterpret_cast<uint4*>(out + sw128(t, c2 + 1 - up)) = up ? w[0] : w[1];
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&S.kv_full[d]);
+                mbar_arrive(&S.raw_empty[s]);
+            }
+        }
+        if (!ok && lane == 0) S.err = 1;
+    } else {
+        // thread t owns TMEM lane t = query vector t (a warp may only touch lanes 32 * (warp % 4) ..)
+        const int quarter = warp & 3;
+        const int t = 32 * quarter + lane;
+        const int r = t % R, head = t / R;
+        const int row = tile.x + r;
+        bool live = head < G && r < tile.y;
+        int pos = pos_last;                            // lanes without a row mask no more than the others
+        if (live) {
+            pos = a.pos[row];
+            if (row_bad(a, row) || (pos >= 0 && a.slot[row] != slot)) {
+                if (h == 0 && blockIdx.z == 0 && head == 0) record_error(a.err, kDevErrBadLen);
+                live = false;
+                pos = pos_last;
+            }
+        }
+        const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16);
+        const size_t o_at = ((size_t)row * a.Hq + h * G + head) * D;
+        float qs = 0.0f;                               // takes dk S to log2 units
+        if (n_blocks > 0) {
+            float x[D];
+#pragma unroll
+            for (int k = 0; k < D; k += 4) {
+                const float4 v = live ? *reinterpret_cast<const float4*>(a.q + o_at + k) : make_float4(0, 0, 0, 0);
+                x[k] = v.x; x[k + 1] = v.y; x[k + 2] = v.z; x[k + 3] = v.w;
+            }
+            float amax = 0.0f;
+#pragma unroll
+            for (int k = 0; k < D; ++k) amax = fmaxf(amax, fabsf(x[k]));
+            const float p2 = pow2_floor(amax), up = pow2_inverse(p2);
+            qs = p2 * kLog2e;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t hi[32], lo[32];
+#pragma unroll
+                for (int k = 0; k < 32; ++k) split2(x[64 * c + 2 * k] * up, x[64 * c + 2 * k + 1] * up, hi[k], lo[k]);
+                TMEM_ST_X32(tl + COL_Q + 32 * c, hi);
+                TMEM_ST_X32(tl + COL_Q + 64 + 32 * c, lo);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&S.q_ready);
+        }
+        // running maximum of dk S (before qs), the same in log2 units, and the sum of weights
+        float top = -INFINITY, top2 = -INFINITY, sum = 0.0f, sigma = 1.0f;
+        const float lazy = kLazy / qs;
+        bool ok = true;
+        for (int j = 0; j < n_blocks; ++j) {
+            const int d = j % TILES;
+            const bool got = mbar_wait_bounded(&S.kv_full[d], (uint32_t)(j / TILES) & 1u) &&
+                             mbar_wait_bounded(&S.s_full[j & 1], (uint32_t)(j >> 1) & 1u);
+            if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t ts = tl + (uint32_t)((j & 1) * KB);
+            uint32_t sv[KB];
+            TMEM_LD_X32(ts, sv);
+            TMEM_LD_X32(ts + 32, (sv + 32));
+            tmem_wait_ld();
+            const int key0 = (first + j) * KB;
+            const int have = S.pages[d];
+            const bool masked = !__all_sync(0xffffffffu, key0 + KB - 1 <= pos && have == (1 << PAGES) - 1);
+            float bmax = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < KB; c += 4) {
+                const float4 k4 = *reinterpret_cast<const float4*>(&S.dk[d][c]);
+                const float f[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = __uint_as_float(sv[c + e]) * f[e];
+                    if (masked && !(key0 + c + e <= pos && ((have >> (c >> 4)) & 1))) x = -INFINITY;
+                    sv[c + e] = __float_as_uint(x);
+                    bmax = fmaxf(bmax, x);
+                }
+            }
+            const float ratio = S.ratio[d];
+            float alpha = ratio;
+            if (top == -INFINITY) {
+                top = bmax;                            // first block with a key: O holds nothing of this row
+                top2 = __fmul_rn(top, qs);
+            } else if (bmax > top + lazy) {
+                const float next = __fmul_rn(bmax, qs);
+                const float f = exp2f(top2 - next);
+                top = bmax;
+                top2 = next;
+                alpha *= f;
+                sum *= f;
+            }
+            const bool rescale = j > 0 && __any_sync(0xffffffffu, alpha != 1.0f);
+            float part_sum[2] = {0.0f, 0.0f};
+            uint32_t hi[32], lo[32];
+#pragma unroll
+            for (int c = 0; c < KB; c += 4) {
+                const float4 v4 = *reinterpret_cast<const float4*>(&S.dv[d][c]);
+                const float f[4] = {v4.x, v4.y, v4.z, v4.w};
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float p = ex2(fmaf(__uint_as_float(sv[c + e]), qs, -top2));
+                    w[e] = p * f[e];
+                    if (masked && !(key0 + c + e <= pos && ((have >> (c >> 4)) & 1))) {
+                        p = 0.0f;
+                        w[e] = 0.0f;
+                    }
+                    part_sum[e & 1] += p;
+                }
+                split2(w[0], w[1], hi[c >> 1], lo[c >> 1]);
+                split2(w[2], w[3], hi[(c >> 1) + 1], lo[(c >> 1) + 1]);
+            }
+            sum += part_sum[0] + part_sum[1];
+            sigma = S.sigma[d];
+            if (rescale) {
+                const bool od = mbar_wait_bounded(&S.o_done, (uint32_t)(j - 1) & 1u);
+                if (!__all_sync(0xffffffffu, od)) { ok = false; break; }
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t ov[32];
+                    TMEM_LD_X32(tl + COL_O + c, ov);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+                    TMEM_ST_X32(tl + COL_O + c, ov);
+                }
+            }
+            TMEM_ST_X32(ts, hi);
+            TMEM_ST_X32(ts + 32, lo);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&S.p_ready[j & 1]);
+        }
+        if (ok && n_blocks > 0) {
+            const bool od = mbar_wait_bounded(&S.o_done, (uint32_t)(n_blocks - 1) & 1u);
+            ok = __all_sync(0xffffffffu, od);
+        }
+        if (!ok) {
+            if (lane == 0) S.err = 1;
+        } else {
+            tc_fence_after();
+            const size_t at = part_index(a, blockIdx.y, h, max_parts, blockIdx.z) + t;
+            if (parts > 1) part_ml[at] = make_float2(top2, sum);
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+                uint32_t ov[16];
+                float o[16];
+                if (n_blocks > 0) {
+                    TMEM_LD_X16(tl + COL_O + c, ov);
+                    tmem_wait_ld();
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = n_blocks > 0 ? __uint_as_float(ov[e]) * sigma : 0.0f;
+                if (parts > 1) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<float4*>(part_o + at * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                } else if (live) {
+                    store_quotients<16>(a, o_at + c, o, sum);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (S.err) {
+        if (threadIdx.x == 0) {
+            record_error(a.err, kDevErrTimeout);
+            for (int j = S.consumed; j < S.issued; ++j)
+                (void)mbar_wait_bounded(&S.raw_full[j % RAW], (uint32_t)(j / RAW) & 1u);
+        }
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+// Joins the parts of a tile and KV head: a warp per query vector, lane l dims [4 l, 4 l + 4).
+__global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const Kv8AttnArgs a, const float* part_o,
+                                                               const float2* part_ml, int max_parts) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.x % a.Hkv, ti = blockIdx.x / a.Hkv;
+    const int G = a.Hq / a.Hkv, R = 128 / G;
+    const int2 tile = a.tiles[ti];
+    pdl_wait();
+    if (tile_bad(a, tile)) return;
+    int slot, first, last;
+    const int pos_last = tile_extent(a, tile, lane, slot);
+    const int parts = part_blocks((pos_last + KB) / KB, max_parts, 0, first, last);
+    if (parts == 1) return;
+    const int t = blockIdx.y * 8 + warp;
+    const int r = t % R, head = t / R, row = tile.x + r;
+    if (head >= G || r >= tile.y || row_bad(a, row) || (a.pos[row] >= 0 && a.slot[row] != slot)) return;
+    float2 ml[kMaxParts];
+    float M = -INFINITY, L = 0.0f;
+    float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < kMaxParts; ++k) {
+        ml[k] = k < parts ? part_ml[part_index(a, ti, h, max_parts, k) + t] : make_float2(-INFINITY, 0.0f);
+        M = fmaxf(M, ml[k].x);
+    }
+#pragma unroll
+    for (int k = 0; k < kMaxParts; ++k) {
+        if (k >= parts) break;
+        const float4 v = reinterpret_cast<const float4*>(part_o + (part_index(a, ti, h, max_parts, k) + t) * D)[lane];
+        // a part without a key (maximum -inf) holds zeros; one whose scores are all NaN, NaN
+        const float f = ml[k].x == M ? 1.0f : exp2f(ml[k].x - M);
+        L = fmaf(ml[k].y, f, L);
+        O.x = fmaf(v.x, f, O.x);
+        O.y = fmaf(v.y, f, O.y);
+        O.z = fmaf(v.z, f, O.z);
+        O.w = fmaf(v.w, f, O.w);
+    }
+    store4(a, ((size_t)row * a.Hq + h * G + head) * D + 4 * lane, O, L);
+}
+
+// Parts that a tile's keys may be cut into: as many as leave the tiles and heads of a call in
+// one wave of a B200's 148 SMs (a CTA fills an SM).
+int max_parts(int n_tiles, int n_kv_heads) {
+    const long long items = (long long)n_tiles * n_kv_heads;
+    return (int)std::max<long long>(1, std::min<long long>(kMaxParts, 148 / items));
+}
+
+template <int FMT>
+cudaError_t launch_prefill(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scratch, cudaStream_t s) {
+    auto kern = kv8_prefill_kernel<FMT>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PfSmem));
+    if (e != cudaSuccess) return e;
+    const int parts = max_parts(a.n_tiles, a.Hkv);
+    float* part_o = static_cast<float*>(scratch);
+    float2* part_ml =
+        parts > 1 ? reinterpret_cast<float2*>(part_o + (size_t)a.n_tiles * a.Hkv * parts * 128 * D) : nullptr;
+    kern<<<dim3(a.Hkv, a.n_tiles, parts), THREADS, sizeof(PfSmem), s>>>(tm, a, part_o, part_ml);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || parts == 1) return e;
+    // launched while the kernel above runs; it waits for that kernel's end before it reads
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.n_tiles * a.Hkv, 16);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv8_prefill_merge_kernel, a, (const float*)part_o, (const float2*)part_ml, parts);
+}
+
+}  // namespace
+}  // namespace fa
+
+extern "C" FA_API size_t fa_op_prefill_attention_kv8_scratch_bytes(int n_tiles, int n_heads, int n_kv_heads) {
+    if (n_tiles <= 0 || n_kv_heads <= 0 || n_heads < n_kv_heads || n_heads % n_kv_heads) return 0;
+    const int parts = fa::max_parts(n_tiles, n_kv_heads);
+    return parts == 1 ? 0 : (size_t)n_tiles * n_kv_heads * parts * 128 * (fa::D * sizeof(float) + sizeof(float2));
+}
+
+extern "C" FA_API int fa_op_prefill_attention_kv8(const float* q, int M, int n_heads, int n_kv_heads, const int* pos,
+                                                  const int* slot, const int* bt, int bt_stride, int n_pages,
+                                                  int format, const void* pool_layer, const int* tiles, int n_tiles,
+                                                  void* scratch, size_t scratch_bytes, uint16_t* out16,
+                                                  uint16_t* out16_lo, float* out32, int* err, void* stream) {
+    using namespace fa;
+    Kv8AttnArgs a{q, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages,
+                  static_cast<const unsigned char*>(pool_layer), reinterpret_cast<const int2*>(tiles), n_tiles,
+                  reinterpret_cast<__half*>(out16), reinterpret_cast<__half*>(out16_lo), out32, err};
+    if (!tiles || n_tiles <= 0 || (reinterpret_cast<uintptr_t>(tiles) & 7))
+        return report_op_error(FA_ERR_INVALID_ARG, "fa_op_prefill_attention_kv8: tiles missing or not 8-byte aligned");
+    if (int rc = kv8_attention_check("fa_op_prefill_attention_kv8", a, format, scratch, scratch_bytes,
+                                     fa_op_prefill_attention_kv8_scratch_bytes(n_tiles, n_heads, n_kv_heads)))
+        return rc;
+    if (n_tiles > 65535)
+        return report_op_error(FA_ERR_CAPACITY, "fa_op_prefill_attention_kv8: more than 65535 tiles");
+    CUtensorMap tm;
+    if (!make_kv8_tile_map(&tm, pool_layer, (long long)n_pages * n_kv_heads * (kTileBytes / 128)))
+        return report_op_error(FA_ERR_CUDA, "fa_op_prefill_attention_kv8: cannot build the page-pool tensor map");
+    const cudaError_t e = format == FA_KV8_INT8 ? launch_prefill<kInt8>(tm, a, scratch, (cudaStream_t)stream)
+                                                : launch_prefill<kE4m3>(tm, a, scratch, (cudaStream_t)stream);
+    if (e == cudaSuccess) return FA_OK;
+    cudaGetLastError();
+    return report_op_error(FA_ERR_CUDA, (std::string("fa_op_prefill_attention_kv8: ") + cudaGetErrorString(e)).c_str());
+}
