@@ -15,11 +15,13 @@
 // 1024 cycles that its MMAs take.
 // The running maximum is lazy (O is rescaled when a block exceeds it by 2^8 or sigma grows).
 //
-// Roles (320 threads): warp 0 issues the page copies (one TMA box and one bulk copy of scales
-// per page) into a ring of raw blocks; warps 6-9 expand a raw block into the f16 K / V tiles of
-// a second ring, with each key's factors; warp 1 holds TMEM and issues the MMAs; warps 2-5
-// load Q, run the softmax and write the outputs. Every mbarrier wait is bounded; on a timeout
-// the CTA records the error, drains its copies and MMAs and frees TMEM.
+// Roles (512 threads): warp 0 issues the page copies (one TMA box and one bulk copy of scales
+// per page) into a ring of raw blocks; warps 4-7 expand a raw block into the f16 K / V tiles of
+// a second ring, with each key's factors; warp 1 holds TMEM and issues the MMAs; warps 8-11 and
+// 12-15 load Q, run the softmax of the even and of the odd blocks and write the outputs. Every
+// mbarrier wait is bounded; on a timeout the CTA records the error, drains its copies and MMAs
+// and frees TMEM.
+#include "k_attn_body.cuh"
 #include "k_kv8_attn.cuh"
 
 #include <algorithm>
@@ -34,11 +36,12 @@ constexpr int KB = 64;                        // keys per block
 constexpr int PAGES = KB / kPageTokens;
 constexpr int RAW = 3;                        // raw ring (8-bit blocks)
 constexpr int TILES = 4;                      // f16 ring
-constexpr int THREADS = 320;
+constexpr int THREADS = 512;
 constexpr int kMaxParts = 16;                 // key ranges of one tile and head
 constexpr int kMinPartBlocks = 8;
-constexpr uint32_t TMEM_COLS = 512;           // S0 [0,64) S1 [64,128) O [128,256) Q hi [256,320) Q lo [320,384)
-constexpr uint32_t COL_O = 128, COL_Q = 256;
+// TMEM columns: S / w of even and odd blocks [0, 64), [64, 128), their O [128, 256), [256, 384),
+// Q hi [384, 448), Q lo [448, 512)
+constexpr uint32_t TMEM_COLS = 512, COL_O = 128, COL_Q = 384;
 constexpr float kLazy = 8.0f;                 // log2 units
 
 struct PfSmem {
@@ -49,7 +52,7 @@ struct PfSmem {
     float dk[TILES][KB];                      // K scales
     float dv[TILES][KB];                      // V scales / sigma
     float sigma[TILES];
-    float ratio[TILES];                       // sigma before the block / sigma
+    float odd[3][128];                        // the odd blocks' maximum, sum and sigma of each query vector
     int raw_pages[RAW];                       // bit q: page q of the block was copied
     int pages[TILES];
     uint64_t raw_full[RAW];
@@ -59,7 +62,8 @@ struct PfSmem {
     uint64_t s_full[2];
     uint64_t p_ready[2];
     uint64_t q_ready;
-    uint64_t o_done;
+    uint64_t o_done[2];
+    uint64_t odd_done;
     uint64_t drain;
     uint32_t tmem_base;
     int pos_last;                             // last key any row of the tile attends to; -1: none
@@ -90,6 +94,10 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    return attn::ffma2(a, make_float2(1.0f, 1.0f), b);
 }
 
 // The key blocks [first, last) of part `part` of an item of nb blocks cut into at most
@@ -152,9 +160,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int s = 0; s < 2; ++s) {
             mbar_init(&S.s_full[s], 1);
             mbar_init(&S.p_ready[s], 128);
+            mbar_init(&S.o_done[s], 1);
         }
-        mbar_init(&S.q_ready, 128);
-        mbar_init(&S.o_done, 1);
+        mbar_init(&S.q_ready, 256);
+        mbar_init(&S.odd_done, 128);
         mbar_init(&S.drain, 1);
         S.err = 0;
         S.issued = 0;
@@ -252,15 +261,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const int jp = j - 1, sp = jp % TILES;
                     if (!mbar_wait_bounded(&S.p_ready[jp & 1], (uint32_t)(jp >> 1) & 1u)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t d_p = tmem + (uint32_t)((jp & 1) * KB);
+                    const uint32_t d_p = tmem + (uint32_t)((jp & 1) * KB), d_o = tmem + COL_O + (uint32_t)((jp & 1) * D);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
                         const uint64_t db = smem_desc_mn128(&S.v[sp][0][kk * 16 * 64], KB * 64 * 2);
-                        tc_mma_f16_ts(tmem + COL_O, d_p + 8 * kk, db, kIdPV, (jp > 0 || kk > 0) ? 1u : 0u);
-                        tc_mma_f16_ts(tmem + COL_O, d_p + 32 + 8 * kk, db, kIdPV, 1u);
+                        tc_mma_f16_ts(d_o, d_p + 8 * kk, db, kIdPV, (jp > 1 || kk > 0) ? 1u : 0u);
+                        tc_mma_f16_ts(d_o, d_p + 32 + 8 * kk, db, kIdPV, 1u);
                     }
                     tc_commit(&S.kv_empty[sp]);
-                    tc_commit(&S.o_done);
+                    tc_commit(&S.o_done[jp & 1]);
                 }
             }
             if (!ok) S.err = 1;
@@ -268,9 +277,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!mbar_wait_bounded(&S.drain, 0)) S.err = 1;
         }
         __syncwarp();
-    } else if (warp >= 6) {
+    } else if (warp >= 4 && warp < 8) {
         // expansion: thread c takes 16-byte chunk c % 8 of tokens c / 8, c / 8 + 16, ..., K and V
-        const int ct = threadIdx.x - 192, cw = warp - 6;
+        const int ct = threadIdx.x - 128, cw = warp - 4;
         const int chunk = ct & 7;
         uint32_t run = 0;                              // exponent field of sigma
         bool ok = true;
@@ -295,7 +304,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                 top = max(top, x == 0x7f800000u ? 0u : x);
             }
             top = max(__reduce_max_sync(0xffffffffu, top), 11u << 23);
-            const uint32_t old = run;
             run = max(run, top);
             if (cw == 0) {
                 const float sigma = __uint_as_float(run - (6u << 23)), inv = pow2_inverse(sigma);
@@ -307,7 +315,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 if (lane == 0) {
                     S.sigma[d] = sigma;
-                    S.ratio[d] = j == 0 ? 1.0f : __uint_as_float(old - (6u << 23)) * inv;
                     S.pages[d] = have;
                 }
             }
@@ -342,8 +349,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
         }
         if (!ok && lane == 0) S.err = 1;
-    } else {
-        // thread t owns TMEM lane t = query vector t (a warp may only touch lanes 32 * (warp % 4) ..)
+    } else if (warp >= 8) {
+        // Warps 8-11 the even blocks, 12-15 the odd ones, each with its own running maximum, sum
+        // and O: while one group works on S of a block, the MMAs make the other's. Thread t of a
+        // group owns TMEM lane t = query vector t (a warp may only touch lanes 32 * (warp % 4) ..).
+        const int odd = warp >= 12 ? 1 : 0;
         const int quarter = warp & 3;
         const int t = 32 * quarter + lane;
         const int r = t % R, head = t / R;
@@ -353,7 +363,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (live) {
             pos = a.pos[row];
             if (row_bad(a, row) || (pos >= 0 && a.slot[row] != slot)) {
-                if (h == 0 && blockIdx.z == 0 && head == 0) record_error(a.err, kDevErrBadLen);
+                if (h == 0 && blockIdx.z == 0 && head == 0 && !odd) record_error(a.err, kDevErrBadLen);
                 live = false;
                 pos = pos_last;
             }
@@ -362,25 +372,25 @@ __global__ void __launch_bounds__(THREADS, 1)
         const size_t o_at = ((size_t)row * a.Hq + h * G + head) * D;
         float qs = 0.0f;                               // takes dk S to log2 units
         if (n_blocks > 0) {
-            float x[D];
-#pragma unroll
-            for (int k = 0; k < D; k += 4) {
-                const float4 v = live ? *reinterpret_cast<const float4*>(a.q + o_at + k) : make_float4(0, 0, 0, 0);
-                x[k] = v.x; x[k + 1] = v.y; x[k + 2] = v.z; x[k + 3] = v.w;
-            }
+            // each group writes half of the dims of Q
+            const float4* src = reinterpret_cast<const float4*>(a.q + o_at);
             float amax = 0.0f;
-#pragma unroll
-            for (int k = 0; k < D; ++k) amax = fmaxf(amax, fabsf(x[k]));
+#pragma unroll 8
+            for (int k = 0; k < D / 4; ++k) {
+                const float4 v = live ? src[k] : make_float4(0, 0, 0, 0);
+                amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+            }
             const float p2 = pow2_floor(amax), up = pow2_inverse(p2);
             qs = p2 * kLog2e;
+            uint32_t hi[32], lo[32];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t hi[32], lo[32];
-#pragma unroll
-                for (int k = 0; k < 32; ++k) split2(x[64 * c + 2 * k] * up, x[64 * c + 2 * k + 1] * up, hi[k], lo[k]);
-                TMEM_ST_X32(tl + COL_Q + 32 * c, hi);
-                TMEM_ST_X32(tl + COL_Q + 64 + 32 * c, lo);
+            for (int k = 0; k < 16; ++k) {
+                const float4 v = live ? src[16 * odd + k] : make_float4(0, 0, 0, 0);
+                split2(v.x * up, v.y * up, hi[2 * k], lo[2 * k]);
+                split2(v.z * up, v.w * up, hi[2 * k + 1], lo[2 * k + 1]);
             }
+            TMEM_ST_X32(tl + COL_Q + 32 * odd, hi);
+            TMEM_ST_X32(tl + COL_Q + 64 + 32 * odd, lo);
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&S.q_ready);
@@ -388,14 +398,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         // running maximum of dk S (before qs), the same in log2 units, and the sum of weights
         float top = -INFINITY, top2 = -INFINITY, sum = 0.0f, sigma = 1.0f;
         const float lazy = kLazy / qs;
+        const uint32_t ts = tl + (uint32_t)(odd * KB), to = tl + COL_O + (uint32_t)(odd * D);
         bool ok = true;
-        for (int j = 0; j < n_blocks; ++j) {
+        for (int j = odd; j < n_blocks; j += 2) {
             const int d = j % TILES;
             const bool got = mbar_wait_bounded(&S.kv_full[d], (uint32_t)(j / TILES) & 1u) &&
-                             mbar_wait_bounded(&S.s_full[j & 1], (uint32_t)(j >> 1) & 1u);
+                             mbar_wait_bounded(&S.s_full[odd], (uint32_t)(j >> 1) & 1u);
             if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
             tc_fence_after();
-            const uint32_t ts = tl + (uint32_t)((j & 1) * KB);
             uint32_t sv[KB];
             TMEM_LD_X32(ts, sv);
             TMEM_LD_X32(ts + 32, (sv + 32));
@@ -403,21 +413,36 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int key0 = (first + j) * KB;
             const int have = S.pages[d];
             const bool masked = !__all_sync(0xffffffffu, key0 + KB - 1 <= pos && have == (1 << PAGES) - 1);
+            const float4* dk = reinterpret_cast<const float4*>(S.dk[d]);
             float bmax = -INFINITY;
 #pragma unroll
             for (int c = 0; c < KB; c += 4) {
-                const float4 k4 = *reinterpret_cast<const float4*>(&S.dk[d][c]);
-                const float f[4] = {k4.x, k4.y, k4.z, k4.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = __uint_as_float(sv[c + e]) * f[e];
-                    if (masked && !(key0 + c + e <= pos && ((have >> (c >> 4)) & 1))) x = -INFINITY;
-                    sv[c + e] = __float_as_uint(x);
-                    bmax = fmaxf(bmax, x);
-                }
+                const float4 f = dk[c >> 2];
+                const float2 x = attn::fmul2(make_float2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), make_float2(f.x, f.y));
+                const float2 y = attn::fmul2(make_float2(__uint_as_float(sv[c + 2]), __uint_as_float(sv[c + 3])), make_float2(f.z, f.w));
+                sv[c] = __float_as_uint(x.x);
+                sv[c + 1] = __float_as_uint(x.y);
+                sv[c + 2] = __float_as_uint(y.x);
+                sv[c + 3] = __float_as_uint(y.y);
             }
-            const float ratio = S.ratio[d];
-            float alpha = ratio;
+            uint32_t seen[2] = {~0u, ~0u};             // keys of the block that the row attends to
+            if (masked) {
+                const int n = min(max(pos + 1 - key0, 0), KB);
+                uint64_t bits = n == KB ? ~0ull : (1ull << n) - 1;
+#pragma unroll
+                for (int q = 0; q < PAGES; ++q)
+                    if (!((have >> q) & 1)) bits &= ~(0xffffull << (16 * q));
+                seen[0] = (uint32_t)bits;
+                seen[1] = (uint32_t)(bits >> 32);
+#pragma unroll
+                for (int c = 0; c < KB; ++c)
+                    if (!((seen[c >> 5] >> (c & 31)) & 1)) sv[c] = 0xff800000u;        // -inf
+            }
+#pragma unroll
+            for (int c = 0; c < KB; ++c) bmax = fmaxf(bmax, __uint_as_float(sv[c]));
+            const float next_sigma = S.sigma[d];
+            float alpha = j > 1 ? sigma * pow2_inverse(next_sigma) : 1.0f;
+            sigma = next_sigma;
             if (top == -INFINITY) {
                 top = bmax;                            // first block with a key: O holds nothing of this row
                 top2 = __fmul_rn(top, qs);
@@ -429,69 +454,95 @@ __global__ void __launch_bounds__(THREADS, 1)
                 alpha *= f;
                 sum *= f;
             }
-            const bool rescale = j > 0 && __any_sync(0xffffffffu, alpha != 1.0f);
-            float part_sum[2] = {0.0f, 0.0f};
-            uint32_t hi[32], lo[32];
-#pragma unroll
-            for (int c = 0; c < KB; c += 4) {
-                const float4 v4 = *reinterpret_cast<const float4*>(&S.dv[d][c]);
-                const float f[4] = {v4.x, v4.y, v4.z, v4.w};
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float p = ex2(fmaf(__uint_as_float(sv[c + e]), qs, -top2));
-                    w[e] = p * f[e];
-                    if (masked && !(key0 + c + e <= pos && ((have >> (c >> 4)) & 1))) {
-                        p = 0.0f;
-                        w[e] = 0.0f;
-                    }
-                    part_sum[e & 1] += p;
-                }
-                split2(w[0], w[1], hi[c >> 1], lo[c >> 1]);
-                split2(w[2], w[3], hi[(c >> 1) + 1], lo[(c >> 1) + 1]);
-            }
-            sum += part_sum[0] + part_sum[1];
-            sigma = S.sigma[d];
-            if (rescale) {
-                const bool od = mbar_wait_bounded(&S.o_done, (uint32_t)(j - 1) & 1u);
+            if (j > 1 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                const bool od = mbar_wait_bounded(&S.o_done[odd], (uint32_t)((j >> 1) - 1) & 1u);
                 if (!__all_sync(0xffffffffu, od)) { ok = false; break; }
                 tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t ov[32];
-                    TMEM_LD_X32(tl + COL_O + c, ov);
+                for (int c = 0; c < D; c += 16) {
+                    uint32_t ov[16];
+                    TMEM_LD_X16(to + c, ov);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-                    TMEM_ST_X32(tl + COL_O + c, ov);
+                    for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+                    TMEM_ST_X16(to + c, ov);
                 }
             }
-            TMEM_ST_X32(ts, hi);
-            TMEM_ST_X32(ts + 32, lo);
+            const float4* dv = reinterpret_cast<const float4*>(S.dv[d]);
+            const float2 qs2 = make_float2(qs, qs), neg = make_float2(-top2, -top2), minus = make_float2(-1.0f, -1.0f);
+            float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                    const float4 f = dv[8 * half + (c >> 2)];
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const int i = 32 * half + c + e;
+                        const float2 x = attn::ffma2(make_float2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), qs2, neg);
+                        float2 p = make_float2(ex2(x.x), ex2(x.y));
+                        float2 w = attn::fmul2(p, e ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
+                        if (masked) {                  // by selection: the maximum may be -inf, a scale NaN
+                            const uint32_t in = seen[half] >> (c + e);
+                            p = make_float2(in & 1 ? p.x : 0.0f, in & 2 ? p.y : 0.0f);
+                            w = make_float2(in & 1 ? w.x : 0.0f, in & 2 ? w.y : 0.0f);
+                        }
+                        acc = add2(acc, p);
+                        const uint32_t hw = pack2(w.x, w.y);
+                        const float2 rest = attn::ffma2(h2_to_f2(hw), minus, w);
+                        hi[(c + e) >> 1] = hw;
+                        lo[(c + e) >> 1] = pack2(rest.x, rest.y);
+                    }
+                }
+                TMEM_ST_X16(ts + 16 * half, hi);
+                TMEM_ST_X16(ts + 32 + 16 * half, lo);
+            }
+            sum += acc.x + acc.y;
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&S.p_ready[j & 1]);
+            mbar_arrive(&S.p_ready[odd]);
         }
-        if (ok && n_blocks > 0) {
-            const bool od = mbar_wait_bounded(&S.o_done, (uint32_t)(n_blocks - 1) & 1u);
+        // the group's last product: block n_blocks - 1 or n_blocks - 2
+        const int mine = (n_blocks + 1 - odd) >> 1;    // blocks of this group
+        if (ok && mine > 0) {
+            const bool od = mbar_wait_bounded(&S.o_done[odd], (uint32_t)(mine - 1) & 1u);
             ok = __all_sync(0xffffffffu, od);
+        }
+        if (odd) {
+            S.odd[0][t] = top2;
+            S.odd[1][t] = sum;
+            S.odd[2][t] = sigma;
+            tc_fence_before();
+            mbar_arrive(&S.odd_done);
+        } else if (ok) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.odd_done, 0));
         }
         if (!ok) {
             if (lane == 0) S.err = 1;
-        } else {
+        } else if (!odd) {
+            // the two groups joined: out = (O0 f0 + O1 f1) / (sum0 f0 + sum1 f1)
             tc_fence_after();
+            const float other = S.odd[0][t];
+            const float best = fmaxf(top2, other);
+            float f0 = top2 == best ? 1.0f : exp2f(top2 - best), f1 = other == best ? 1.0f : exp2f(other - best);
+            sum = sum * f0 + S.odd[1][t] * f1;
+            f0 *= sigma;
+            f1 *= S.odd[2][t];
             const size_t at = part_index(a, blockIdx.y, h, max_parts, blockIdx.z) + t;
-            if (parts > 1) part_ml[at] = make_float2(top2, sum);
+            if (parts > 1) part_ml[at] = make_float2(best, sum);
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
-                uint32_t ov[16];
+                uint32_t ov[16], ow[16];
                 float o[16];
-                if (n_blocks > 0) {
-                    TMEM_LD_X16(tl + COL_O + c, ov);
-                    tmem_wait_ld();
-                }
+                if (n_blocks > 0) TMEM_LD_X16(tl + COL_O + c, ov);
+                if (n_blocks > 1) TMEM_LD_X16(tl + COL_O + D + c, ow);
+                tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = n_blocks > 0 ? __uint_as_float(ov[e]) * sigma : 0.0f;
+                for (int e = 0; e < 16; ++e) {
+                    o[e] = n_blocks > 0 ? __uint_as_float(ov[e]) * f0 : 0.0f;
+                    if (n_blocks > 1) o[e] = fmaf(__uint_as_float(ow[e]), f1, o[e]);
+                }
                 if (parts > 1) {
 #pragma unroll
                     for (int e = 0; e < 16; e += 4)
