@@ -96,6 +96,32 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one;
+}
+// tc_mma_f16_ts and tc_commit by the lane whose `one` is set.
+__device__ __forceinline__ void tc_mma_f16_ts_if(uint32_t one, uint32_t tmem_d, uint32_t tmem_a, uint64_t db,
+                                                 uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit_if(uint32_t one, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(one)
+        : "memory");
+}
+
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return attn::ffma2(a, make_float2(1.0f, 1.0f), b);
 }
@@ -142,7 +168,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                        float2* part_ml) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     PfSmem& S = *reinterpret_cast<PfSmem*>(smem_raw);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
     const int h = blockIdx.x, max_parts = gridDim.z;
     const int G = a.Hq / a.Hkv, R = 128 / G;
     pdl_trigger();
@@ -190,7 +216,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = S.tmem_base;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, S.tmem_base, 0);
     const int pos_last = S.pos_last, slot = S.slot;
     int first = 0, last = 0;
     const int parts = part_blocks((pos_last + KB) / KB, max_parts, blockIdx.z, first, last);
@@ -238,43 +264,52 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (!ok && lane == 0) S.err = 1;
     } else if (warp == 1) {
-        if (lane == 0 && n_blocks > 0) {
+        if (n_blocks > 0) {
+            // The whole warp runs the loop and one lane issues: the operands of an MMA then stay in
+            // uniform registers (issued from a divergent branch, moving them there took longer than
+            // the MMAs: 2070 cycles a block).
             constexpr uint32_t kIdS = idesc_f16(128, KB, false, false);
             constexpr uint32_t kIdPV = idesc_f16(128, D, false, true);
-            bool ok = mbar_wait_bounded(&S.q_ready, 0);
+            const uint32_t one = elect_one();
+            const uint64_t k_desc = smem_desc_k128(S.k[0][0]), v_desc = smem_desc_mn128(S.v[0][0], KB * 64 * 2);
+            bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.q_ready, 0));
             tc_fence_after();
             for (int j = 0; ok && j <= n_blocks; ++j) {
                 if (j < n_blocks) {
                     const int s = j % TILES;
-                    if (!mbar_wait_bounded(&S.kv_full[s], (uint32_t)(j / TILES) & 1u)) { ok = false; break; }
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.kv_full[s], (uint32_t)(j / TILES) & 1u));
+                    if (!ok) break;
                     tc_fence_after();
                     const uint32_t d_s = tmem + (uint32_t)((j & 1) * KB);
+                    const uint64_t db = k_desc + (uint32_t)(s * (int)sizeof(S.k[0]) >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk) {
-                        const uint64_t db = smem_desc_k128(S.k[s][kk >> 2]) + ((uint32_t)((kk & 3) * 32) >> 4);
-                        tc_mma_f16_ts(d_s, tmem + COL_Q + 8 * kk, db, kIdS, kk > 0 ? 1u : 0u);
-                        tc_mma_f16_ts(d_s, tmem + COL_Q + 64 + 8 * kk, db, kIdS, 1u);
+                        const uint64_t at = db + ((kk >> 2) * (int)sizeof(S.k[0][0]) + (kk & 3) * 32) / 16;
+                        tc_mma_f16_ts_if(one, d_s, tmem + COL_Q + 8 * kk, at, kIdS, kk > 0 ? 1u : 0u);
+                        tc_mma_f16_ts_if(one, d_s, tmem + COL_Q + 64 + 8 * kk, at, kIdS, 1u);
                     }
-                    tc_commit(&S.s_full[j & 1]);
+                    tc_commit_if(one, &S.s_full[j & 1]);
                 }
                 if (j >= 1) {
                     const int jp = j - 1, sp = jp % TILES;
-                    if (!mbar_wait_bounded(&S.p_ready[jp & 1], (uint32_t)(jp >> 1) & 1u)) { ok = false; break; }
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.p_ready[jp & 1], (uint32_t)(jp >> 1) & 1u));
+                    if (!ok) break;
                     tc_fence_after();
                     const uint32_t d_p = tmem + (uint32_t)((jp & 1) * KB), d_o = tmem + COL_O + (uint32_t)((jp & 1) * D);
+                    const uint64_t db = v_desc + (uint32_t)(sp * (int)sizeof(S.v[0]) >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
-                        const uint64_t db = smem_desc_mn128(&S.v[sp][0][kk * 16 * 64], KB * 64 * 2);
-                        tc_mma_f16_ts(d_o, d_p + 8 * kk, db, kIdPV, (jp > 1 || kk > 0) ? 1u : 0u);
-                        tc_mma_f16_ts(d_o, d_p + 32 + 8 * kk, db, kIdPV, 1u);
+                        const uint64_t at = db + kk * 16 * 64 * 2 / 16;
+                        tc_mma_f16_ts_if(one, d_o, d_p + 8 * kk, at, kIdPV, (jp > 1 || kk > 0) ? 1u : 0u);
+                        tc_mma_f16_ts_if(one, d_o, d_p + 32 + 8 * kk, at, kIdPV, 1u);
                     }
-                    tc_commit(&S.kv_empty[sp]);
-                    tc_commit(&S.o_done[jp & 1]);
+                    tc_commit_if(one, &S.kv_empty[sp]);
+                    tc_commit_if(one, &S.o_done[jp & 1]);
                 }
             }
-            if (!ok) S.err = 1;
-            tc_commit(&S.drain);
-            if (!mbar_wait_bounded(&S.drain, 0)) S.err = 1;
+            tc_commit_if(one, &S.drain);
+            if (!mbar_wait_bounded(&S.drain, 0)) ok = false;
+            if (!ok && lane == 0) S.err = 1;
         }
         __syncwarp();
     } else if (warp >= 4 && warp < 8) {
