@@ -50,13 +50,9 @@ __device__ __forceinline__ float pow2_floor(float x) {
 }
 __device__ __forceinline__ float pow2_inverse(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
 
-// N consecutive outputs x / l from offset o (a multiple of 4; of 8 for N = 16): 0 where no
-// token takes part (l = 0).
+// N consecutive outputs from offset o, a multiple of 4.
 template <int N>
-__device__ __forceinline__ void store_quotients(const Kv8AttnArgs& a, size_t o, const float (&x)[N], float l) {
-    float v[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = l == 0.0f ? 0.0f : x[k] / l;
+__device__ __forceinline__ void store_values(const Kv8AttnArgs& a, size_t o, const float (&v)[N]) {
     if (a.out32) {
 #pragma unroll
         for (int k = 0; k < N; k += 4)
@@ -78,6 +74,14 @@ __device__ __forceinline__ void store_quotients(const Kv8AttnArgs& a, size_t o, 
             if (a.out16_lo) *reinterpret_cast<uint2*>(a.out16_lo + o + k) = make_uint2(lo[0], lo[1]);
         }
     }
+}
+// The outputs x / l: 0 where no token takes part (l = 0).
+template <int N>
+__device__ __forceinline__ void store_quotients(const Kv8AttnArgs& a, size_t o, const float (&x)[N], float l) {
+    float v[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = l == 0.0f ? 0.0f : x[k] / l;
+    store_values<N>(a, o, v);
 }
 __device__ __forceinline__ void store16(const Kv8AttnArgs& a, size_t o, const float (&x)[16], float l) {
     store_quotients<16>(a, o, x, l);

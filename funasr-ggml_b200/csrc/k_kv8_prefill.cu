@@ -39,31 +39,34 @@ constexpr int TILES = 4;                      // f16 ring
 constexpr int THREADS = 512;
 constexpr int kMaxParts = 16;                 // key ranges of one tile and head
 constexpr int kMinPartBlocks = 8;
-// TMEM columns: S / w of even and odd blocks [0, 64), [64, 128), their O [128, 256), [256, 384),
-// Q hi [384, 448), Q lo [448, 512)
-constexpr uint32_t TMEM_COLS = 512, COL_O = 128, COL_Q = 384;
-constexpr float kLazy = 8.0f;                 // log2 units
+// TMEM columns: S / w of block j at 64 (j % 3), O of the even blocks [192, 320) and of the odd
+// ones [320, 448), Q hi [448, 512)
+constexpr int SBUF = 3;
+constexpr uint32_t TMEM_COLS = 512, COL_O = 192, COL_Q = 448;
+constexpr float kLazy = 11.0f;                // log2 units
+constexpr uint32_t kSigmaShift = 3;           // the largest V scale over sigma is 2^3 to 2^4: w < 2^15
 
 struct PfSmem {
     __half k[TILES][2][KB * 64];              // [dim half][64 tokens][64 dims], 128 B swizzle
     __half v[TILES][2][KB * 64];
+    __half q_lo[2][128 * 64];                 // [dim half][128 query vectors][64 dims], swizzled
     unsigned char raw[RAW][PAGES][2 * kPartBytes];
     float raw_scales[RAW][PAGES][2 * kPageTokens];
     float dk[TILES][KB];                      // K scales
     float dv[TILES][KB];                      // V scales / sigma
     float sigma[TILES];
-    float odd[3][128];                        // the odd blocks' maximum, sum and sigma of each query vector
+    float qs[128];                            // what takes dk S of a query vector to log2 units
+    float state[2][3][128];                   // even / odd blocks' maximum, sum and sigma of each vector
     int raw_pages[RAW];                       // bit q: page q of the block was copied
     int pages[TILES];
     uint64_t raw_full[RAW];
     uint64_t raw_empty[RAW];
     uint64_t kv_full[TILES];
     uint64_t kv_empty[TILES];
-    uint64_t s_full[2];
-    uint64_t p_ready[2];
+    uint64_t s_full[SBUF];
+    uint64_t p_ready[SBUF];
     uint64_t q_ready;
     uint64_t o_done[2];
-    uint64_t odd_done;
     uint64_t drain;
     uint32_t tmem_base;
     int pos_last;                             // last key any row of the tile attends to; -1: none
@@ -102,7 +105,7 @@ __device__ __forceinline__ uint32_t elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
     return one;
 }
-// tc_mma_f16_ts and tc_commit by the lane whose `one` is set.
+// tc_mma_f16_ts, tc_mma_f16 and tc_commit by the lane whose `one` is set.
 __device__ __forceinline__ void tc_mma_f16_ts_if(uint32_t one, uint32_t tmem_d, uint32_t tmem_a, uint64_t db,
                                                  uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -111,6 +114,16 @@ __device__ __forceinline__ void tc_mma_f16_ts_if(uint32_t one, uint32_t tmem_d, 
         "setp.ne.b32 q, %5, 0;\n\t"
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
         "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_f16_if(uint32_t one, uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
+                                              uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(one)
         : "memory");
 }
 __device__ __forceinline__ void tc_commit_if(uint32_t one, uint64_t* bar) {
@@ -125,6 +138,9 @@ __device__ __forceinline__ void tc_commit_if(uint32_t one, uint64_t* bar) {
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return attn::ffma2(a, make_float2(1.0f, 1.0f), b);
 }
+
+// A barrier of warps 8-15.
+__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // The key blocks [first, last) of part `part` of an item of nb blocks cut into at most
 // max_parts, and the number of parts.
@@ -183,13 +199,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(&S.kv_full[s], 4);
             mbar_init(&S.kv_empty[s], 1);
         }
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < SBUF; ++s) {
             mbar_init(&S.s_full[s], 1);
             mbar_init(&S.p_ready[s], 128);
-            mbar_init(&S.o_done[s], 1);
         }
+        mbar_init(&S.o_done[0], 1);
+        mbar_init(&S.o_done[1], 1);
         mbar_init(&S.q_ready, 256);
-        mbar_init(&S.odd_done, 128);
         mbar_init(&S.drain, 1);
         S.err = 0;
         S.issued = 0;
@@ -204,6 +220,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     const int2 tile = a.tiles[blockIdx.y];
     const bool bad = tile_bad(a, tile);
+    // warps 8-15: 16 query vectors each, lane l dims [4 l, 4 l + 4); vectors without a row are zero
+    float4 qv[16];
+    if (warp >= 8) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int v = (warp - 8) * 16 + k, r = v % R, head = v / R;
+            qv[k] = !bad && head < G && r < tile.y
+                        ? reinterpret_cast<const float4*>(a.q + ((size_t)(tile.x + r) * a.Hq + h * G + head) * D)[lane]
+                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    }
     if (warp == 2) {
         int slot = 0;
         const int last = bad ? -1 : tile_extent(a, tile, lane, slot);
@@ -272,39 +299,42 @@ __global__ void __launch_bounds__(THREADS, 1)
             constexpr uint32_t kIdPV = idesc_f16(128, D, false, true);
             const uint32_t one = elect_one();
             const uint64_t k_desc = smem_desc_k128(S.k[0][0]), v_desc = smem_desc_mn128(S.v[0][0], KB * 64 * 2);
+            const uint64_t q_desc = smem_desc_k128(S.q_lo[0]);
             bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.q_ready, 0));
-            tc_fence_after();
-            for (int j = 0; ok && j <= n_blocks; ++j) {
-                if (j < n_blocks) {
-                    const int s = j % TILES;
-                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.kv_full[s], (uint32_t)(j / TILES) & 1u));
+            // S of block j + 2 before O of block j: with three S buffers it needs only block j - 1's
+            // product, so a group finds its next S ready when it ends a block
+            for (int i = 0; ok && i < n_blocks + 2; ++i) {
+                if (i < n_blocks) {
+                    const int s = i % TILES;
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.kv_full[s], (uint32_t)(i / TILES) & 1u));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t d_s = tmem + (uint32_t)((j & 1) * KB);
+                    const uint32_t d_s = tmem + (uint32_t)(i % SBUF * KB);
                     const uint64_t db = k_desc + (uint32_t)(s * (int)sizeof(S.k[0]) >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk) {
-                        const uint64_t at = db + ((kk >> 2) * (int)sizeof(S.k[0][0]) + (kk & 3) * 32) / 16;
+                        const uint32_t in_row = (kk & 3) * 32 / 16;
+                        const uint64_t at = db + (kk >> 2) * (int)sizeof(S.k[0][0]) / 16 + in_row;
                         tc_mma_f16_ts_if(one, d_s, tmem + COL_Q + 8 * kk, at, kIdS, kk > 0 ? 1u : 0u);
-                        tc_mma_f16_ts_if(one, d_s, tmem + COL_Q + 64 + 8 * kk, at, kIdS, 1u);
+                        tc_mma_f16_if(one, d_s, q_desc + (kk >> 2) * (int)sizeof(S.q_lo[0]) / 16 + in_row, at, kIdS, 1u);
                     }
-                    tc_commit_if(one, &S.s_full[j & 1]);
+                    tc_commit_if(one, &S.s_full[i % SBUF]);
                 }
-                if (j >= 1) {
-                    const int jp = j - 1, sp = jp % TILES;
-                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.p_ready[jp & 1], (uint32_t)(jp >> 1) & 1u));
+                if (i >= 2) {
+                    const int j = i - 2, s = j % TILES;
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.p_ready[j % SBUF], (uint32_t)(j / SBUF) & 1u));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t d_p = tmem + (uint32_t)((jp & 1) * KB), d_o = tmem + COL_O + (uint32_t)((jp & 1) * D);
-                    const uint64_t db = v_desc + (uint32_t)(sp * (int)sizeof(S.v[0]) >> 4);
+                    const uint32_t d_p = tmem + (uint32_t)(j % SBUF * KB), d_o = tmem + COL_O + (uint32_t)((j & 1) * D);
+                    const uint64_t db = v_desc + (uint32_t)(s * (int)sizeof(S.v[0]) >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
                         const uint64_t at = db + kk * 16 * 64 * 2 / 16;
-                        tc_mma_f16_ts_if(one, d_o, d_p + 8 * kk, at, kIdPV, (jp > 1 || kk > 0) ? 1u : 0u);
+                        tc_mma_f16_ts_if(one, d_o, d_p + 8 * kk, at, kIdPV, (j > 1 || kk > 0) ? 1u : 0u);
                         tc_mma_f16_ts_if(one, d_o, d_p + 32 + 8 * kk, at, kIdPV, 1u);
                     }
-                    tc_commit_if(one, &S.kv_empty[sp]);
-                    tc_commit_if(one, &S.o_done[jp & 1]);
+                    tc_commit_if(one, &S.kv_empty[s]);
+                    tc_commit_if(one, &S.o_done[j & 1]);
                 }
             }
             tc_commit_if(one, &S.drain);
@@ -323,6 +353,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.raw_full[s], (uint32_t)(j / RAW) & 1u));
             if (ok && j >= TILES)
                 ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.kv_empty[d], (uint32_t)(j / TILES - 1) & 1u));
+            if (ok && j == TILES - 1)                  // Q's high parts pass through the last tile (below)
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.q_ready, 0));
             if (!ok) break;
             if (ct == 0) S.consumed = j + 1;
             const int have = S.raw_pages[s];
@@ -341,7 +373,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             top = max(__reduce_max_sync(0xffffffffu, top), 11u << 23);
             run = max(run, top);
             if (cw == 0) {
-                const float sigma = __uint_as_float(run - (6u << 23)), inv = pow2_inverse(sigma);
+                const float sigma = __uint_as_float(run - (kSigmaShift << 23)), inv = pow2_inverse(sigma);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int t = lane + 32 * e;
@@ -405,42 +437,58 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16);
         const size_t o_at = ((size_t)row * a.Hq + h * G + head) * D;
-        float qs = 0.0f;                               // takes dk S to log2 units
         if (n_blocks > 0) {
-            // each group writes half of the dims of Q
-            const float4* src = reinterpret_cast<const float4*>(a.q + o_at);
-            float amax = 0.0f;
-#pragma unroll 8
-            for (int k = 0; k < D / 4; ++k) {
-                const float4 v = live ? src[k] : make_float4(0, 0, 0, 0);
-                amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-            }
-            const float p2 = pow2_floor(amax), up = pow2_inverse(p2);
-            qs = p2 * kLog2e;
-            uint32_t hi[32], lo[32];
+            // Q as a pair: low parts to shared memory as they are, high parts by way of the last tile
+            // of the f16 ring, since a lane writes a whole row of TMEM
+            unsigned char* stage = reinterpret_cast<unsigned char*>(S.k[TILES - 1][0]);
+            unsigned char* stage2 = reinterpret_cast<unsigned char*>(S.v[TILES - 1][0]);
+            const int hf = lane >> 4, chunk = (lane & 15) >> 1;
+            const uint32_t sub = (uint32_t)(lane & 1) * 8;
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-                const float4 v = live ? src[16 * odd + k] : make_float4(0, 0, 0, 0);
-                split2(v.x * up, v.y * up, hi[2 * k], lo[2 * k]);
-                split2(v.z * up, v.w * up, hi[2 * k + 1], lo[2 * k + 1]);
+                const int v = (warp - 8) * 16 + k;
+                const float4 x = qv[k];
+                const float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+                const float p2 = pow2_floor(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))));
+                const float up = pow2_inverse(p2);
+                uint2 hi, lo;
+                split2(x.x * up, x.y * up, hi.x, lo.x);
+                split2(x.z * up, x.w * up, hi.y, lo.y);
+                const uint32_t off = sw128(v, chunk) + sub;
+                *reinterpret_cast<uint2*>((hf ? stage2 : stage) + off) = hi;
+                *reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(S.q_lo[hf]) + off) = lo;
+                if (lane == 0) S.qs[v] = p2 * kLog2e;
             }
-            TMEM_ST_X32(tl + COL_Q + 32 * odd, hi);
-            TMEM_ST_X32(tl + COL_Q + 64 + 32 * odd, lo);
+            group_sync();
+            // each group writes half of the dims
+            uint32_t row_hi[32];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const uint4 x = lds128((odd ? stage2 : stage) + sw128(t, c));
+                row_hi[4 * c] = x.x;
+                row_hi[4 * c + 1] = x.y;
+                row_hi[4 * c + 2] = x.z;
+                row_hi[4 * c + 3] = x.w;
+            }
+            TMEM_ST_X32(tl + COL_Q + 32 * odd, row_hi);
             tmem_wait_st();
+            fence_proxy_async_smem();
             tc_fence_before();
             mbar_arrive(&S.q_ready);
         }
+        const float qs = n_blocks > 0 ? S.qs[t] : 0.0f;
         // running maximum of dk S (before qs), the same in log2 units, and the sum of weights
         float top = -INFINITY, top2 = -INFINITY, sum = 0.0f, sigma = 1.0f;
         const float lazy = kLazy / qs;
-        const uint32_t ts = tl + (uint32_t)(odd * KB), to = tl + COL_O + (uint32_t)(odd * D);
+        const uint32_t to = tl + COL_O + (uint32_t)(odd * D);
         bool ok = true;
         for (int j = odd; j < n_blocks; j += 2) {
             const int d = j % TILES;
             const bool got = mbar_wait_bounded(&S.kv_full[d], (uint32_t)(j / TILES) & 1u) &&
-                             mbar_wait_bounded(&S.s_full[odd], (uint32_t)(j >> 1) & 1u);
+                             mbar_wait_bounded(&S.s_full[j % SBUF], (uint32_t)(j / SBUF) & 1u);
             if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
             tc_fence_after();
+            const uint32_t ts = tl + (uint32_t)(j % SBUF * KB);
             uint32_t sv[KB];
             TMEM_LD_X32(ts, sv);
             TMEM_LD_X32(ts + 32, (sv + 32));
@@ -536,7 +584,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             sum += acc.x + acc.y;
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&S.p_ready[odd]);
+            mbar_arrive(&S.p_ready[j % SBUF]);
         }
         // the group's last product: block n_blocks - 1 or n_blocks - 2
         const int mine = (n_blocks + 1 - odd) >> 1;    // blocks of this group
@@ -544,46 +592,45 @@ __global__ void __launch_bounds__(THREADS, 1)
             const bool od = mbar_wait_bounded(&S.o_done[odd], (uint32_t)(mine - 1) & 1u);
             ok = __all_sync(0xffffffffu, od);
         }
-        if (odd) {
-            S.odd[0][t] = top2;
-            S.odd[1][t] = sum;
-            S.odd[2][t] = sigma;
-            tc_fence_before();
-            mbar_arrive(&S.odd_done);
-        } else if (ok) {
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.odd_done, 0));
-        }
-        if (!ok) {
-            if (lane == 0) S.err = 1;
-        } else if (!odd) {
-            // the two groups joined: out = (O0 f0 + O1 f1) / (sum0 f0 + sum1 f1)
-            tc_fence_after();
-            const float other = S.odd[0][t];
-            const float best = fmaxf(top2, other);
-            float f0 = top2 == best ? 1.0f : exp2f(top2 - best), f1 = other == best ? 1.0f : exp2f(other - best);
-            sum = sum * f0 + S.odd[1][t] * f1;
-            f0 *= sigma;
-            f1 *= S.odd[2][t];
+        if (!ok && lane == 0) S.err = 1;
+        S.state[odd][0][t] = top2;
+        S.state[odd][1][t] = sum;
+        S.state[odd][2][t] = sigma;
+        tc_fence_before();
+        group_sync();
+        tc_fence_after();
+        if (!S.err) {
+            // the two joined: out = (O0 f0 + O1 f1) / (sum0 f0 + sum1 f1); each group half of the dims
+            const float m0 = S.state[0][0][t], m1 = S.state[1][0][t], best = fmaxf(m0, m1);
+            float f0 = m0 == best ? 1.0f : exp2f(m0 - best), f1 = m1 == best ? 1.0f : exp2f(m1 - best);
+            sum = S.state[0][1][t] * f0 + S.state[1][1][t] * f1;
+            f0 *= S.state[0][2][t];
+            f1 *= S.state[1][2][t];
             const size_t at = part_index(a, blockIdx.y, h, max_parts, blockIdx.z) + t;
-            if (parts > 1) part_ml[at] = make_float2(best, sum);
+            if (parts > 1 && !odd) part_ml[at] = make_float2(best, sum);
+            if (parts == 1) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                f0 *= inv;
+                f1 *= inv;
+            }
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-                uint32_t ov[16], ow[16];
-                float o[16];
-                if (n_blocks > 0) TMEM_LD_X16(tl + COL_O + c, ov);
-                if (n_blocks > 1) TMEM_LD_X16(tl + COL_O + D + c, ow);
+            for (int c = 64 * odd; c < 64 * odd + 64; c += 32) {
+                uint32_t ov[32], ow[32];
+                if (n_blocks > 0) TMEM_LD_X32(tl + COL_O + c, ov);
+                if (n_blocks > 1) TMEM_LD_X32(tl + COL_O + D + c, ow);
                 tmem_wait_ld();
+                float o[32];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
+                for (int e = 0; e < 32; ++e) {
                     o[e] = n_blocks > 0 ? __uint_as_float(ov[e]) * f0 : 0.0f;
                     if (n_blocks > 1) o[e] = fmaf(__uint_as_float(ow[e]), f1, o[e]);
                 }
                 if (parts > 1) {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4)
+                    for (int e = 0; e < 32; e += 4)
                         *reinterpret_cast<float4*>(part_o + at * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 } else if (live) {
-                    store_quotients<16>(a, o_at + c, o, sum);
+                    store_values<32>(a, o_at + c, o);
                 }
             }
         }
