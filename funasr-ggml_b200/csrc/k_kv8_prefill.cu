@@ -385,28 +385,36 @@ __global__ void __launch_bounds__(THREADS, 1)
                     S.pages[d] = have;
                 }
             }
+            // token 16 i + r of the block, dims 16 chunk ..: all loads before the first store
+            const int r = ct >> 3;
+            uint4 x[2 * PAGES];
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
-                unsigned char* out = reinterpret_cast<unsigned char*>(part ? S.v[d][chunk >> 2] : S.k[d][chunk >> 2]);
+            for (int i = 0; i < 2 * PAGES; ++i)
+                x[i] = lds128(S.raw[s][i >> 1] + (i & 1) * kPartBytes + r * 128 + ((chunk ^ (r & 7)) << 4));
+            // tokens of pages left out, and V behind the last token (unwritten bytes may be e4m3 NaN)
+            if (have != (1 << PAGES) - 1 || key0 + KB - 1 > pos_last) {
 #pragma unroll
-                for (int i = 0; i < PAGES; ++i) {
-                    const int r = ct >> 3;             // token 16 i + r
-                    const int t = i * kPageTokens + r;
-                    uint4 x = lds128(S.raw[s][i] + part * kPartBytes + r * 128 + ((chunk ^ (r & 7)) << 4));
-                    // tokens of pages left out, and V behind the last token (unwritten bytes may be e4m3 NaN)
-                    if (!((have >> i) & 1) || (part && key0 + t > pos_last)) x = make_uint4(0, 0, 0, 0);
-                    __half2 y[8];
-                    expand4<FMT>(x.x, y[0], y[1]);
-                    expand4<FMT>(x.y, y[2], y[3]);
-                    expand4<FMT>(x.z, y[4], y[5]);
-                    expand4<FMT>(x.w, y[6], y[7]);
-                    const uint4* w = reinterpret_cast<const uint4*>(y);
-                    // dims 16 chunk ..: chunks 2 (chunk % 4), + 1 of the half's row; the upper half's threads
-                    // write them in the other order, which spreads a row's stores over all banks
-                    const int up = chunk >> 2, c2 = 2 * (chunk & 3);
-                    *reinterpret_cast<uint4*>(out + sw128(t, c2 + up)) = up ? w[1] : w[0];
-                    *reinterpret_cast<uint4*>(out + sw128(t, c2 + 1 - up)) = up ? w[0] : w[1];
-                }
+                for (int i = 0; i < 2 * PAGES; ++i)
+                    if (!((have >> (i >> 1)) & 1) || ((i & 1) && key0 + (i >> 1) * kPageTokens + r > pos_last))
+                        x[i] = make_uint4(0, 0, 0, 0);
+            }
+            // chunks 2 (chunk % 4), + 1 of the half's row; the upper half's threads write them in the
+            // other order, which spreads a row's stores over all banks
+            const int up = chunk >> 2, c2 = 2 * (chunk & 3);
+            const uint32_t o0 = sw128(r, c2 + up), o1 = sw128(r, c2 + 1 - up);
+            unsigned char* k_out = reinterpret_cast<unsigned char*>(S.k[d][up]);
+            unsigned char* v_out = reinterpret_cast<unsigned char*>(S.v[d][up]);
+#pragma unroll
+            for (int i = 0; i < 2 * PAGES; ++i) {
+                __half2 y[8];
+                expand4<FMT>(x[i].x, y[0], y[1]);
+                expand4<FMT>(x[i].y, y[2], y[3]);
+                expand4<FMT>(x[i].z, y[4], y[5]);
+                expand4<FMT>(x[i].w, y[6], y[7]);
+                const uint4* w = reinterpret_cast<const uint4*>(y);
+                unsigned char* out = ((i & 1) ? v_out : k_out) + (i >> 1) * kPageTokens * 128;
+                *reinterpret_cast<uint4*>(out + o0) = up ? w[1] : w[0];
+                *reinterpret_cast<uint4*>(out + o1) = up ? w[0] : w[1];
             }
             fence_proxy_async_smem();
             __syncwarp();
