@@ -47,16 +47,19 @@ __device__ __forceinline__ HeadRowMeta qkv_head_meta(const AppendArgs& a, int m,
 
 // RMSNorm and rotation of one head vector in a warp: x holds the lane's dims l, l+32, l+64,
 // l+96, w their norm weights, rot the rotations (cos, sin) of the pairs (l, l+64) and
-// (l+32, l+96).
-__device__ __forceinline__ void head_norm_rope(const float (&w)[4], const float2 (&rot)[2], float eps, float (&x)[4]) {
-    constexpr int D = 128;
+// (l+32, l+96). In three steps: a lane's share of the sum of squares, the scale, the rest.
+__device__ __forceinline__ double norm_squares(const float (&x)[4]) {
     double ss = 0.0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) ss += (double)__fmul_rn(x[k], x[k]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    return ss;
+}
+__device__ __forceinline__ float norm_scale(double ss, float eps) {
+    constexpr int D = 128;
     const float mean = (float)(ss * (1.0 / D));      // D = 128: exactly ss / D
-    const float scale = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, eps)));
+    return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, eps)));
+}
+__device__ __forceinline__ void norm_rope_apply(const float (&w)[4], const float2 (&rot)[2], float scale, float (&x)[4]) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] = __fmul_rn(__fmul_rn(x[k], scale), w[k]);
     // pair (x[0], x[2]) uses rotation index lane, pair (x[1], x[3]) index lane + 32
@@ -67,6 +70,12 @@ __device__ __forceinline__ void head_norm_rope(const float (&w)[4], const float2
         x[k] = __fsub_rn(__fmul_rn(x0, r.x), __fmul_rn(x1, r.y));
         x[k + 2] = __fadd_rn(__fmul_rn(x0, r.y), __fmul_rn(x1, r.x));
     }
+}
+__device__ __forceinline__ void head_norm_rope(const float (&w)[4], const float2 (&rot)[2], float eps, float (&x)[4]) {
+    double ss = norm_squares(x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    norm_rope_apply(w, rot, norm_scale(ss, eps), x);
 }
 
 // q_dst (optional): where a q head goes instead of a.q_out (128 floats, any address space);

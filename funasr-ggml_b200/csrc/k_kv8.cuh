@@ -41,28 +41,36 @@ __device__ __forceinline__ float scale_of(uint32_t amax_bits) {
     return __uint_as_float((uint32_t)max(k, 1) << 23);
 }
 
-// x / d rounded to the nearest integer, ties to even, exactly: the quotient from the
-// reciprocal is off by less than one, and its remainder x - q d is exact in f32 (x and q d
-// are multiples of the smaller of their last places and nearly cancel), so comparing it with
-// d / 2 settles which side of the border x / d lies on.
-__device__ __forceinline__ int round_quotient(float x, float d, float inv, float half_d) {
-    float q = rintf(__fmul_rn(x, inv));
-    const float r = __fmaf_rn(-q, d, x);
-    const float a = fabsf(r);
-    if (a > half_d || (a == half_d && ((int)q & 1))) q += copysignf(1.0f, r);
-    return (int)q;
+// x / d rounded to the nearest integer, ties to even, exactly, as the low byte of the result.
+// m = 1.5 * 2^23 + x * inv rounds the product to an integer that is off by less than one from
+// the quotient; its remainder r = x - q d is exact in f32 (x and q d are multiples of the
+// smaller of their last places and nearly cancel), so comparing |r| with d / 2 settles on which
+// side of the border x / d lies. border collects the largest |r|: only where that reaches d / 2
+// does a value need settle().
+constexpr float kRoundMagic = 12582912.0f;         // 1.5 * 2^23: an even integer, low byte 0
+__device__ __forceinline__ uint32_t round_quotient(float x, float d, float inv, float& border) {
+    const float m = __fmaf_rn(x, inv, kRoundMagic);
+    border = fmaxf(border, fabsf(__fmaf_rn(-__fsub_rn(m, kRoundMagic), d, x)));
+    return __float_as_uint(m);
+}
+__device__ __forceinline__ uint32_t settle(uint32_t m, float x, float d) {
+    const float r = __fmaf_rn(-__fsub_rn(__uint_as_float(m), kRoundMagic), d, x), a = fabsf(r), h = 0.5f * d;
+    return a > h || (a == h && (m & 1)) ? m + (r > 0.0f ? 1u : ~0u) : m;
 }
 
 // Four values of a vector with scale d as stored bytes. inv = 1 / d (for e4m3 exact).
 template <int FMT>
 __device__ __forceinline__ uint32_t pack4(const float* x, float d, float inv) {
     if (FMT == kInt8) {
-        const float h = 0.5f * d;
-        const uint32_t a = (uint32_t)round_quotient(x[0], d, inv, h) & 0xffu;
-        const uint32_t b = (uint32_t)round_quotient(x[1], d, inv, h) & 0xffu;
-        const uint32_t c = (uint32_t)round_quotient(x[2], d, inv, h) & 0xffu;
-        const uint32_t e = (uint32_t)round_quotient(x[3], d, inv, h) & 0xffu;
-        return a | (b << 8) | (c << 16) | (e << 24);
+        uint32_t m[4];
+        float border = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m[k] = round_quotient(x[k], d, inv, border);
+        if (border >= 0.5f * d) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m[k] = settle(m[k], x[k], d);
+        }
+        return __byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410);
     }
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * inv, x[1] * inv), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * inv, x[3] * inv), __NV_SATFINITE, __NV_E4M3);

@@ -80,38 +80,68 @@ struct Kv8AppendArgs {
     int* err;
 };
 
-// Raw append: a warp per (row, layer, KV head), its half-warps the K and the V vector, a
-// lane 8 consecutive values.
-template <int FMT, typename T>
-__global__ void __launch_bounds__(256) kv8_append_kernel(Kv8AppendArgs a) {
-    const long long gw = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (gw >= (long long)a.M * a.n_layers * a.Hkv) return;
-    const int h = (int)(gw % a.Hkv);
-    const int l = (int)(gw / a.Hkv % a.n_layers);
-    const int m = (int)(gw / a.Hkv / a.n_layers);
+// Raw append: a warp per P (layer, KV head) pairs of a row, its half-warps the K and the V
+// vector of a pair, a lane 8 consecutive values of each; the loads of all pairs are under way
+// before the row's place in the pool is looked up. The pairs' largest magnitudes are reduced
+// over the half-warp together (each exchange halves the pairs a lane carries), so that the
+// scales and their reciprocals are computed once, side by side, and handed back.
+template <int FMT, typename T, int P>
+__global__ void __launch_bounds__(256) kv8_append_kernel(Kv8AppendArgs a, unsigned blocks_per_row) {
+    static_assert(P == 1 || P == 4, "the exchanges below");
+    const int m = blockIdx.x / blocks_per_row;
+    const int i0 = (int)((blockIdx.x - m * blocks_per_row) * 8 + (threadIdx.x >> 5)) * P;
+    const int lane = threadIdx.x & 31, part = lane >> 4, c = lane & 15;
+    const int n_pairs = a.n_layers * a.Hkv;
+    if (i0 >= n_pairs) return;
+    const T* src = reinterpret_cast<const T*>(part ? a.v : a.k) + (size_t)m * a.row_stride + 8 * c;
+    float x[P][8];
+#pragma unroll
+    for (int u = 0; u < P; ++u) load8(src + (size_t)min(i0 + u, n_pairs - 1) * D, x[u]);
     const int pos = a.pos[m];
     const int page = token_page(a.block_table, a.bt_stride, a.n_pages, a.slot[m], pos, a.err, lane == 0);
     if (page < 0) return;
-    const int part = lane >> 4, c = lane & 15;
-    float x[8];
-    load8(reinterpret_cast<const T*>(part ? a.v : a.k) + (size_t)m * a.row_stride + ((size_t)l * a.Hkv + h) * D + 8 * c,
-          x);
-    uint32_t amax = 0;
+    uint32_t amax[P];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
+    for (int u = 0; u < P; ++u) {
+        amax[u] = 0;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float d = scale_of<FMT>(amax);
-    uint2 q = make_uint2(0, 0);
-    if (amax < 0x7f800000u) {
-        const float inv = __frcp_rn(d);
-        q = make_uint2(pack4<FMT>(x, d, inv), pack4<FMT>(x + 4, d, inv));
+        for (int i = 0; i < 8; ++i) amax[u] = max(amax[u], __float_as_uint(x[u][i]) & 0x7fffffffu);
     }
-    unsigned char* tile = a.pool + (((size_t)l * a.n_pages + page) * a.Hkv + h) * kTileBytes;
+    uint32_t top = amax[0];
+    if (P == 4) {                                      // lane c ends with pair c / 4
+        uint32_t two[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t keep = (c & 8) ? amax[(i + 2) % P] : amax[i % P], send = (c & 8) ? amax[i % P] : amax[(i + 2) % P];
+            two[i] = max(keep, __shfl_xor_sync(0xffffffffu, send, 8));
+        }
+        const uint32_t keep = (c & 4) ? two[1] : two[0], send = (c & 4) ? two[0] : two[1];
+        top = max(keep, __shfl_xor_sync(0xffffffffu, send, 4));
+    } else {
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 4));
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const float d_mine = scale_of<FMT>(top), inv_mine = __frcp_rn(d_mine);
     const int t = pos % kPageTokens;
-    *reinterpret_cast<uint2*>(tile + part * kPartBytes + t * D + 8 * c) = q;
-    if (c == 0) reinterpret_cast<float*>(tile + kScaleOff)[part * kPageTokens + t] = d;
+    int l = i0 / a.Hkv, h = i0 - l * a.Hkv;
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+        const float d = P == 1 ? d_mine : __shfl_sync(0xffffffffu, d_mine, (lane & 16) + 4 * u);
+        const float inv = P == 1 ? inv_mine : __shfl_sync(0xffffffffu, inv_mine, (lane & 16) + 4 * u);
+        if (i0 + u < n_pairs) {
+            uint2 q = make_uint2(0, 0);
+            if (d == d) q = make_uint2(pack4<FMT>(x[u], d, inv), pack4<FMT>(x[u] + 4, d, inv));
+            unsigned char* tile = a.pool + (((size_t)l * a.n_pages + page) * a.Hkv + h) * kTileBytes;
+            *reinterpret_cast<uint2*>(tile + part * kPartBytes + t * D + 8 * c) = q;
+            if (c == 0) reinterpret_cast<float*>(tile + kScaleOff)[part * kPageTokens + t] = d;
+        }
+        if (++h == a.Hkv) {
+            h = 0;
+            ++l;
+        }
+    }
 }
 
 struct Kv8QkvArgs {
@@ -132,51 +162,98 @@ struct Kv8QkvArgs {
     int* err;
 };
 
-// Kernel (1) with an 8-bit end: a warp per (row, head vector), lane l holding dims l, l+32,
-// l+64, l+96 (both rotation pairs of a lane stay in it).
-template <int FMT>
+// Kernel (1) with an 8-bit end: a CTA per row and 8 V of its head vectors, a warp V of them
+// (lane l holding dims l, l+32, l+64, l+96: both rotation pairs of a lane stay in it), whose
+// loads are under way together with that of the row's position. With V = 4 the vectors' sums
+// of squares are reduced over the warp together: each exchange halves the vectors a lane
+// carries and pairs the same lanes as the xor reduction of one vector does, so the sums are the
+// same bits, and the norms' square root and division, and the scales and reciprocals, are
+// computed once, side by side.
+template <int FMT, int V>
 __global__ void __launch_bounds__(256) kv8_qkv_kernel(Kv8QkvArgs a) {
+    static_assert(V == 1 || V == 4, "the exchanges below");
     const int m = blockIdx.x;
-    const int j = blockIdx.y * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    if (j >= a.Hq + 2 * a.Hkv) return;
+    const int j0 = blockIdx.y * 8 * V + (threadIdx.x >> 5);
+    const int n_vec = a.Hq + 2 * a.Hkv;
+    if (j0 >= n_vec) return;
+    float x[V][4];
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+        const float* src = a.qkv + ((size_t)m * n_vec + min(j0 + 8 * u, n_vec - 1)) * D + lane;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[u][k] = src[32 * k];
+    }
     const int pos = a.pos[m];
     if (pos == -1) return;
     if (pos < 0 || pos >= a.max_pos) {
         if (lane == 0) record_error(a.err, kDevErrBadPos);
         return;
     }
-    const bool is_q = j < a.Hq, is_k = !is_q && j < a.Hq + a.Hkv;
-    float x[4];
+    const float2* cs = a.rope + (size_t)pos * (D / 2);
+    const float2 rot[2] = {cs[lane], cs[lane + 32]};
+    const bool stores = j0 + 8 * (V - 1) >= a.Hq;                 // a K or V head among the warp's
+    const int page =
+        stores ? token_page(a.block_table, a.bt_stride, a.n_pages, a.slot[m], pos, a.err, lane == 0) : -1;
+    float scale[V];
+    if (V == 4) {
+        double two[2];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = a.qkv[((size_t)m * (a.Hq + 2 * a.Hkv) + j) * D + lane + 32 * k];
-    if (is_q || is_k) {
-        const float* w = is_q ? a.qn_w : a.kn_w;
-        const float wv[4] = {w[lane], w[lane + 32], w[lane + 64], w[lane + 96]};
-        const float2* cs = a.rope + (size_t)pos * (D / 2);
-        const float2 rot[2] = {cs[lane], cs[lane + 32]};
-        head_norm_rope(wv, rot, a.eps, x);
-    }
-    if (is_q) {
-        float* dst = a.q_out + ((size_t)m * a.Hq + j) * D;
+        for (int i = 0; i < 2; ++i) {
+            const double lo = norm_squares(x[i % V]), hi = norm_squares(x[(i + 2) % V]);
+            two[i] = ((lane & 16) ? hi : lo) + __shfl_xor_sync(0xffffffffu, (lane & 16) ? lo : hi, 16);
+        }
+        double ss = ((lane & 8) ? two[1] : two[0]) + __shfl_xor_sync(0xffffffffu, (lane & 8) ? two[0] : two[1], 8);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) dst[lane + 32 * k] = __fmul_rn(x[k], a.q_scale);
-        return;
+        for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float mine = norm_scale(ss, a.eps);                 // lane l: vector l / 8
+#pragma unroll
+        for (int u = 0; u < V; ++u) scale[u] = __shfl_sync(0xffffffffu, mine, 8 * u);
+    } else {
+        double ss = norm_squares(x[0]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        scale[0] = norm_scale(ss, a.eps);
     }
-    const int h = is_k ? j - a.Hq : j - a.Hq - a.Hkv, part = is_k ? 0 : 1;
-    const int page = token_page(a.block_table, a.bt_stride, a.n_pages, a.slot[m], pos, a.err, lane == 0);
+    uint32_t top = 0;                                             // lane l: of the warp's stored vector l % V
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+        const int j = j0 + 8 * u;
+        if (j >= n_vec) break;
+        if (j < a.Hq + a.Hkv) {
+            const float* w = j < a.Hq ? a.qn_w : a.kn_w;
+            const float wv[4] = {w[lane], w[lane + 32], w[lane + 64], w[lane + 96]};
+            norm_rope_apply(wv, rot, scale[u], x[u]);
+        }
+        if (j < a.Hq) {
+            float* dst = a.q_out + ((size_t)m * a.Hq + j) * D + lane;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) dst[32 * k] = __fmul_rn(x[u][k], a.q_scale);
+        } else {
+            uint32_t amax = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) amax = max(amax, __float_as_uint(x[u][k]) & 0x7fffffffu);
+            amax = __reduce_max_sync(0xffffffffu, amax);
+            if (lane % V == u) top = amax;
+        }
+    }
     if (page < 0) return;
-    uint32_t amax = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) amax = max(amax, __float_as_uint(x[k]) & 0x7fffffffu);
-    amax = __reduce_max_sync(0xffffffffu, amax);
-    const float d = scale_of<FMT>(amax);
-    const uint32_t q = amax < 0x7f800000u ? pack4<FMT>(x, d, __frcp_rn(d)) : 0u;
-    unsigned char* tile = a.pool + ((size_t)page * a.Hkv + h) * kTileBytes;
+    const float d_mine = scale_of<FMT>(top), inv_mine = __frcp_rn(d_mine);
     const int t = pos % kPageTokens;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) tile[part * kPartBytes + t * D + lane + 32 * k] = (unsigned char)(q >> (8 * k));
-    if (lane == 0) reinterpret_cast<float*>(tile + kScaleOff)[part * kPageTokens + t] = d;
+    for (int u = 0; u < V; ++u) {
+        const int j = j0 + 8 * u;
+        if (j < a.Hq) continue;
+        if (j >= n_vec) break;
+        const int part = j < a.Hq + a.Hkv ? 0 : 1, h = j - a.Hq - part * a.Hkv;
+        const float d = __shfl_sync(0xffffffffu, d_mine, u), inv = __shfl_sync(0xffffffffu, inv_mine, u);
+        const uint32_t q = d == d ? pack4<FMT>(x[u], d, inv) : 0u;
+        unsigned char* tile = a.pool + ((size_t)page * a.Hkv + h) * kTileBytes;
+        unsigned char* dst = tile + part * kPartBytes + t * D + lane;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) dst[32 * k] = (unsigned char)(q >> (8 * k));
+        if (lane == 0) reinterpret_cast<float*>(tile + kScaleOff)[part * kPageTokens + t] = d;
+    }
 }
 
 struct Kv8GatherArgs {
@@ -223,8 +300,10 @@ __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const fl
 }
 
 // Gather: one CTA per page of one sequence in one layer; a thread 8 values of one token,
-// over the heads' K and V parts. The value d * q is formed in f32 and rounded once to the
+// over the heads' K and V parts, kGatherVecs loads under way at a time. The value d * q is formed in f32 and rounded once to the
 // output type.
+constexpr int kGatherVecs = 16;                // 8: 1.5 % slower on 32 streams of up to 320 tokens in 28 layers
+
 template <int FMT, typename T>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(Kv8GatherArgs a) {
     const int m = blockIdx.y, l = blockIdx.z;
@@ -247,24 +326,33 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(Kv8GatherArgs a) {
     if (token < t0 || token >= t0 + n) return;
     const unsigned char* tiles = a.pool + ((size_t)l * a.n_pages + page) * a.Hkv * kTileBytes;
     const size_t row = (size_t)row0 + (token - t0);
-#pragma unroll 4
-    for (int j = 0; j < 2 * a.Hkv; ++j) {
-        const int h = j >> 1, part = j & 1;
-        const unsigned char* tile = tiles + (size_t)h * kTileBytes;
-        const uint2 w = *reinterpret_cast<const uint2*>(tile + part * kPartBytes + t * D + 8 * c);
-        const float d = reinterpret_cast<const float*>(tile + kScaleOff)[part * kPageTokens + t];
-        __half2 v[4];
-        expand4<FMT>(w.x, v[0], v[1]);
-        expand4<FMT>(w.y, v[2], v[3]);
-        float x[8];
+    for (int j0 = 0; j0 < 2 * a.Hkv; j0 += kGatherVecs) {
+        uint2 w[kGatherVecs];
+        float d[kGatherVecs];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(v[i]);
-            x[2 * i] = f.x * d;
-            x[2 * i + 1] = f.y * d;
+        for (int u = 0; u < kGatherVecs; ++u) {
+            const int j = min(j0 + u, 2 * a.Hkv - 1);
+            const unsigned char* tile = tiles + (size_t)(j >> 1) * kTileBytes;
+            w[u] = *reinterpret_cast<const uint2*>(tile + (j & 1) * kPartBytes + t * D + 8 * c);
+            d[u] = reinterpret_cast<const float*>(tile + kScaleOff)[(j & 1) * kPageTokens + t];
         }
-        T* out = reinterpret_cast<T*>(part ? a.v_out : a.k_out);
-        store8(out + (((size_t)l * a.Hkv + h) * a.total_rows + row) * D + 8 * c, x);
+#pragma unroll
+        for (int u = 0; u < kGatherVecs; ++u) {
+            const int j = j0 + u;
+            if (j >= 2 * a.Hkv) break;
+            __half2 v[4];
+            expand4<FMT>(w[u].x, v[0], v[1]);
+            expand4<FMT>(w[u].y, v[2], v[3]);
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(v[i]);
+                x[2 * i] = f.x * d[u];
+                x[2 * i + 1] = f.y * d[u];
+            }
+            T* out = reinterpret_cast<T*>((j & 1) ? a.v_out : a.k_out);
+            store8(out + (((size_t)l * a.Hkv + (j >> 1)) * a.total_rows + row) * D + 8 * c, x);
+        }
     }
 }
 
@@ -276,11 +364,29 @@ int launched(const char* what) {
     return report_op_error(FA_ERR_CUDA, (std::string(what) + ": " + cudaGetErrorString(e)).c_str());
 }
 
+// Whether a warp takes several vectors: once the warps of one vector each would fill the GPU
+// (148 SMs x 64 warps); below that more warps shorten the call.
+bool several_per_warp(long long vectors) { return vectors > 148 * 64; }
+
+template <int FMT, typename T>
+void launch_append(const Kv8AppendArgs& a, unsigned per_row, bool four, cudaStream_t s) {
+    const unsigned blocks = (unsigned)a.M * per_row;
+    if (four) kv8_append_kernel<FMT, T, 4><<<blocks, 256, 0, s>>>(a, per_row);
+    else kv8_append_kernel<FMT, T, 1><<<blocks, 256, 0, s>>>(a, per_row);
+}
+
 template <int FMT>
-void append_by_type(const Kv8AppendArgs& a, int type, unsigned blocks, cudaStream_t s) {
-    if (type == FA_TYPE_F32) kv8_append_kernel<FMT, float><<<blocks, 256, 0, s>>>(a);
-    else if (type == FA_TYPE_F16) kv8_append_kernel<FMT, __half><<<blocks, 256, 0, s>>>(a);
-    else kv8_append_kernel<FMT, __nv_bfloat16><<<blocks, 256, 0, s>>>(a);
+void append_by_type(const Kv8AppendArgs& a, int type, unsigned per_row, bool four, cudaStream_t s) {
+    if (type == FA_TYPE_F32) launch_append<FMT, float>(a, per_row, four, s);
+    else if (type == FA_TYPE_F16) launch_append<FMT, __half>(a, per_row, four, s);
+    else launch_append<FMT, __nv_bfloat16>(a, per_row, four, s);
+}
+
+template <int V>
+void launch_qkv(const Kv8QkvArgs& a, int format, cudaStream_t s) {
+    const dim3 grid(a.M, (a.Hq + 2 * a.Hkv + 8 * V - 1) / (8 * V));
+    if (format == FA_KV8_INT8) kv8_qkv_kernel<kInt8, V><<<grid, 256, 0, s>>>(a);
+    else kv8_qkv_kernel<kE4m3, V><<<grid, 256, 0, s>>>(a);
 }
 
 template <int FMT>
@@ -315,13 +421,15 @@ extern "C" FA_API int fa_op_kv8_append(const void* k, const void* v, int src_typ
                                "fa_op_kv8_append: row_stride must cover a row and be a multiple of 16 bytes");
     if (misaligned(k, 16) || misaligned(v, 16) || misaligned(pool, 128))
         return report_op_error(FA_ERR_INVALID_ARG, "fa_op_kv8_append: k and v must be 16-byte, pool 128-byte aligned");
-    const long long blocks = ((long long)M * n_layers * n_kv_heads + 7) / 8;
-    if ((long long)n_layers * n_kv_heads > (1 << 20) || blocks > 0x7fffffffll)
+    const long long pairs = (long long)n_layers * n_kv_heads;
+    const bool four = several_per_warp(M * pairs);
+    const long long per_row = four ? (pairs + 31) / 32 : (pairs + 7) / 8;
+    if (pairs > 0x7fffffffll || M * per_row > 0x7fffffffll)
         return report_op_error(FA_ERR_CAPACITY, "fa_op_kv8_append: too many vectors for one call");
     Kv8AppendArgs a{k, v, row_stride, M, n_layers, n_kv_heads, pos, slot, bt, bt_stride, n_pages,
                     static_cast<unsigned char*>(pool), err};
-    if (format == FA_KV8_INT8) append_by_type<kv8::kInt8>(a, src_type, (unsigned)blocks, (cudaStream_t)stream);
-    else append_by_type<kv8::kE4m3>(a, src_type, (unsigned)blocks, (cudaStream_t)stream);
+    if (format == FA_KV8_INT8) append_by_type<kv8::kInt8>(a, src_type, (unsigned)per_row, four, (cudaStream_t)stream);
+    else append_by_type<kv8::kE4m3>(a, src_type, (unsigned)per_row, four, (cudaStream_t)stream);
     return launched("fa_op_kv8_append");
 }
 
@@ -344,9 +452,9 @@ extern "C" FA_API int fa_op_qknorm_rope_append_kv8(const float* qkv, int M, int 
     Kv8QkvArgs a{qkv, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages, qn, kn, eps,
                  1.0f / std::sqrt((float)kv8::D), reinterpret_cast<const float2*>(rope), max_pos,
                  static_cast<unsigned char*>(pool_layer), q_out, err};
-    const dim3 grid(M, (n_heads + 2 * n_kv_heads + 7) / 8);
-    if (format == FA_KV8_INT8) kv8_qkv_kernel<kv8::kInt8><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
-    else kv8_qkv_kernel<kv8::kE4m3><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
+    const long long n_vec = (long long)n_heads + 2ll * n_kv_heads;
+    if (several_per_warp(M * n_vec)) launch_qkv<4>(a, format, (cudaStream_t)stream);
+    else launch_qkv<1>(a, format, (cudaStream_t)stream);
     return launched("fa_op_qknorm_rope_append_kv8");
 }
 
