@@ -45,9 +45,10 @@ __device__ __forceinline__ HeadRowMeta qkv_head_meta(const AppendArgs& a, int m,
     return h;
 }
 
-// RMSNorm and rotation of one head vector in a warp: x holds the lane's dims l, l+32, l+64,
-// l+96, w their norm weights, rot the rotations (cos, sin) of the pairs (l, l+64) and
-// (l+32, l+96). In three steps: a lane's share of the sum of squares, the scale, the rest.
+// RMSNorm and rotation of one head vector in a warp: x holds four of its dims, d, e, d+64, e+64
+// (here d = l, e = l+32), w their norm weights, rot the rotations (cos, sin) of the pairs
+// (d, d+64) and (e, e+64). In three steps: a lane's share of the sum of squares, the scale, the
+// rest.
 __device__ __forceinline__ double norm_squares(const float (&x)[4]) {
     double ss = 0.0;
 #pragma unroll
@@ -62,7 +63,6 @@ __device__ __forceinline__ float norm_scale(double ss, float eps) {
 __device__ __forceinline__ void norm_rope_apply(const float (&w)[4], const float2 (&rot)[2], float scale, float (&x)[4]) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] = __fmul_rn(__fmul_rn(x[k], scale), w[k]);
-    // pair (x[0], x[2]) uses rotation index lane, pair (x[1], x[3]) index lane + 32
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const float2 r = rot[k];

@@ -144,6 +144,10 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8AppendArgs a, unsign
     }
 }
 
+// Warps of a CTA: 4096 rows of 32 head vectors take 27.4 us with 8, 22.7 with 4, 22.2 with 2 and
+// 22.9 with 1 (a CTA's registers are free again only when its slowest warp ends).
+constexpr int kQkvWarps = 2;
+
 struct Kv8QkvArgs {
     const float* qkv;        // [M][(Hq + 2 Hkv) * 128]
     int M, Hq, Hkv;
@@ -162,37 +166,47 @@ struct Kv8QkvArgs {
     int* err;
 };
 
-// Kernel (1) with an 8-bit end: a CTA per row and 8 V of its head vectors, a warp V of them
-// (lane l holding dims l, l+32, l+64, l+96: both rotation pairs of a lane stay in it), whose
+// Kernel (1) with an 8-bit end: a CTA per row and kQkvWarps V of its head vectors, a warp V of
+// them
+// (lane l holding dims 2l, 2l+1, 64+2l, 65+2l: both rotation pairs of a lane stay in it), whose
 // loads are under way together with that of the row's position. With V = 4 the vectors' sums
 // of squares are reduced over the warp together: each exchange halves the vectors a lane
 // carries and pairs the same lanes as the xor reduction of one vector does, so the sums are the
 // same bits, and the norms' square root and division, and the scales and reciprocals, are
 // computed once, side by side.
+__device__ __forceinline__ void load4(const float* vec, int lane, float (&x)[4]) {
+    const float2 a = reinterpret_cast<const float2*>(vec)[lane], b = reinterpret_cast<const float2*>(vec)[lane + 32];
+    x[0] = a.x;
+    x[1] = a.y;
+    x[2] = b.x;
+    x[3] = b.y;
+}
+
 template <int FMT, int V>
-__global__ void __launch_bounds__(256) kv8_qkv_kernel(Kv8QkvArgs a) {
+__global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
     static_assert(V == 1 || V == 4, "the exchanges below");
     const int m = blockIdx.x;
     const int lane = threadIdx.x & 31;
-    const int j0 = blockIdx.y * 8 * V + (threadIdx.x >> 5);
+    const int j0 = blockIdx.y * kQkvWarps * V + (threadIdx.x >> 5);
     const int n_vec = a.Hq + 2 * a.Hkv;
     if (j0 >= n_vec) return;
     float x[V][4];
 #pragma unroll
     for (int u = 0; u < V; ++u) {
-        const float* src = a.qkv + ((size_t)m * n_vec + min(j0 + 8 * u, n_vec - 1)) * D + lane;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[u][k] = src[32 * k];
+        load4(a.qkv + ((size_t)m * n_vec + min(j0 + kQkvWarps * u, n_vec - 1)) * D, lane, x[u]);
     }
+    float qw[4], kw[4];
+    load4(a.qn_w, lane, qw);
+    load4(a.kn_w, lane, kw);
     const int pos = a.pos[m];
     if (pos == -1) return;
     if (pos < 0 || pos >= a.max_pos) {
         if (lane == 0) record_error(a.err, kDevErrBadPos);
         return;
     }
-    const float2* cs = a.rope + (size_t)pos * (D / 2);
-    const float2 rot[2] = {cs[lane], cs[lane + 32]};
-    const bool stores = j0 + 8 * (V - 1) >= a.Hq;                 // a K or V head among the warp's
+    const float4 cs = reinterpret_cast<const float4*>(a.rope + (size_t)pos * (D / 2))[lane];
+    const float2 rot[2] = {make_float2(cs.x, cs.y), make_float2(cs.z, cs.w)};
+    const bool stores = j0 + kQkvWarps * (V - 1) >= a.Hq;                 // a K or V head among the warp's
     const int page =
         stores ? token_page(a.block_table, a.bt_stride, a.n_pages, a.slot[m], pos, a.err, lane == 0) : -1;
     float scale[V];
@@ -218,18 +232,15 @@ __global__ void __launch_bounds__(256) kv8_qkv_kernel(Kv8QkvArgs a) {
     uint32_t top = 0;                                             // lane l: of the warp's stored vector l % V
 #pragma unroll
     for (int u = 0; u < V; ++u) {
-        const int j = j0 + 8 * u;
+        const int j = j0 + kQkvWarps * u;
         if (j >= n_vec) break;
-        if (j < a.Hq + a.Hkv) {
-            const float* w = j < a.Hq ? a.qn_w : a.kn_w;
-            const float wv[4] = {w[lane], w[lane + 32], w[lane + 64], w[lane + 96]};
-            norm_rope_apply(wv, rot, scale[u], x[u]);
-        }
         if (j < a.Hq) {
-            float* dst = a.q_out + ((size_t)m * a.Hq + j) * D + lane;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) dst[32 * k] = __fmul_rn(x[u][k], a.q_scale);
+            norm_rope_apply(qw, rot, scale[u], x[u]);
+            float2* dst = reinterpret_cast<float2*>(a.q_out + ((size_t)m * a.Hq + j) * D) + lane;
+            dst[0] = make_float2(__fmul_rn(x[u][0], a.q_scale), __fmul_rn(x[u][1], a.q_scale));
+            dst[32] = make_float2(__fmul_rn(x[u][2], a.q_scale), __fmul_rn(x[u][3], a.q_scale));
         } else {
+            if (j < a.Hq + a.Hkv) norm_rope_apply(kw, rot, scale[u], x[u]);
             uint32_t amax = 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) amax = max(amax, __float_as_uint(x[u][k]) & 0x7fffffffu);
@@ -242,16 +253,16 @@ __global__ void __launch_bounds__(256) kv8_qkv_kernel(Kv8QkvArgs a) {
     const int t = pos % kPageTokens;
 #pragma unroll
     for (int u = 0; u < V; ++u) {
-        const int j = j0 + 8 * u;
+        const int j = j0 + kQkvWarps * u;
         if (j < a.Hq) continue;
         if (j >= n_vec) break;
         const int part = j < a.Hq + a.Hkv ? 0 : 1, h = j - a.Hq - part * a.Hkv;
         const float d = __shfl_sync(0xffffffffu, d_mine, u), inv = __shfl_sync(0xffffffffu, inv_mine, u);
         const uint32_t q = d == d ? pack4<FMT>(x[u], d, inv) : 0u;
         unsigned char* tile = a.pool + ((size_t)page * a.Hkv + h) * kTileBytes;
-        unsigned char* dst = tile + part * kPartBytes + t * D + lane;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) dst[32 * k] = (unsigned char)(q >> (8 * k));
+        uint16_t* dst = reinterpret_cast<uint16_t*>(tile + part * kPartBytes + t * D) + lane;
+        dst[0] = (uint16_t)q;
+        dst[32] = (uint16_t)(q >> 16);
         if (lane == 0) reinterpret_cast<float*>(tile + kScaleOff)[part * kPageTokens + t] = d;
     }
 }
@@ -384,9 +395,9 @@ void append_by_type(const Kv8AppendArgs& a, int type, unsigned per_row, bool fou
 
 template <int V>
 void launch_qkv(const Kv8QkvArgs& a, int format, cudaStream_t s) {
-    const dim3 grid(a.M, (a.Hq + 2 * a.Hkv + 8 * V - 1) / (8 * V));
-    if (format == FA_KV8_INT8) kv8_qkv_kernel<kInt8, V><<<grid, 256, 0, s>>>(a);
-    else kv8_qkv_kernel<kE4m3, V><<<grid, 256, 0, s>>>(a);
+    const dim3 grid(a.M, (a.Hq + 2 * a.Hkv + kQkvWarps * V - 1) / (kQkvWarps * V));
+    if (format == FA_KV8_INT8) kv8_qkv_kernel<kInt8, V><<<grid, kQkvWarps * 32, 0, s>>>(a);
+    else kv8_qkv_kernel<kE4m3, V><<<grid, kQkvWarps * 32, 0, s>>>(a);
 }
 
 template <int FMT>
@@ -444,9 +455,11 @@ extern "C" FA_API int fa_op_qknorm_rope_append_kv8(const float* qkv, int M, int 
         return report_op_error(FA_ERR_INVALID_ARG, "fa_op_qknorm_rope_append_kv8: null or non-positive argument");
     if (!known_format(format))
         return report_op_error(FA_ERR_INVALID_ARG, "fa_op_qknorm_rope_append_kv8: unknown format");
-    if (misaligned(qkv, 16) || misaligned(q_out, 16) || misaligned(rope, 16) || misaligned(pool_layer, 128))
+    if (misaligned(qkv, 16) || misaligned(q_out, 16) || misaligned(rope, 16) || misaligned(qn, 8) || misaligned(kn, 8) ||
+        misaligned(pool_layer, 128))
         return report_op_error(FA_ERR_INVALID_ARG,
-                               "fa_op_qknorm_rope_append_kv8: qkv, rope and q_out must be 16-byte, pool 128-byte aligned");
+                               "fa_op_qknorm_rope_append_kv8: qkv, rope and q_out must be 16-byte, the norm weights 8-byte, the pool "
+                               "128-byte aligned");
     if ((long long)n_heads + 2ll * n_kv_heads > 65535)
         return report_op_error(FA_ERR_CAPACITY, "fa_op_qknorm_rope_append_kv8: too many heads");
     Kv8QkvArgs a{qkv, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages, qn, kn, eps,
