@@ -80,6 +80,8 @@ cudaError_t configure_attention();
 void configure_gemm();
 void configure_gemm_tc();
 void configure_gemm_tc_skinny();
+void configure_kv8_attention();
+void configure_kv8_prefill();
 }  // namespace fa
 
 static int ensure_configured() {
@@ -93,6 +95,8 @@ static int ensure_configured() {
         fa::configure_gemm_tc_skinny();
         fa::configure_prefill_attention();
         fa::configure_row_step();
+        fa::configure_kv8_attention();
+        fa::configure_kv8_prefill();
         g_configured[dev] = true;
     }
     return FA_OK;

@@ -76,18 +76,16 @@ constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 148 * kCtasPerSm;     // one resident wave of a B200
 constexpr int kItemUnits = 2;
 
-template <int NT>
-constexpr int kStages = NT == 1 ? 4 : 3;
-
+constexpr int kStages = 3;                     // 128 rows x 2048 tokens: 2 stages 97, 3 95, 4 98 us
 template <int NT>
 struct DecodeSmem {
-    unsigned char tiles[kWarps][kStages<NT>][2 * kPartBytes];   // K then V, 128 B swizzle
-    float scales[kWarps][kStages<NT>][2 * kPageTokens];         // K then V
+    unsigned char tiles[kWarps][kStages][2 * kPartBytes];   // K then V, 128 B swizzle
+    float scales[kWarps][kStages][2 * kPageTokens];         // K then V
     // the warps' first partials; their last ones go over the warp's ring once it is drained
     float acc[kWarps][4 * NT][D];
     float2 ml[kWarps][2][4 * NT];                               // running maximum (log2 units), sum
     int4 item[kWarps][2];                                       // (row, KV head, first page, pages), row -1: none
-    uint64_t bars[kWarps][kStages<NT>];
+    uint64_t bars[kWarps][kStages];
     long long scan[kWarps];
     int np[kWarps][2];
     int start[3];                                               // the CTA's first row, KV head, unit
@@ -227,7 +225,7 @@ __device__ __forceinline__ float split_query(const float (&x)[32], int g, int t,
 template <int FMT, int NT>
 __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     kv8_decode_kernel(const __grid_constant__ CUtensorMap tm_pool, const Kv8AttnArgs a, void* scratch) {
-    constexpr int ST = kStages<NT>;
+    constexpr int ST = kStages;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     DecodeSmem<NT>& S = *reinterpret_cast<DecodeSmem<NT>*>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -697,12 +695,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv8_merge_kernel(const Kv8At
 
 template <int FMT, int NT>
 cudaError_t launch_decode(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scratch, int grid, cudaStream_t s) {
-    auto kern = kv8_decode_kernel<FMT, NT>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DecodeSmem<NT>));
-    if (e != cudaSuccess) return e;
-    kern<<<grid, kWarps * 32, sizeof(DecodeSmem<NT>), s>>>(tm, a, scratch);
+    kv8_decode_kernel<FMT, NT><<<grid, kWarps * 32, sizeof(DecodeSmem<NT>), s>>>(tm, a, scratch);
     if (grid == 1) return cudaGetLastError();
-    e = cudaGetLastError();
+    const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     // launched while the decode kernel runs; it waits for that kernel's end before it reads
     cudaLaunchConfig_t cfg = {};
@@ -718,6 +713,16 @@ cudaError_t launch_decode(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scr
 }
 
 }  // namespace
+
+// Opt the kernels into their dynamic shared memory on the current device.
+void configure_kv8_attention() {
+    const cudaFuncAttribute attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    cudaFuncSetAttribute(kv8_decode_kernel<kInt8, 1>, attr, (int)sizeof(DecodeSmem<1>));
+    cudaFuncSetAttribute(kv8_decode_kernel<kInt8, 2>, attr, (int)sizeof(DecodeSmem<2>));
+    cudaFuncSetAttribute(kv8_decode_kernel<kE4m3, 1>, attr, (int)sizeof(DecodeSmem<1>));
+    cudaFuncSetAttribute(kv8_decode_kernel<kE4m3, 2>, attr, (int)sizeof(DecodeSmem<2>));
+}
+
 }  // namespace fa
 
 extern "C" FA_API size_t fa_op_attention_kv8_scratch_bytes(int M, int n_heads, int n_kv_heads) {
@@ -737,6 +742,7 @@ extern "C" FA_API int fa_op_paged_attention_kv8(const float* q, int M, int n_hea
     if (int rc = kv8_attention_check("fa_op_paged_attention_kv8", a, format, scratch, scratch_bytes,
                        fa_op_attention_kv8_scratch_bytes(M, n_heads, n_kv_heads)))
         return rc;
+    if (int rc = ensure_device_configured()) return report_op_error(rc, "fa_op_paged_attention_kv8: no CUDA device");
     CUtensorMap tm;
     if (!make_kv8_tile_map(&tm, pool_layer, (long long)n_pages * n_kv_heads * (kTileBytes / 128)))
         return report_op_error(FA_ERR_CUDA, "fa_op_paged_attention_kv8: cannot build the page-pool tensor map");

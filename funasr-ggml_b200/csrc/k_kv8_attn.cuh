@@ -16,6 +16,7 @@
 namespace fa {
 
 int report_op_error(int code, const char* msg);   // fa_api.cu
+int ensure_device_configured();                   // fa_api.cu: kernel attributes of the current device, once
 
 namespace kv8 {
 
@@ -40,8 +41,8 @@ struct Kv8AttnArgs {
 
 // A row that cannot be served.
 __device__ __forceinline__ bool row_bad(const Kv8AttnArgs& a, int m) {
-    const int pos = a.pos[m];
-    return pos < -1 || pos / kPageTokens >= a.bt_stride || (pos >= 0 && a.slot[m] < 0);
+    const int pos = a.pos[m], slot = a.slot[m];      // both under way at once
+    return pos < -1 || pos / kPageTokens >= a.bt_stride || (pos >= 0 && slot < 0);
 }
 
 // The power of two at or below x, within 2^-126 .. 2^126, and the inverse of such a one.

@@ -707,15 +707,12 @@ int max_parts(int n_tiles, int n_kv_heads) {
 
 template <int FMT>
 cudaError_t launch_prefill(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scratch, cudaStream_t s) {
-    auto kern = kv8_prefill_kernel<FMT>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PfSmem));
-    if (e != cudaSuccess) return e;
     const int parts = max_parts(a.n_tiles, a.Hkv);
     float* part_o = static_cast<float*>(scratch);
     float2* part_ml =
         parts > 1 ? reinterpret_cast<float2*>(part_o + (size_t)a.n_tiles * a.Hkv * parts * 128 * D) : nullptr;
-    kern<<<dim3(a.Hkv, a.n_tiles, parts), THREADS, sizeof(PfSmem), s>>>(tm, a, part_o, part_ml);
-    e = cudaGetLastError();
+    kv8_prefill_kernel<FMT><<<dim3(a.Hkv, a.n_tiles, parts), THREADS, sizeof(PfSmem), s>>>(tm, a, part_o, part_ml);
+    const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || parts == 1) return e;
     // launched while the kernel above runs; it waits for that kernel's end before it reads
     cudaLaunchConfig_t cfg = {};
@@ -731,6 +728,14 @@ cudaError_t launch_prefill(const CUtensorMap& tm, const Kv8AttnArgs& a, void* sc
 }
 
 }  // namespace
+
+// Opt the kernels into their dynamic shared memory on the current device.
+void configure_kv8_prefill() {
+    const cudaFuncAttribute attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    cudaFuncSetAttribute(kv8_prefill_kernel<kInt8>, attr, (int)sizeof(PfSmem));
+    cudaFuncSetAttribute(kv8_prefill_kernel<kE4m3>, attr, (int)sizeof(PfSmem));
+}
+
 }  // namespace fa
 
 extern "C" FA_API size_t fa_op_prefill_attention_kv8_scratch_bytes(int n_tiles, int n_heads, int n_kv_heads) {
@@ -755,6 +760,7 @@ extern "C" FA_API int fa_op_prefill_attention_kv8(const float* q, int M, int n_h
         return rc;
     if (n_tiles > 65535)
         return report_op_error(FA_ERR_CAPACITY, "fa_op_prefill_attention_kv8: more than 65535 tiles");
+    if (int rc = ensure_device_configured()) return report_op_error(rc, "fa_op_prefill_attention_kv8: no CUDA device");
     CUtensorMap tm;
     if (!make_kv8_tile_map(&tm, pool_layer, (long long)n_pages * n_kv_heads * (kTileBytes / 128)))
         return report_op_error(FA_ERR_CUDA, "fa_op_prefill_attention_kv8: cannot build the page-pool tensor map");
