@@ -37,13 +37,17 @@ constexpr int PAGES = KB / kPageTokens;
 constexpr int RAW = 3;                        // raw ring (8-bit blocks)
 constexpr int TILES = 4;                      // f16 ring
 constexpr int THREADS = 512;
+constexpr int kRegsIssue = 72, kRegsExpand = 88, kRegsSoftmax = 176;
+static_assert(kRegsIssue + kRegsExpand + 2 * kRegsSoftmax <= 4 * 128, "registers of the launch");
 constexpr int kMaxParts = 16;                 // key ranges of one tile and head
 constexpr int kMinPartBlocks = 8;
 // TMEM columns: S / w of block j at 64 (j % 3), O of the even blocks [192, 320) and of the odd
 // ones [320, 448), Q hi [448, 512)
 constexpr int SBUF = 3;
 constexpr uint32_t TMEM_COLS = 512, COL_O = 192, COL_Q = 448;
-constexpr float kLazy = 11.0f;                // log2 units
+// A running maximum is set kRoom above the block's and stays until a block exceeds it by kLazy
+// (log2 units): weights reach 2^kLazy, and O is rescaled once in kRoom + kLazy.
+constexpr float kLazy = 11.0f, kRoom = 4.0f;
 constexpr uint32_t kSigmaShift = 3;           // the largest V scale over sigma is 2^3 to 2^4: w < 2^15
 
 struct PfSmem {
@@ -137,6 +141,12 @@ __device__ __forceinline__ void tc_commit_if(uint32_t one, uint64_t* bar) {
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return attn::ffma2(a, make_float2(1.0f, 1.0f), b);
+}
+
+__device__ __forceinline__ uint2 lds64(const void* p) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(smem_u32(p)));
+    return v;
 }
 
 // A barrier of warps 8-15.
@@ -249,8 +259,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int parts = part_blocks((pos_last + KB) / KB, max_parts, blockIdx.z, first, last);
     const int n_blocks = bad || blockIdx.z >= parts ? 0 : last - first;
 
-    if (bad || (int)blockIdx.z >= parts) {
-        // nothing issued: fall through to the TMEM release
+    // 128 registers a thread at launch, of which the softmax warps take over what the others can
+    // spare: 128 threads each of kRegsIssue + kRegsExpand + 2 kRegsSoftmax = 4 x 128
+    const bool idle = bad || (int)blockIdx.z >= parts;  // nothing issued: on to the TMEM release
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    if (idle) {
     } else if (warp == 0) {
         const int* bt = a.block_table + (size_t)slot * a.bt_stride;
         const int last_page = pos_last / kPageTokens;
@@ -342,10 +356,14 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!ok && lane == 0) S.err = 1;
         }
         __syncwarp();
-    } else if (warp >= 4 && warp < 8) {
-        // expansion: thread c takes 16-byte chunk c % 8 of tokens c / 8, c / 8 + 16, ..., K and V
+    }
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsExpand));
+        // expansion: a thread takes 8 bytes, dims 8 c .., of every eighth token, K and V (one 16-byte
+        // chunk of the f16 tile each: eight lanes read and write whole rows, without bank conflicts)
         const int ct = threadIdx.x - 128, cw = warp - 4;
-        const int chunk = ct & 7;
+        const int c = ct & 15, r = ct >> 4;
+        const uint32_t raw_at = r * 128 + (((c >> 1) ^ r) << 4) + (c & 1) * 8;
         uint32_t run = 0;                              // exponent field of sigma
         bool ok = true;
         for (int j = 0; j < n_blocks; ++j) {
@@ -385,36 +403,29 @@ __global__ void __launch_bounds__(THREADS, 1)
                     S.pages[d] = have;
                 }
             }
-            // token 16 i + r of the block, dims 16 chunk ..: all loads before the first store
-            const int r = ct >> 3;
-            uint4 x[2 * PAGES];
+            // token 8 i + r of the block, dims 8 c ..: all loads of K (then V) before the first store
+            unsigned char* k_out = reinterpret_cast<unsigned char*>(S.k[d][c >> 3]) + sw128(r, c & 7);
+            unsigned char* v_out = reinterpret_cast<unsigned char*>(S.v[d][c >> 3]) + sw128(r, c & 7);
+            const bool whole = have == (1 << PAGES) - 1 && key0 + KB - 1 <= pos_last;
 #pragma unroll
-            for (int i = 0; i < 2 * PAGES; ++i)
-                x[i] = lds128(S.raw[s][i >> 1] + (i & 1) * kPartBytes + r * 128 + ((chunk ^ (r & 7)) << 4));
-            // tokens of pages left out, and V behind the last token (unwritten bytes may be e4m3 NaN)
-            if (have != (1 << PAGES) - 1 || key0 + KB - 1 > pos_last) {
+            for (int part = 0; part < 2; ++part) {
+                uint2 x[KB / 8];
 #pragma unroll
-                for (int i = 0; i < 2 * PAGES; ++i)
-                    if (!((have >> (i >> 1)) & 1) || ((i & 1) && key0 + (i >> 1) * kPageTokens + r > pos_last))
-                        x[i] = make_uint4(0, 0, 0, 0);
-            }
-            // chunks 2 (chunk % 4), + 1 of the half's row; the upper half's threads write them in the
-            // other order, which spreads a row's stores over all banks
-            const int up = chunk >> 2, c2 = 2 * (chunk & 3);
-            const uint32_t o0 = sw128(r, c2 + up), o1 = sw128(r, c2 + 1 - up);
-            unsigned char* k_out = reinterpret_cast<unsigned char*>(S.k[d][up]);
-            unsigned char* v_out = reinterpret_cast<unsigned char*>(S.v[d][up]);
+                for (int i = 0; i < KB / 8; ++i)
+                    x[i] = lds64(S.raw[s][i >> 1] + part * kPartBytes + (i & 1) * 1024 + raw_at);
+                // tokens of pages left out, and V behind the last token (unwritten bytes may be e4m3 NaN)
+                if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 2 * PAGES; ++i) {
-                __half2 y[8];
-                expand4<FMT>(x[i].x, y[0], y[1]);
-                expand4<FMT>(x[i].y, y[2], y[3]);
-                expand4<FMT>(x[i].z, y[4], y[5]);
-                expand4<FMT>(x[i].w, y[6], y[7]);
-                const uint4* w = reinterpret_cast<const uint4*>(y);
-                unsigned char* out = ((i & 1) ? v_out : k_out) + (i >> 1) * kPageTokens * 128;
-                *reinterpret_cast<uint4*>(out + o0) = up ? w[1] : w[0];
-                *reinterpret_cast<uint4*>(out + o1) = up ? w[0] : w[1];
+                    for (int i = 0; i < KB / 8; ++i)
+                        if (!((have >> (i >> 1)) & 1) || (part && key0 + 8 * i + r > pos_last)) x[i] = make_uint2(0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < KB / 8; ++i) {
+                    __half2 y[4];
+                    expand4<FMT>(x[i].x, y[0], y[1]);
+                    expand4<FMT>(x[i].y, y[2], y[3]);
+                    *reinterpret_cast<uint4*>((part ? v_out : k_out) + i * 1024) = *reinterpret_cast<const uint4*>(y);
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -424,7 +435,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
         }
         if (!ok && lane == 0) S.err = 1;
-    } else if (warp >= 8) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+        if (!idle) {
         // Warps 8-11 the even blocks, 12-15 the odd ones, each with its own running maximum, sum
         // and O: while one group works on S of a block, the MMAs make the other's. Thread t of a
         // group owns TMEM lane t = query vector t (a warp may only touch lanes 32 * (warp % 4) ..).
@@ -487,7 +500,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const float qs = n_blocks > 0 ? S.qs[t] : 0.0f;
         // running maximum of dk S (before qs), the same in log2 units, and the sum of weights
         float top = -INFINITY, top2 = -INFINITY, sum = 0.0f, sigma = 1.0f;
-        const float lazy = kLazy / qs;
+        const float lazy = fminf(kLazy / qs, 1e37f), room = fminf(kRoom / qs, 1e37f);
         const uint32_t to = tl + COL_O + (uint32_t)(odd * D);
         bool ok = true;
         for (int j = odd; j < n_blocks; j += 2) {
@@ -535,12 +548,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             float alpha = j > 1 ? sigma * pow2_inverse(next_sigma) : 1.0f;
             sigma = next_sigma;
             if (top == -INFINITY) {
-                top = bmax;                            // first block with a key: O holds nothing of this row
+                top = bmax + room;                     // first block with a key: O holds nothing of this row
                 top2 = __fmul_rn(top, qs);
             } else if (bmax > top + lazy) {
-                const float next = __fmul_rn(bmax, qs);
+                top = bmax + room;
+                const float next = __fmul_rn(top, qs);
                 const float f = exp2f(top2 - next);
-                top = bmax;
                 top2 = next;
                 alpha *= f;
                 sum *= f;
@@ -641,6 +654,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     store_values<32>(a, o_at + c, o);
                 }
             }
+        }
         }
     }
     tc_fence_before();
