@@ -635,23 +635,23 @@ __global__ void __launch_bounds__(THREADS, 1)
                 f1 *= inv;
             }
 #pragma unroll 1
-            for (int c = 64 * odd; c < 64 * odd + 64; c += 32) {
-                uint32_t ov[32], ow[32];
-                if (n_blocks > 0) TMEM_LD_X32(tl + COL_O + c, ov);
-                if (n_blocks > 1) TMEM_LD_X32(tl + COL_O + D + c, ow);
+            for (int c = 64 * odd; c < 64 * odd + 64; c += 16) {   // small: every CTA fetches this code once
+                uint32_t ov[16], ow[16];
+                if (n_blocks > 0) TMEM_LD_X16(tl + COL_O + c, ov);
+                if (n_blocks > 1) TMEM_LD_X16(tl + COL_O + D + c, ow);
                 tmem_wait_ld();
-                float o[32];
+                float o[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
+                for (int e = 0; e < 16; ++e) {
                     o[e] = n_blocks > 0 ? __uint_as_float(ov[e]) * f0 : 0.0f;
                     if (n_blocks > 1) o[e] = fmaf(__uint_as_float(ow[e]), f1, o[e]);
                 }
                 if (parts > 1) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
+                    for (int e = 0; e < 16; e += 4)
                         *reinterpret_cast<float4*>(part_o + at * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 } else if (live) {
-                    store_values<32>(a, o_at + c, o);
+                    store_values<16>(a, o_at + c, o);
                 }
             }
         }
