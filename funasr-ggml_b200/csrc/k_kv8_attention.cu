@@ -32,7 +32,7 @@ int kv8_attention_check(const std::string& what, const Kv8AttnArgs& a, int forma
         misaligned(a.out32, 16) || misaligned(scratch, 16))
         return report_op_error(FA_ERR_INVALID_ARG,
                                (what + ": q, outputs and scratch must be 16-byte, pool 128-byte aligned").c_str());
-    if (a.Hq > 65535 || (long long)a.bt_stride * kPageTokens > 0x7fffffffll)
+    if (a.Hq > 65535 || (long long)a.bt_stride * kPageTokens > (1ll << 30))
         return report_op_error(FA_ERR_CAPACITY, (what + ": n_heads or bt_stride too large").c_str());
     if ((long long)a.n_pages * a.Hkv * (kTileBytes / 128) > 0x7fffffffll)
         return report_op_error(FA_ERR_CAPACITY, (what + ": the pool has too many pages").c_str());

@@ -617,6 +617,149 @@ def test_prefill_attention_flags_bad_tiles(torch_cuda, tile, pos, page, bits):
             assert (got[64:] == 5).all()
 
 
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,chunks", [
+    (16, 8, [(4000, 3)]), (16, 8, [(1100, 64), (3000, 70)]), (8, 1, [(6000, 20)]), (32, 8, [(2500, 32)]),
+    (5, 5, [(1500, 130)]), (16, 2, [(9000, 1)])])
+def test_prefill_attention_few_tiles_over_long_contexts(torch_cuda, fmt, hq, hkv, chunks):
+    """Calls of few tiles, whose keys are cut into parts: every row against the definition."""
+    torch = torch_cuda
+    rng = np.random.default_rng(hq + chunks[0][0])
+    lens = [b + n for b, n in chunks]
+    pool, bt, n_pages = _filled(rng, lens, 1, hkv, fmt)
+    pos = np.concatenate([np.arange(b, b + n) for b, n in chunks]).astype(np.int32)
+    slot = np.repeat(np.arange(len(chunks)), [n for _, n in chunks]).astype(np.int32)
+    first = np.concatenate([[0], np.cumsum([n for _, n in chunks])[:-1]])
+    tiles = _tiles([(int(f), n) for f, (_, n) in zip(first, chunks)], 128 * hkv // hq)
+    assert fa_dec.op_prefill_attention_kv8_scratch_bytes(len(tiles), hq, hkv) > 0
+    M = len(pos)
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    err = _err(torch)
+    out16, lo = (torch.zeros((M, hq * 128), dtype=torch.float16, device="cuda") for _ in range(2))
+    got = _prefill(torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, slot), dev(torch, bt), n_pages, fmt,
+                   dev(torch, pool), tiles, err, out16, lo).cpu().numpy()
+    pair = (out16.float() + lo.float()).cpu().numpy()
+    assert int(err) == 0
+    for m in range(M):
+        k, v = (x[0] for x in P.read(pool, bt[slot[m]], 0, pos[m] + 1, fmt))
+        want = P.attention(q[m], k, v).reshape(-1)
+        assert np.abs(got[m] - want).max() <= _bound(q[m], k, v)
+        assert rel_rms(got[m], want) <= 5e-6, m
+        assert np.abs(pair[m] - got[m]).max() <= np.abs(got[m]).max() * 2.0 ** -21 + 2.0 ** -24
+
+
+def test_prefill_attention_parts_with_padding_nan_and_a_bad_page(torch_cuda):
+    """Keys in parts: rows that see none of a part's keys, a NaN vector in the last part only,
+    a page outside the pool in the middle, a row of another sequence."""
+    torch = torch_cuda
+    rng = np.random.default_rng(14)
+    hq, hkv, n = 16, 8, 4000
+    pool, bt, n_pages = _filled(rng, [n, 64], 1, hkv, P.INT8)
+    _, scales = P.parts(pool)
+    scales[0, bt[0, 3900 // 16], 3, 1, 3900 % 16] = np.nan
+    kb = bt.copy()
+    kb[0, 2000 // 16] = n_pages + 7                               # tokens 2000..2015
+    pos = np.array([-1, 5, 63, 1500, 3899, 3900, 3999, 3999], np.int32)
+    slot = np.array([77, 0, 0, 0, 0, 0, 0, 1], np.int32)
+    M = len(pos)
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    err = _err(torch)
+    got = _prefill(torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, slot), dev(torch, kb), n_pages, P.INT8,
+                   dev(torch, pool), np.array([[0, 8]], np.int32), err).cpu().numpy()
+    assert int(err) == 2 | 8
+    assert not got[0].any() and (got[7] == 5).all()
+    for m in range(1, 7):
+        keep = np.array([t for t in range(pos[m] + 1) if not 2000 <= t < 2016])
+        k, v = (x[0][:, keep] for x in P.read(pool, bt[0], 0, pos[m] + 1, P.INT8))
+        want, out = P.attention(q[m], k, v), got[m].reshape(hq, 128)
+        heads = [h for h in range(hq) if not (pos[m] >= 3900 and h // 2 == 3)]
+        assert rel_rms(out[heads], want[heads]) <= 5e-6, m
+        assert np.isnan(out).all(-1).tolist() == [h not in heads for h in range(hq)]
+
+
+@pytest.mark.parametrize("hq,hkv,M,longest", [(16, 8, 700, 40), (64, 64, 9, 300), (8, 2, 1500, 17), (200, 200, 3, 50),
+                                               (16, 8, 2, 16)])
+def test_decode_attention_many_short_rows_and_many_heads(torch_cuda, hq, hkv, M, longest):
+    """More rows than a CTA has threads, rows of one page beside long ones, padding runs, more KV
+    heads than usual; f16 output alone, no error word."""
+    torch = torch_cuda
+    rng = np.random.default_rng(M)
+    lens = rng.integers(1, longest + 1, 40).tolist()
+    lens[3] = 3 * longest
+    pool, bt, n_pages = _filled(rng, lens, 1, hkv, P.INT8)
+    slot = rng.integers(0, 40, M).astype(np.int32)
+    pos = np.array([rng.integers(0, lens[s]) for s in slot], np.int32)
+    pos[M // 3:M // 3 + M // 5] = -1
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    out16 = torch.full((M, hq * 128), 5.0, dtype=torch.float16, device="cuda")
+    size = fa_dec.op_attention_kv8_scratch_bytes(M, hq, hkv)
+    d = [dev(torch, a) for a in (q, pos, slot, bt, pool)]
+    p, scratch = [x.data_ptr() for x in d], _scratch(torch, size)
+    fa_dec.op_paged_attention_kv8(p[0], M, hq, hkv, p[1], p[2], p[3], bt.shape[1], n_pages, P.INT8, p[4],
+                                  scratch.data_ptr(), size, out16=out16.data_ptr(), stream=_stream(torch))
+    got = out16.float().cpu().numpy()
+    for m in np.unique(np.concatenate([np.arange(0, M, max(1, M // 60)), [M - 1]])):
+        if pos[m] < 0:
+            assert not got[m].any()
+            continue
+        k, v = (x[0] for x in P.read(pool, bt[slot[m]], 0, pos[m] + 1, P.INT8))
+        want = P.attention(q[m], k, v).reshape(-1)
+        # half a step of f16 (2^-11 relative, 2^-25 among the subnormals) on top of the f32 bound
+        assert (np.abs(got[m] - want) <= _bound(q[m], k, v) + np.abs(want) * 2.0 ** -11 + 2.0 ** -25).all()
+
+
+def test_all_rows_padding(torch_cuda):
+    torch = torch_cuda
+    hq, hkv, M = 16, 8, 70
+    pos, slot = dev(torch, np.full(M, -1, np.int32)), dev(torch, np.full(M, 10 ** 6, np.int32))
+    bt, pool = dev(torch, np.full((1, 4), 99, np.int32)), torch.full((1, 2, hkv, P.TILE), 255, dtype=torch.uint8, device="cuda")
+    q, err = torch.full((M, hq, 128), float("nan"), device="cuda"), _err(torch)
+    assert not bool(_decode(torch, q, hq, hkv, pos, slot, bt, 2, P.E4M3, pool, err).any())
+    assert not bool(_prefill(torch, q, hq, hkv, pos, slot, bt, 2, P.E4M3, pool, _tiles([(0, M)], 64), err).any())
+    kv = torch.ones((M, hkv * 128), device="cuda")
+    _append(torch, kv, kv, P.F32, hkv * 128, M, 1, hkv, pos, slot, bt, 2, P.E4M3, pool, err)
+    assert bool((pool == 255).all()) and int(err) == 0
+
+
+def test_prefill_from_a_graph_and_two_at_once(torch_cuda):
+    """One captured prefill call (keys in parts) replayed with other positions, while another
+    call with scratch of its own runs on a second stream."""
+    torch = torch_cuda
+    rng = np.random.default_rng(15)
+    hq, hkv, n, M = 16, 8, 3000, 40
+    pool, bt, n_pages = _filled(rng, [n], 1, hkv, P.E4M3)
+    d_pool, d_bt, slot = dev(torch, pool), dev(torch, bt), dev(torch, np.zeros(M, np.int32))
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    d_q, pos, err = dev(torch, q), dev(torch, np.arange(M, dtype=np.int32)), _err(torch)
+    tiles = dev(torch, np.array([[0, M]], np.int32))
+    size = fa_dec.op_prefill_attention_kv8_scratch_bytes(1, hq, hkv)
+    scratch, out = _scratch(torch, size), torch.zeros((M, hq * 128), device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        fa_dec.op_prefill_attention_kv8(d_q.data_ptr(), M, hq, hkv, pos.data_ptr(), slot.data_ptr(), d_bt.data_ptr(),
+                                        bt.shape[1], n_pages, P.E4M3, d_pool.data_ptr(), tiles.data_ptr(), 1,
+                                        scratch.data_ptr(), size, out32=out.data_ptr(), err=err.data_ptr(),
+                                        stream=_stream(torch))
+    other = None
+    for start in (0, 500, n - M):
+        pos.copy_(dev(torch, np.arange(start, start + M, dtype=np.int32)))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        beside = _prefill(torch, d_q, hq, hkv, dev(torch, np.arange(n - M, n, dtype=np.int32)), slot, d_bt, n_pages,
+                          P.E4M3, d_pool, np.array([[0, M]], np.int32), err)
+        torch.cuda.synchronize()
+        assert other is None or torch.equal(other, beside)
+        other = beside
+        got = out.cpu().numpy()
+        for m in range(0, M, 7):
+            k, v = (x[0] for x in P.read(pool, bt[0], 0, start + m + 1, P.E4M3))
+            assert rel_rms(got[m], P.attention(q[m], k, v).reshape(-1)) <= 5e-6
+    assert torch.equal(out, other) and int(err) == 0
+
+
 # ---------------------------------------------------------------- together --
 @pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
 def test_a_layers_steps_together_and_from_a_graph(torch_cuda, fmt):
