@@ -325,12 +325,18 @@ __global__ void __launch_bounds__(THREADS, 1)
                     tc_fence_after();
                     const uint32_t d_s = tmem + (uint32_t)(i % SBUF * KB);
                     const uint64_t db = k_desc + (uint32_t)(s * (int)sizeof(S.k[0]) >> 4);
+                    // the low parts first: the sums are rounded at the size of the low products then, and
+                    // only the eight steps of the high parts at that of a score
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk) {
-                        const uint32_t in_row = (kk & 3) * 32 / 16;
-                        const uint64_t at = db + (kk >> 2) * (int)sizeof(S.k[0][0]) / 16 + in_row;
-                        tc_mma_f16_ts_if(one, d_s, tmem + COL_Q + 8 * kk, at, kIdS, kk > 0 ? 1u : 0u);
-                        tc_mma_f16_if(one, d_s, q_desc + (kk >> 2) * (int)sizeof(S.q_lo[0]) / 16 + in_row, at, kIdS, 1u);
+                        const uint64_t in_tile = (kk >> 2) * (int)sizeof(S.k[0][0]) / 16 + (kk & 3) * 32 / 16;
+                        const uint64_t in_q = (kk >> 2) * (int)sizeof(S.q_lo[0]) / 16 + (kk & 3) * 32 / 16;
+                        tc_mma_f16_if(one, d_s, q_desc + in_q, db + in_tile, kIdS, kk > 0 ? 1u : 0u);
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk) {
+                        const uint64_t in_tile = (kk >> 2) * (int)sizeof(S.k[0][0]) / 16 + (kk & 3) * 32 / 16;
+                        tc_mma_f16_ts_if(one, d_s, tmem + COL_Q + 8 * kk, db + in_tile, kIdS, 1u);
                     }
                     tc_commit_if(one, &S.s_full[i % SBUF]);
                 }
