@@ -37,8 +37,12 @@ constexpr int PAGES = KB / kPageTokens;
 constexpr int RAW = 3;                        // raw ring (8-bit blocks)
 constexpr int TILES = 4;                      // f16 ring
 constexpr int THREADS = 512;
-constexpr int kRegsIssue = 72, kRegsExpand = 88, kRegsSoftmax = 176;
+constexpr int kRegsIssue = 56, kRegsExpand = 72, kRegsSoftmax = 192;
 static_assert(kRegsIssue + kRegsExpand + 2 * kRegsSoftmax <= 4 * 128, "registers of the launch");
+// Blocks summed in TMEM at a time. The tensor core's f32 sums are truncated, so their error grows
+// with their length (2.4e-6 of the output over 60 blocks); stretches are joined in f32 arithmetic
+// rounded to nearest.
+constexpr int STRETCH = 32;
 constexpr int kMaxParts = 16;                 // key ranges of one tile and head
 constexpr int kMinPartBlocks = 8;
 // TMEM columns: S / w of block j at 64 (j % 3), O of the even blocks [192, 320) and of the odd
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
                         const uint64_t at = db + kk * 16 * 64 * 2 / 16;
-                        tc_mma_f16_ts_if(one, d_o, d_p + 8 * kk, at, kIdPV, (j > 1 || kk > 0) ? 1u : 0u);
+                        tc_mma_f16_ts_if(one, d_o, d_p + 8 * kk, at, kIdPV, (j % STRETCH > 1 || kk > 0) ? 1u : 0u);
                         tc_mma_f16_ts_if(one, d_o, d_p + 32 + 8 * kk, at, kIdPV, 1u);
                     }
                     tc_commit_if(one, &S.kv_empty[s]);
@@ -504,12 +508,19 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_arrive(&S.q_ready);
         }
         const float qs = n_blocks > 0 ? S.qs[t] : 0.0f;
-        // running maximum of dk S (before qs), the same in log2 units, and the sum of weights
-        float top = -INFINITY, top2 = -INFINITY, sum = 0.0f, sigma = 1.0f;
         const float lazy = fminf(kLazy / qs, 1e37f), room = fminf(kRoom / qs, 1e37f);
         const uint32_t to = tl + COL_O + (uint32_t)(odd * D);
+        const size_t at = part_index(a, blockIdx.y, h, max_parts, blockIdx.z) + t;
+        // over the stretches joined so far: maximum, sum, and the group's half of the dims
+        float all_max = -INFINITY, all_sum = 0.0f, acc[64];
+#pragma unroll
+        for (int e = 0; e < 64; ++e) acc[e] = 0.0f;
         bool ok = true;
-        for (int j = odd; j < n_blocks; j += 2) {
+        for (int j0 = 0; j0 == 0 || j0 < n_blocks; j0 += STRETCH) {
+        const int j1 = min(j0 + STRETCH, n_blocks);
+        // running maximum of dk S (before qs), the same in log2 units, and the sum of weights
+        float top = -INFINITY, top2 = -INFINITY, sum = 0.0f, sigma = 1.0f;
+        for (int j = j0 + odd; ok && j < j1; j += 2) {
             const int d = j % TILES;
             const bool got = mbar_wait_bounded(&S.kv_full[d], (uint32_t)(j / TILES) & 1u) &&
                              mbar_wait_bounded(&S.s_full[j % SBUF], (uint32_t)(j / SBUF) & 1u);
@@ -551,7 +562,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int c = 0; c < KB; ++c) bmax = fmaxf(bmax, __uint_as_float(sv[c]));
             const float next_sigma = S.sigma[d];
-            float alpha = j > 1 ? sigma * pow2_inverse(next_sigma) : 1.0f;
+            float alpha = j - j0 > 1 ? sigma * pow2_inverse(next_sigma) : 1.0f;
             sigma = next_sigma;
             if (top == -INFINITY) {
                 top = bmax + room;                     // first block with a key: O holds nothing of this row
@@ -564,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 alpha *= f;
                 sum *= f;
             }
-            if (j > 1 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+            if (j - j0 > 1 && __any_sync(0xffffffffu, alpha != 1.0f)) {
                 const bool od = mbar_wait_bounded(&S.o_done[odd], (uint32_t)((j >> 1) - 1) & 1u);
                 if (!__all_sync(0xffffffffu, od)) { ok = false; break; }
                 tc_fence_after();
@@ -580,7 +591,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             const float4* dv = reinterpret_cast<const float4*>(S.dv[d]);
             const float2 qs2 = make_float2(qs, qs), neg = make_float2(-top2, -top2), minus = make_float2(-1.0f, -1.0f);
-            float2 acc = make_float2(0.0f, 0.0f);
+            float2 psum = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 uint32_t hi[16], lo[16];
@@ -598,7 +609,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                             p = make_float2(in & 1 ? p.x : 0.0f, in & 2 ? p.y : 0.0f);
                             w = make_float2(in & 1 ? w.x : 0.0f, in & 2 ? w.y : 0.0f);
                         }
-                        acc = add2(acc, p);
+                        psum = add2(psum, p);
                         const uint32_t hw = pack2(w.x, w.y);
                         const float2 rest = attn::ffma2(h2_to_f2(hw), minus, w);
                         hi[(c + e) >> 1] = hw;
@@ -608,15 +619,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                 TMEM_ST_X16(ts + 16 * half, hi);
                 TMEM_ST_X16(ts + 32 + 16 * half, lo);
             }
-            sum += acc.x + acc.y;
+            sum += psum.x + psum.y;
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&S.p_ready[j % SBUF]);
         }
-        // the group's last product: block n_blocks - 1 or n_blocks - 2
-        const int mine = (n_blocks + 1 - odd) >> 1;    // blocks of this group
-        if (ok && mine > 0) {
-            const bool od = mbar_wait_bounded(&S.o_done[odd], (uint32_t)(mine - 1) & 1u);
+        // the group's last product of the stretch: block j1 - 1 or j1 - 2
+        const int last_j = ((j1 - 1 - odd) & ~1) + odd;
+        if (ok && last_j >= j0 && j1 > odd) {
+            const bool od = mbar_wait_bounded(&S.o_done[odd], (uint32_t)(last_j >> 1) & 1u);
             ok = __all_sync(0xffffffffu, od);
         }
         if (!ok && lane == 0) S.err = 1;
@@ -627,37 +638,51 @@ __global__ void __launch_bounds__(THREADS, 1)
         group_sync();
         tc_fence_after();
         if (!S.err) {
-            // the two joined: out = (O0 f0 + O1 f1) / (sum0 f0 + sum1 f1); each group half of the dims
-            const float m0 = S.state[0][0][t], m1 = S.state[1][0][t], best = fmaxf(m0, m1);
+            // the two groups and the stretches before joined: acc = O0 f0 + O1 f1 + fa acc, each group half
+            // of the dims
+            const float m0 = S.state[0][0][t], m1 = S.state[1][0][t], best = fmaxf(fmaxf(m0, m1), all_max);
             float f0 = m0 == best ? 1.0f : exp2f(m0 - best), f1 = m1 == best ? 1.0f : exp2f(m1 - best);
-            sum = S.state[0][1][t] * f0 + S.state[1][1][t] * f1;
+            const float fa = all_max == best ? 1.0f : exp2f(all_max - best);
+            all_sum = S.state[0][1][t] * f0 + S.state[1][1][t] * f1 + all_sum * fa;
+            all_max = best;
             f0 *= S.state[0][2][t];
             f1 *= S.state[1][2][t];
-            const size_t at = part_index(a, blockIdx.y, h, max_parts, blockIdx.z) + t;
-            if (parts > 1 && !odd) part_ml[at] = make_float2(best, sum);
-            if (parts == 1) {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                f0 *= inv;
-                f1 *= inv;
-            }
-#pragma unroll 1
-            for (int c = 64 * odd; c < 64 * odd + 64; c += 16) {   // small: every CTA fetches this code once
-                uint32_t ov[16], ow[16];
-                if (n_blocks > 0) TMEM_LD_X16(tl + COL_O + c, ov);
-                if (n_blocks > 1) TMEM_LD_X16(tl + COL_O + D + c, ow);
-                tmem_wait_ld();
-                float o[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    o[e] = n_blocks > 0 ? __uint_as_float(ov[e]) * f0 : 0.0f;
-                    if (n_blocks > 1) o[e] = fmaf(__uint_as_float(ow[e]), f1, o[e]);
+            for (int c = 0; c < 64; c += 16) {
+                uint32_t ov[16];
+                if (j1 > j0) {
+                    TMEM_LD_X16(tl + COL_O + 64 * odd + c, ov);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(__uint_as_float(ov[e]), f0, acc[c + e] * fa);
                 }
-                if (parts > 1) {
+                if (j1 - j0 > 1) {
+                    TMEM_LD_X16(tl + COL_O + D + 64 * odd + c, ov);
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        *reinterpret_cast<float4*>(part_o + at * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(__uint_as_float(ov[e]), f1, acc[c + e]);
+                }
+            }
+        }
+        tc_fence_before();
+        group_sync();                                  // O and the state may be written again
+        tc_fence_after();
+        }
+        if (!S.err) {
+            // the part's un-normalised sum, or the output
+            const float inv = parts > 1 ? 1.0f : all_sum == 0.0f ? 0.0f : 1.0f / all_sum;
+            if (parts > 1 && !odd) part_ml[at] = make_float2(all_max, all_sum);
+#pragma unroll
+            for (int c = 0; c < 64; c += 8) {
+                float o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = acc[c + e] * inv;
+                if (parts > 1) {
+                    float4* dst = reinterpret_cast<float4*>(part_o + at * D + 64 * odd + c);
+                    dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+                    dst[1] = make_float4(o[4], o[5], o[6], o[7]);
                 } else if (live) {
-                    store_values<16>(a, o_at + c, o);
+                    store_values<8>(a, o_at + 64 * odd + c, o);
                 }
             }
         }
