@@ -58,6 +58,10 @@ __device__ __forceinline__ uint32_t settle(uint32_t m, float x, float d) {
     return a > h || (a == h && (m & 1)) ? m + (r > 0.0f ? 1u : ~0u) : m;
 }
 
+__device__ __forceinline__ uint32_t join4(const uint32_t (&m)[4]) {      // low bytes
+    return __byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410);
+}
+
 // Four values of a vector with scale d as stored bytes. inv = 1 / d (for e4m3 exact).
 template <int FMT>
 __device__ __forceinline__ uint32_t pack4(const float* x, float d, float inv) {
@@ -70,7 +74,7 @@ __device__ __forceinline__ uint32_t pack4(const float* x, float d, float inv) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) m[k] = settle(m[k], x[k], d);
         }
-        return __byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410);
+        return join4(m);
     }
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * inv, x[1] * inv), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * inv, x[3] * inv), __NV_SATFINITE, __NV_E4M3);

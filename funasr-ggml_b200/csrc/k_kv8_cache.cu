@@ -175,6 +175,73 @@ __device__ __forceinline__ void load4(const float* vec, int lane, float (&x)[4])
     x[3] = b.y;
 }
 
+// K is stored as if it had been computed in 64 bits and rounded once. Its f32 values are off by
+// less than 11 x 2^-24 of the vector's largest (the norm's scale by 3.5 roundings, two products
+// and a rotation by 4, whose terms together reach sqrt(2) of it), so their bytes can differ from
+// those of the exact values only next to a border: where one lies within that distance (and for
+// int8 what an ulp of the scale moves it by), the vector is computed again in 64 bits, a few
+// vectors in a hundred.
+constexpr float kKeyError = 12.5f / (1 << 24);
+
+// pack4 of key values, unless a value that differs by e may round otherwise (near).
+template <int FMT>
+__device__ __forceinline__ uint32_t pack_key(const float (&x)[4], float d, float inv, float e, bool& near) {
+    if (FMT == kInt8) {
+        uint32_t m[4];
+        float border = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m[k] = round_quotient(x[k], d, inv, border);
+        near = border >= 0.5f * d - e;
+        return join4(m);
+    }
+    const float a[4] = {x[0] - e, x[1] - e, x[2] - e, x[3] - e}, b[4] = {x[0] + e, x[1] + e, x[2] + e, x[3] + e};
+    const uint32_t q = pack4<FMT>(a, d, inv);
+    near = q != pack4<FMT>(b, d, inv);
+    return q;
+}
+
+// A key vector in 64 bits, by a warp: the lane's four stored bytes, and the scale.
+template <int FMT>
+__device__ __noinline__ uint32_t exact_key(const float* vec, int lane, const float* w, const float2* rot, float eps,
+                                           float& d) {
+    const float2 lo = reinterpret_cast<const float2*>(vec)[lane], hi = reinterpret_cast<const float2*>(vec)[lane + 32];
+    double y[4] = {lo.x, lo.y, hi.x, hi.y};
+    double ss = y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3];
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const double scale = rsqrt(ss * (1.0 / D) + (double)eps);
+    double amax = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] *= scale * (double)w[k];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const double a = y[k], b = y[k + 2], c = rot[k].x, s = rot[k].y;
+        y[k] = a * c - b * s;
+        y[k + 2] = a * s + b * c;
+        amax = fmax(amax, fmax(fabs(y[k]), fabs(y[k + 2])));
+    }
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    uint32_t q = 0;
+    if (FMT == kInt8) {
+        d = fmaxf(__double2float_rn(amax / 127.0), kMinScale);
+        const double inv = 1.0 / (double)d;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q |= ((uint32_t)__double2int_rn(y[k] * inv) & 0xffu) << (8 * k);
+        return q;
+    }
+    d = scale_of<FMT>(__float_as_uint(__double2float_ru(amax)));   // at most 448 d, and so rounded up
+    const double inv = (double)__frcp_rn(d);                      // exact: a power of two
+    float f[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {                                  // towards zero with the rest kept in the last bit
+        const double v = y[k] * inv;
+        const float z = __double2float_rz(v);
+        f[k] = (double)z == v ? z : __uint_as_float(__float_as_uint(z) | 1u);
+    }
+    return pack4<FMT>(f, 1.0f, 1.0f);
+}
+
 // Kernel (1) with an 8-bit end: a CTA per row and kQkvWarps * V of its head vectors, a warp V of
 // them (lane l holding dims 2l, 2l+1, 64+2l, 65+2l: both rotation pairs of a lane stay in it),
 // whose loads are under way together with that of the row's position. With V = 4 the vectors'
@@ -250,6 +317,12 @@ __global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
     }
     if (page < 0) return;
     const float d_mine = scale_of<FMT>(top), inv_mine = __frcp_rn(d_mine);
+    const float amax_mine = __uint_as_float(top), e_mine = amax_mine * kKeyError;
+    // e4m3 scales that the error of the largest value may change
+    const uint32_t unsure =
+        FMT == kInt8 ? 0u
+                     : __ballot_sync(0xffffffffu, scale_of<FMT>(__float_as_uint(amax_mine + e_mine)) !=
+                                                      scale_of<FMT>(__float_as_uint(amax_mine - e_mine)));
     const int t = pos % kPageTokens;
 #pragma unroll
     for (int u = 0; u < V; ++u) {
@@ -257,8 +330,19 @@ __global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
         if (j < a.Hq) continue;
         if (j >= n_vec) break;
         const int part = j < a.Hq + a.Hkv ? 0 : 1, h = j - a.Hq - part * a.Hkv;
-        const float d = __shfl_sync(0xffffffffu, d_mine, u), inv = __shfl_sync(0xffffffffu, inv_mine, u);
-        const uint32_t q = d == d ? pack4<FMT>(x[u], d, inv) : 0u;
+        float d = __shfl_sync(0xffffffffu, d_mine, u);
+        const float inv = __shfl_sync(0xffffffffu, inv_mine, u);
+        uint32_t q = 0;
+        if (d == d) {
+            if (part == 0) {
+                bool near;
+                q = pack_key<FMT>(x[u], d, inv, __shfl_sync(0xffffffffu, e_mine, u), near);
+                if (((unsure >> u) & 1) || __any_sync(0xffffffffu, near))
+                    q = exact_key<FMT>(a.qkv + ((size_t)m * n_vec + j) * D, lane, kw, rot, a.eps, d);
+            } else {
+                q = pack4<FMT>(x[u], d, inv);
+            }
+        }
         unsigned char* tile = a.pool + ((size_t)page * a.Hkv + h) * kTileBytes;
         uint16_t* dst = reinterpret_cast<uint16_t*>(tile + part * kPartBytes + t * D) + lane;
         dst[0] = (uint16_t)q;

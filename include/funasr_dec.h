@@ -410,13 +410,17 @@ FA_API size_t fa_op_kv8_page_bytes(int n_kv_heads); /* one page of one layer; 0 
  * values of src_type (FA_TYPE_F32, F16 or BF16), row_stride elements apart (so K and V may be
  * slices of one projection), 16-byte aligned; pool [n_layers][n_pages][n_kv_heads][4224].
  * Rows of one call go to distinct (slot, pos). A position below -1 or past the block-table row
- * sets error bit 4 and a page outside the pool bit 2; such a row appends nothing. */
+ * or a negative slot sets error bit 4, and a page outside the pool bit 2; such a row appends
+ * nothing. */
 FA_API int fa_op_kv8_append(const void* k_dev, const void* v_dev, int src_type, int64_t row_stride, int M,
                             int n_layers, int n_kv_heads, const int* pos_dev, const int* slot_dev,
                             const int* block_table_dev, int bt_stride, int n_pages, int format, void* pool_dev,
                             int* err_dev, void* stream);
 /* Kernel (1) with an 8-bit end: fa_op_qknorm_rope_append with qkv [M][n_heads + 2 n_kv_heads][128],
- * q_out [M][n_heads][128] (the same bits), K (normed and rotated) and V quantised from f32. */
+ * q_out [M][n_heads][128] in the same f32 arithmetic. K's stored bytes are those of the norm
+ * and rotation in 64 bits, rounded once (its int8 scale is within 2^-20 of theirs); V is
+ * quantised as it is. qkv, rope and q_out 16-byte, the norm weights 8-byte aligned. Errors as
+ * for the raw append; a position past the rotation table sets bit 4 too. */
 FA_API int fa_op_qknorm_rope_append_kv8(const float* qkv_dev, int M, int n_heads, int n_kv_heads, const int* pos_dev,
                                         const int* slot_dev, const int* block_table_dev, int bt_stride, int n_pages,
                                         const float* q_norm_dev, const float* k_norm_dev, float eps,
@@ -437,8 +441,8 @@ FA_API int fa_op_kv8_gather(const void* pool_dev, int format, int n_layers, int 
  * the rows' lengths. scratch_dev: fa_op_attention_kv8_scratch_bytes(...) bytes, 16-byte
  * aligned, of any content; calls that overlap on the GPU (captured graphs that run at the same
  * time among them) need scratch of their own. A position below -1 or past the block-table row
- * sets error bit 8 and that row is not written; a page outside the pool sets bit 2 and its
- * tokens are left out. */
+ * or a negative slot sets error bit 8 and that row is not written; a page outside the pool sets
+ * bit 2 and its tokens are left out. bt_stride is limited to 2^26 pages. */
 FA_API size_t fa_op_attention_kv8_scratch_bytes(int M, int n_heads, int n_kv_heads);
 FA_API int fa_op_paged_attention_kv8(const float* q_dev, int M, int n_heads, int n_kv_heads, const int* pos_dev,
                                      const int* slot_dev, const int* block_table_dev, int bt_stride, int n_pages,
@@ -448,7 +452,9 @@ FA_API int fa_op_paged_attention_kv8(const float* q_dev, int M, int n_heads, int
 /* Causal attention of prefill tiles (fa_op_prefill_attention's 8-bit form). tiles_dev holds
  * n_tiles pairs (first row, rows): up to 128 * n_kv_heads / n_heads (rounded down) consecutive
  * rows of one sequence with non-decreasing positions; each row attends to tokens [0, pos[m]].
- * A bad tile sets error bit 4 and writes nothing; rows, pages and scratch as above. */
+ * A bad tile sets error bit 4 and writes nothing; a row of another slot than the rest of its
+ * tile (than the row that attends furthest) sets bit 8 and is not written; rows, pages and
+ * scratch otherwise as above. */
 FA_API size_t fa_op_prefill_attention_kv8_scratch_bytes(int n_tiles, int n_heads, int n_kv_heads);
 FA_API int fa_op_prefill_attention_kv8(const float* q_dev, int M, int n_heads, int n_kv_heads, const int* pos_dev,
                                        const int* slot_dev, const int* block_table_dev, int bt_stride, int n_pages,

@@ -104,6 +104,15 @@ def norm_rotate(x, w, rot, eps=np.float32(1e-5)):
     return np.concatenate([a * c - b * s, a * s + b * c], -1).astype(np.float32)
 
 
+def norm_rotate_exact(x, w, rot, eps=np.float32(1e-5)):
+    """norm_rotate in 64 bits (x, w, rot and eps are f32 values)."""
+    x = x.astype(np.float64)
+    y = x / np.sqrt((x * x).mean(-1, keepdims=True) + np.float64(eps)) * w.astype(np.float64)
+    a, b = y[..., :64], y[..., 64:]
+    c, s = rot[:, None, :, 0].astype(np.float64), rot[:, None, :, 1].astype(np.float64)
+    return np.concatenate([a * c - b * s, a * s + b * c], -1)
+
+
 def attention(q, k, v):
     """q [Hq][128], k and v [Hkv][n][128]: softmax(q k) v in 64 bits, [Hq][128]."""
     q = np.asarray(q, np.float64)

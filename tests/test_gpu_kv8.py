@@ -210,11 +210,44 @@ def test_qknorm_rope_append_matches_definition(torch_cuda, fmt, hq, hkv, M):
     rot = rope[np.maximum(pos, 0)]
     q = P.norm_rotate(qkv[:, :hq], qn, rot) * np.float32(1 / np.sqrt(np.float32(128)))
     q[~live] = 7
-    k = P.norm_rotate(qkv[:, hq:hq + hkv], kn, rot)
+    k = P.norm_rotate_exact(qkv[:, hq:hq + hkv], kn, rot)
     P.write(pool, bt, np.zeros(M, np.int32), pos, k[:, None], qkv[:, hq + hkv:][:, None], fmt)
     assert np.array_equal(q_out.cpu().numpy(), q)
-    assert np.array_equal(d_pool.cpu().numpy(), pool)
+    got = d_pool.cpu().numpy()
+    (raw, d), (raw_w, d_w) = P.parts(got), P.parts(pool)
+    # K's bytes are those of 64 bits; its int8 scale comes from the f32 maximum, which is off by
+    # 2^-20 at most (an e4m3 scale is a power of two); V is exact
+    assert np.array_equal(raw, raw_w)
+    assert np.array_equal(d[..., 1, :].view(np.uint32), d_w[..., 1, :].view(np.uint32))
+    live_d = np.isfinite(d_w[..., 0, :])
+    assert np.array_equal(live_d, np.isfinite(d[..., 0, :]))
+    off = np.abs(d[..., 0, :][live_d].astype(np.float64) - d_w[..., 0, :][live_d])
+    assert (off <= np.abs(d_w[..., 0, :][live_d]) * (2.0 ** -20 if fmt == P.INT8 else 0)).all()
     assert int(d_err) == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_qknorm_rope_append_keys_next_to_borders(torch_cuda, fmt):
+    """A hundred thousand key vectors: every byte that of the 64-bit value rounded once, those
+    within the f32 error of a border among them."""
+    torch = torch_cuda
+    rng = np.random.default_rng(23)
+    hq, hkv, M, max_pos = 1, 40, 2500, 2512
+    qkv = _vectors(rng, M, hq + 2 * hkv)
+    w = np.ones(128, np.float32)
+    rope = np.asarray(oracle.rope_table(max_pos), np.float32).reshape(max_pos, 64, 2)
+    pos, n_pages = np.arange(M, dtype=np.int32), max_pos // 16
+    bt = rng.permutation(n_pages).astype(np.int32)[None]
+    pool, err = torch.zeros((1, n_pages, hkv, P.TILE), dtype=torch.uint8, device="cuda"), _err(torch)
+    q = torch.zeros((M, hq, 128), device="cuda")
+    d = [dev(torch, a) for a in (qkv, pos, np.zeros(M, np.int32), bt, w, rope)]
+    p = [x.data_ptr() for x in d]
+    fa_dec.op_qknorm_rope_append_kv8(p[0], M, hq, hkv, p[1], p[2], p[3], n_pages, n_pages, p[4], p[4], 1e-5, p[5],
+                                     max_pos, fmt, pool.data_ptr(), q.data_ptr(), err.data_ptr(), _stream(torch))
+    raw, _ = P.parts(pool.cpu().numpy())
+    got = raw[0, bt[0, pos // 16], :, 0, pos % 16]
+    want, _ = P.quantise(P.norm_rotate_exact(qkv[:, hq:hq + hkv], w, rope[:M]), fmt)
+    assert np.array_equal(got, want) and int(err) == 0
 
 
 def test_qknorm_rope_append_q_equals_the_f16_pools_op(torch_cuda):
