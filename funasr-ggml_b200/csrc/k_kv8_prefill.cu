@@ -62,6 +62,7 @@ struct PfSmem {
     float raw_scales[RAW][PAGES][2 * kPageTokens];
     float dk[TILES][KB];                      // K scales
     float dv[TILES][KB];                      // V scales / sigma
+    float dv_raw[TILES][KB];                  // V scales
     float sigma[TILES];
     float qs[128];                            // what takes dk S of a query vector to log2 units
     float state[2][3][128];                   // even / odd blocks' maximum, sum and sigma of each vector
@@ -156,6 +157,12 @@ __device__ __forceinline__ uint2 lds64(const void* p) {
 // A barrier of warps 8-15.
 __device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
+// The exponent field of x, 0 for an infinity or NaN.
+__device__ __forceinline__ uint32_t finite_exponent(float x) {
+    const uint32_t e = __float_as_uint(x) & 0x7f800000u;
+    return e == 0x7f800000u ? 0u : e;
+}
+
 // The key blocks [first, last) of part `part` of an item of nb blocks cut into at most
 // max_parts, and the number of parts.
 __device__ __forceinline__ int part_blocks(int nb, int max_parts, int part, int& first, int& last) {
@@ -190,6 +197,47 @@ __device__ __forceinline__ bool tile_bad(const Kv8AttnArgs& a, int2 tile) {
 // units, sum) [items][parts][128]; item = tile * Hkv + KV head.
 __host__ __device__ inline size_t part_index(const Kv8AttnArgs& a, int tile, int h, int parts, int part) {
     return (((size_t)tile * a.Hkv + h) * parts + part) * 128;
+}
+
+// The second pass over a block's scores (dk S in sv): p = exp2(dk S qs - top2), whose sum is
+// returned, and the weights p f (f: V scales over sigma, times `more` where MASKED) as f16 pairs
+// to TMEM over S. Keys not in `seen` weigh nothing: by selection, since the maximum may be -inf
+// and a scale NaN.
+template <bool MASKED>
+__device__ __forceinline__ float2 weights(const uint32_t (&sv)[KB], const float* factors, float more,
+                                          const uint32_t (&seen)[2], float qs, float top2, uint32_t ts) {
+    const float4* dv = reinterpret_cast<const float4*>(factors);
+    const float2 qs2 = make_float2(qs, qs), neg = make_float2(-top2, -top2), minus = make_float2(-1.0f, -1.0f);
+    float2 psum = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+            float4 f = dv[8 * half + (c >> 2)];
+            if (MASKED) f = make_float4(f.x * more, f.y * more, f.z * more, f.w * more);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const int i = 32 * half + c + e;
+                const float2 x = attn::ffma2(make_float2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), qs2, neg);
+                float2 p = make_float2(ex2(x.x), ex2(x.y));
+                float2 w = attn::fmul2(p, e ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
+                if (MASKED) {
+                    const uint32_t in = seen[half] >> (c + e);
+                    p = make_float2(in & 1 ? p.x : 0.0f, in & 2 ? p.y : 0.0f);
+                    w = make_float2(in & 1 ? w.x : 0.0f, in & 2 ? w.y : 0.0f);
+                }
+                psum = add2(psum, p);
+                const uint32_t hw = pack2(w.x, w.y);
+                const float2 rest = attn::ffma2(h2_to_f2(hw), minus, w);
+                hi[(c + e) >> 1] = hw;
+                lo[(c + e) >> 1] = pack2(rest.x, rest.y);
+            }
+        }
+        TMEM_ST_X16(ts + 16 * half, hi);
+        TMEM_ST_X16(ts + 32 + 16 * half, lo);
+    }
+    return psum;
 }
 
 template <int FMT>
@@ -395,8 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const int t = lane + 32 * e;
                 const bool in = ((have >> (t >> 4)) & 1) && key0 + t <= pos_last;
                 dv[e] = in ? S.raw_scales[s][t >> 4][kPageTokens + (t & 15)] : 0.0f;
-                const uint32_t x = __float_as_uint(dv[e]) & 0x7f800000u;
-                top = max(top, x == 0x7f800000u ? 0u : x);
+                top = max(top, finite_exponent(dv[e]));
             }
             top = max(__reduce_max_sync(0xffffffffu, top), 11u << 23);
             run = max(run, top);
@@ -407,6 +454,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const int t = lane + 32 * e;
                     S.dk[d][t] = S.raw_scales[s][t >> 4][t & 15];
                     S.dv[d][t] = dv[e] * inv;
+                    S.dv_raw[d][t] = dv[e];
                 }
                 if (lane == 0) {
                     S.sigma[d] = sigma;
@@ -519,7 +567,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int j0 = 0; j0 == 0 || j0 < n_blocks; j0 += STRETCH) {
         const int j1 = min(j0 + STRETCH, n_blocks);
         // running maximum of dk S (before qs), the same in log2 units, and the sum of weights
-        float top = -INFINITY, top2 = -INFINITY, sum = 0.0f, sigma = 1.0f;
+        float top = -INFINITY, top2 = -INFINITY, sum = 0.0f, sigma = 0.0f;
         for (int j = j0 + odd; ok && j < j1; j += 2) {
             const int d = j % TILES;
             const bool got = mbar_wait_bounded(&S.kv_full[d], (uint32_t)(j / TILES) & 1u) &&
@@ -561,7 +609,23 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
 #pragma unroll
             for (int c = 0; c < KB; ++c) bmax = fmaxf(bmax, __uint_as_float(sv[c]));
-            const float next_sigma = S.sigma[d];
+            // a sigma of the row's own where it does not see every key: a large V that it may not see must
+            // not scale its weights away
+            float next_sigma = S.sigma[d];
+            if (masked) {
+                const float4* raw = reinterpret_cast<const float4*>(S.dv_raw[d]);
+                uint32_t own = 11u << 23;
+#pragma unroll
+                for (int c = 0; c < KB; c += 4) {
+                    const float4 f = raw[c >> 2];
+                    const uint32_t in = seen[c >> 5] >> (c & 31);
+                    if (in & 1) own = max(own, finite_exponent(f.x));
+                    if (in & 2) own = max(own, finite_exponent(f.y));
+                    if (in & 4) own = max(own, finite_exponent(f.z));
+                    if (in & 8) own = max(own, finite_exponent(f.w));
+                }
+                next_sigma = fmaxf(sigma, __uint_as_float(own - (kSigmaShift << 23)));
+            }
             float alpha = j - j0 > 1 ? sigma * pow2_inverse(next_sigma) : 1.0f;
             sigma = next_sigma;
             if (top == -INFINITY) {
@@ -589,36 +653,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     TMEM_ST_X16(to + c, ov);
                 }
             }
-            const float4* dv = reinterpret_cast<const float4*>(S.dv[d]);
-            const float2 qs2 = make_float2(qs, qs), neg = make_float2(-top2, -top2), minus = make_float2(-1.0f, -1.0f);
-            float2 psum = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int c = 0; c < 32; c += 4) {
-                    const float4 f = dv[8 * half + (c >> 2)];
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const int i = 32 * half + c + e;
-                        const float2 x = attn::ffma2(make_float2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), qs2, neg);
-                        float2 p = make_float2(ex2(x.x), ex2(x.y));
-                        float2 w = attn::fmul2(p, e ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
-                        if (masked) {                  // by selection: the maximum may be -inf, a scale NaN
-                            const uint32_t in = seen[half] >> (c + e);
-                            p = make_float2(in & 1 ? p.x : 0.0f, in & 2 ? p.y : 0.0f);
-                            w = make_float2(in & 1 ? w.x : 0.0f, in & 2 ? w.y : 0.0f);
-                        }
-                        psum = add2(psum, p);
-                        const uint32_t hw = pack2(w.x, w.y);
-                        const float2 rest = attn::ffma2(h2_to_f2(hw), minus, w);
-                        hi[(c + e) >> 1] = hw;
-                        lo[(c + e) >> 1] = pack2(rest.x, rest.y);
-                    }
-                }
-                TMEM_ST_X16(ts + 16 * half, hi);
-                TMEM_ST_X16(ts + 32 + 16 * half, lo);
-            }
+            const float2 psum = masked ? weights<true>(sv, S.dv_raw[d], pow2_inverse(sigma), seen, qs, top2, ts)
+                                       : weights<false>(sv, S.dv[d], 1.0f, seen, qs, top2, ts);
             sum += psum.x + psum.y;
             tmem_wait_st();
             tc_fence_before();

@@ -538,6 +538,32 @@ def test_nan_vectors_reach_their_own_rows_only(torch_cuda, fmt, which):
     assert np.array_equal(nan, want)
 
 
+@pytest.mark.parametrize("base,M", [(0, 70), (37, 64), (500, 100), (1000, 20)])
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_large_later_values_leave_earlier_rows(torch_cuda, fmt, which, base, M):
+    """K and V of 1e30 in the second half of a chunk: a row before them is as accurate, in terms
+    of what it attends to, as without them."""
+    torch = torch_cuda
+    rng = np.random.default_rng(base + M)
+    hq, hkv, n = 16, 8, base + M
+    pool, bt, n_pages = _filled(rng, [n], 1, hkv, fmt)
+    _, scales = P.parts(pool)
+    late = np.arange(base + M // 2, n)
+    for part in (0, 1):
+        scales[0, bt[0, late // 16], :, part, late % 16] *= np.float32(1e30)
+    pos = np.arange(base, n).astype(np.int32)
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    args = (torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, np.zeros(M, np.int32)), dev(torch, bt), n_pages,
+            fmt, dev(torch, pool))
+    err = _err(torch)
+    got = (_decode(*args, err) if which == "decode" else _prefill(*args, _tiles([(0, M)], 64), err)).cpu().numpy()
+    assert int(err) == 0
+    for m in range(M // 2):
+        k, v = (x[0] for x in P.read(pool, bt[0], 0, pos[m] + 1, fmt))
+        assert np.abs(got[m] - P.attention(q[m], k, v).reshape(-1)).max() <= _bound(q[m], k, v), m
+
+
 @pytest.mark.parametrize("bad", ["pos", "past_table", "slot", "page", "page_negative"])
 def test_decode_attention_flags_bad_rows(torch_cuda, bad):
     torch = torch_cuda
