@@ -113,7 +113,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8AppendArgs a, unsign
         uint32_t two[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t keep = (c & 8) ? amax[(i + 2) % P] : amax[i % P], send = (c & 8) ? amax[i % P] : amax[(i + 2) % P];
+            const uint32_t keep = (c & 8) ? amax[(i + 2) % P] : amax[i % P];
+            const uint32_t send = (c & 8) ? amax[i % P] : amax[(i + 2) % P];
             two[i] = max(keep, __shfl_xor_sync(0xffffffffu, send, 8));
         }
         const uint32_t keep = (c & 4) ? two[1] : two[0], send = (c & 4) ? two[0] : two[1];
@@ -145,8 +146,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8AppendArgs a, unsign
     }
 }
 
-// Warps of a CTA: 4096 rows of 32 head vectors take 27.4 us with 8, 22.7 with 4, 22.2 with 2 and
-// 22.9 with 1 (a CTA's registers are free again only when its slowest warp ends).
+// Warps of a CTA: 4096 rows of 32 head vectors took 27.4 us with 8, 22.7 with 4, 22.2 with 2 and
+// 22.9 with 1, before keys were rounded exactly (a CTA's registers are free again only when its slowest warp ends).
 constexpr int kQkvWarps = 2;
 
 struct Kv8QkvArgs {
@@ -178,10 +179,11 @@ __device__ __forceinline__ void load4(const float* vec, int lane, float (&x)[4])
 // K is stored as if it had been computed in 64 bits and rounded once. Its f32 values are off by
 // less than 11 x 2^-24 of the vector's largest (the norm's scale by 3.5 roundings, two products
 // and a rotation by 4, whose terms together reach sqrt(2) of it), so their bytes can differ from
-// those of the exact values only next to a border: where one lies within that distance (and for
-// int8 what an ulp of the scale moves it by), the vector is computed again in 64 bits, a few
-// vectors in a hundred.
-constexpr float kKeyError = 12.5f / (1 << 24);
+// those of the exact values only next to a border: where one lies within that distance (for int8
+// twice that and an ulp, since the scale is off by as much), the vector is computed again in 64
+// bits, a few vectors in a hundred.
+template <int FMT>
+constexpr float kKeyError = (FMT == kInt8 ? 23.5f : 12.5f) / (1 << 24);
 
 // pack4 of key values, unless a value that differs by e may round otherwise (near).
 template <int FMT>
@@ -248,7 +250,8 @@ __device__ __noinline__ uint32_t exact_key(const float* vec, int lane, const flo
 // sums of squares are reduced over the warp together: each exchange halves the vectors a lane
 // carries, and the norms' square root and division, and the scales and reciprocals, are computed
 // once, side by side.
-// Bound: issue and HBM. 4096 rows of 32 vectors (111 MB) take 22.2 us, 5.0 TB/s.
+// Bound: issue (2.7 instructions a cycle) and HBM. 4096 rows of 32 vectors (111 MB) take 26.2 us,
+// 4.25 TB/s; 22.2 with keys rounded from their f32 values.
 template <int FMT, int V>
 __global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
     static_assert(V == 1 || V == 4, "the exchanges below");
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
     }
     if (page < 0) return;
     const float d_mine = scale_of<FMT>(top), inv_mine = __frcp_rn(d_mine);
-    const float amax_mine = __uint_as_float(top), e_mine = amax_mine * kKeyError;
+    const float amax_mine = __uint_as_float(top), e_mine = amax_mine * kKeyError<FMT>;
     // e4m3 scales that the error of the largest value may change
     const uint32_t unsure =
         FMT == kInt8 ? 0u
@@ -395,8 +398,8 @@ __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const fl
 }
 
 // Gather: one CTA per page of one sequence in one layer; a thread 8 values of one token,
-// over the heads' K and V parts, kGatherVecs loads under way at a time. The value d * q is formed in f32 and rounded once to the
-// output type.
+// over the heads' K and V parts, kGatherVecs loads under way at a time. The value d * q is formed
+// in f32 and rounded once to the output type.
 constexpr int kGatherVecs = 16;                // 8: 1.5 % slower on 32 streams of up to 320 tokens in 28 layers
 
 template <int FMT, typename T>
@@ -517,9 +520,10 @@ extern "C" FA_API int fa_op_kv8_append(const void* k, const void* v, int src_typ
     if (misaligned(k, 16) || misaligned(v, 16) || misaligned(pool, 128))
         return report_op_error(FA_ERR_INVALID_ARG, "fa_op_kv8_append: k and v must be 16-byte, pool 128-byte aligned");
     const long long pairs = (long long)n_layers * n_kv_heads;
+    if (pairs > 0x7fffffffll) return report_op_error(FA_ERR_CAPACITY, "fa_op_kv8_append: too many vectors for one call");
     const bool four = several_per_warp(M * pairs);
     const long long per_row = four ? (pairs + 31) / 32 : (pairs + 7) / 8;
-    if (pairs > 0x7fffffffll || M * per_row > 0x7fffffffll)
+    if (M * per_row > 0x7fffffffll)
         return report_op_error(FA_ERR_CAPACITY, "fa_op_kv8_append: too many vectors for one call");
     Kv8AppendArgs a{k, v, row_stride, M, n_layers, n_kv_heads, pos, slot, bt, bt_stride, n_pages,
                     static_cast<unsigned char*>(pool), err};
@@ -539,11 +543,11 @@ extern "C" FA_API int fa_op_qknorm_rope_append_kv8(const float* qkv, int M, int 
         return report_op_error(FA_ERR_INVALID_ARG, "fa_op_qknorm_rope_append_kv8: null or non-positive argument");
     if (!known_format(format))
         return report_op_error(FA_ERR_INVALID_ARG, "fa_op_qknorm_rope_append_kv8: unknown format");
-    if (misaligned(qkv, 16) || misaligned(q_out, 16) || misaligned(rope, 16) || misaligned(qn, 8) || misaligned(kn, 8) ||
-        misaligned(pool_layer, 128))
+    if (misaligned(qkv, 16) || misaligned(q_out, 16) || misaligned(rope, 16) || misaligned(qn, 8) ||
+        misaligned(kn, 8) || misaligned(pool_layer, 128))
         return report_op_error(FA_ERR_INVALID_ARG,
-                               "fa_op_qknorm_rope_append_kv8: qkv, rope and q_out must be 16-byte, the norm weights 8-byte, the pool "
-                               "128-byte aligned");
+                               "fa_op_qknorm_rope_append_kv8: qkv, rope and q_out must be 16-byte, the norm "
+                               "weights 8-byte, the pool 128-byte aligned");
     if ((long long)n_heads + 2ll * n_kv_heads > 65535)
         return report_op_error(FA_ERR_CAPACITY, "fa_op_qknorm_rope_append_kv8: too many heads");
     Kv8QkvArgs a{qkv, M, n_heads, n_kv_heads, pos, slot, bt, bt_stride, n_pages, qn, kn, eps,
