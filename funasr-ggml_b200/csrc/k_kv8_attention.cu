@@ -71,10 +71,17 @@ namespace {
 //                                       that takes the page's largest dv to [2^10, 2^11)
 // The page's product starts from zero and is added to the running output by one f32 fma per
 // value, so the sum over pages is rounded to nearest.
+//
+// Bound: HBM. 128 rows of 2048 tokens (16 heads on 8, 554 MB of tiles) take 95-98 us: 84 us of
+// pages at the rate of a copy, then some 5 us each of start (lengths, split, page look-ups: four
+// dependent loads) and of merge; without its arithmetic the kernel takes as long. Short calls are
+// those two chains: one row of 256 tokens 8.2 us, 16 rows of 1 to 1021 tokens 11.3 us. 12 or 6
+// warps a CTA took 98.6 and 98.9 us; two to four CTAs' worth of grid a slot 102 to 109; the
+// merge inside the kernel (arrival words) 101, and 10.3 for the one row.
 constexpr int kWarps = 4;
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 148 * kCtasPerSm;     // one resident wave of a B200
-constexpr int kItemUnits = 2;
+constexpr int kItemUnits = 2;                  // with ranges per warp: 16 ragged rows 25.6 -> 12.8 us
 
 constexpr int kStages = 3;                     // 128 rows x 2048 tokens: 2 stages 97, 3 95, 4 98 us
 template <int NT>
@@ -435,8 +442,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
 #pragma unroll
             for (int c = 0; c < NT; ++c) {
                 const int from = 8 * t + (g >> 1);
-                const uint32_t x0 = __shfl_sync(0xffffffffu, w0[c], from), y0 = __shfl_sync(0xffffffffu, w0[c], from + 4);
-                const uint32_t x1 = __shfl_sync(0xffffffffu, w1[c], from), y1 = __shfl_sync(0xffffffffu, w1[c], from + 4);
+                const uint32_t x0 = __shfl_sync(0xffffffffu, w0[c], from);
+                const uint32_t y0 = __shfl_sync(0xffffffffu, w0[c], from + 4);
+                const uint32_t x1 = __shfl_sync(0xffffffffu, w1[c], from);
+                const uint32_t y1 = __shfl_sync(0xffffffffu, w1[c], from + 4);
                 wb[c][0] = __byte_perm(x0, y0, sel);
                 wb[c][1] = __byte_perm(x1, y1, sel);
             }
@@ -751,9 +760,11 @@ extern "C" FA_API int fa_op_paged_attention_kv8(const float* q, int M, int n_hea
     const bool wide = n_heads / n_kv_heads > 4;
     const cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e;
-    if (format == FA_KV8_INT8) e = wide ? launch_decode<kInt8, 2>(tm, a, scratch, grid, st) : launch_decode<kInt8, 1>(tm, a, scratch, grid, st);
-    else e = wide ? launch_decode<kE4m3, 2>(tm, a, scratch, grid, st) : launch_decode<kE4m3, 1>(tm, a, scratch, grid, st);
-    if (e != cudaSuccess) cudaGetLastError();
-    return e == cudaSuccess ? FA_OK
-                            : report_op_error(FA_ERR_CUDA, (std::string("fa_op_paged_attention_kv8: ") + cudaGetErrorString(e)).c_str());
+    if (format == FA_KV8_INT8)
+        e = wide ? launch_decode<kInt8, 2>(tm, a, scratch, grid, st) : launch_decode<kInt8, 1>(tm, a, scratch, grid, st);
+    else
+        e = wide ? launch_decode<kE4m3, 2>(tm, a, scratch, grid, st) : launch_decode<kE4m3, 1>(tm, a, scratch, grid, st);
+    if (e == cudaSuccess) return FA_OK;
+    cudaGetLastError();
+    return report_op_error(FA_ERR_CUDA, (std::string("fa_op_paged_attention_kv8: ") + cudaGetErrorString(e)).c_str());
 }

@@ -5,15 +5,18 @@
 // KV head and, where a call has few tiles, a part of the tile's keys: its up to 128 query
 // vectors (vector v = row v % R, head v / R) are the M side of every MMA, so a page is read and
 // expanded to f16 once for all of them. Per block of 64 keys (4 pages):
-//   S  = Q . K^T        tcgen05.mma kind::f16, M 128, N 64, K 128; Q in TMEM as the pair
-//                       hi = f16(q'), lo = f16(q' - hi), q' = q scaled by a power of two to [1, 2)
-//   p  = exp2(dk S - m) one query vector per thread; w = p dv / sigma, sigma a power of two at
-//                       the largest dv so far (times 2^-6): f16 pairs, written over S in TMEM
+//   S  = Q . K^T        tcgen05.mma kind::f16, M 128, N 64, K 128; Q as the pair hi = f16(q'),
+//                       lo = f16(q' - hi), q' = q scaled by a power of two to [1, 2): 22 bits
+//   p  = exp2(dk S - m) one query vector per thread; w = p dv / sigma, sigma a power of two under
+//                       the largest dv that the row has seen: f16 pairs, written over S in TMEM
 //   O += w . V          M 128, N 128 (dims), K 64 (keys), V MN-major
-// Both A operands are in TMEM because shared memory would otherwise bound the kernel: a block
-// reads 128 KB of it for the MMAs with Q and w there, 64 KB (only K and V) without, against the
-// 1024 cycles that its MMAs take.
-// The running maximum is lazy (O is rescaled when a block exceeds it by 2^8 or sigma grows).
+// A weight's pair is exact to 2^-25 at the least, so an output is off by up to 2^-24 of the
+// largest |V| that its row attends to (and of nothing that it does not attend to), which is what
+// f32 sums of the values give too unless the largest V has next to no weight.
+// w and Q's high parts, the A operands of three quarters of the MMAs, are in TMEM: with all of Q
+// and w in shared memory a block would read 128 KB of it for its MMAs, against 1024 cycles that
+// they take. The running maximum is lazy: O is rescaled when a block exceeds it by 2^kLazy or
+// sigma grows.
 //
 // Roles (512 threads): warp 0 issues the page copies (one TMA box and one bulk copy of scales
 // per page) into a ring of raw blocks; warps 4-7 expand a raw block into the f16 K / V tiles of
@@ -21,6 +24,14 @@
 // 12-15 load Q, run the softmax of the even and of the odd blocks and write the outputs. Every
 // mbarrier wait is bounded; on a timeout the CTA records the error, drains its copies and MMAs
 // and frees TMEM.
+//
+// Bound: per block of 64 keys and 128 query vectors the MMAs take 1170 cycles (with the pairs'
+// second products twice those of plain f16) and the kernel about 1560: softmax issue and the
+// hand-over between softmax and MMAs are the rest. 4 chunks of 417 to 512 rows at 3500 tokens (16
+// query heads on 8, 248 CTAs of one SM each) take 130 us; 300 with one softmax group, 174 with two
+// S buffers, 142 to 155 with masked and whole blocks in one pass. A chunk of 112 rows takes 14.6 us.
+// A persistent form with an even split of the blocks took 160 and 26: every change of tile costs
+// 10 us of queries, joins and output, which separate CTAs overlap.
 #include "k_attn_body.cuh"
 #include "k_kv8_attn.cuh"
 
@@ -40,8 +51,8 @@ constexpr int THREADS = 512;
 constexpr int kRegsIssue = 56, kRegsExpand = 72, kRegsSoftmax = 192;
 static_assert(kRegsIssue + kRegsExpand + 2 * kRegsSoftmax <= 4 * 128, "registers of the launch");
 // Blocks summed in TMEM at a time. The tensor core's f32 sums are truncated, so their error grows
-// with their length (2.4e-6 of the output over 60 blocks); stretches are joined in f32 arithmetic
-// rounded to nearest.
+// with their length (2.4e-6 of the output over 60 blocks, 1.6e-6 with stretches); stretches are
+// joined in f32 arithmetic rounded to nearest, which costs 6 % over one sum.
 constexpr int STRETCH = 32;
 constexpr int kMaxParts = 16;                 // key ranges of one tile and head
 constexpr int kMinPartBlocks = 8;
@@ -61,9 +72,9 @@ struct PfSmem {
     unsigned char raw[RAW][PAGES][2 * kPartBytes];
     float raw_scales[RAW][PAGES][2 * kPageTokens];
     float dk[TILES][KB];                      // K scales
-    float dv[TILES][KB];                      // V scales / sigma
-    float dv_raw[TILES][KB];                  // V scales
-    float sigma[TILES];
+    float dv[TILES][KB];                      // V scales / sigma, for rows that see the whole block
+    float dv_raw[TILES][KB];                  // V scales, for the others
+    float sigma[TILES];                       // of all keys up to the block's last
     float qs[128];                            // what takes dk S of a query vector to log2 units
     float state[2][3][128];                   // even / odd blocks' maximum, sum and sigma of each vector
     int raw_pages[RAW];                       // bit q: page q of the block was copied
@@ -315,106 +326,106 @@ __global__ void __launch_bounds__(THREADS, 1)
     // spare: 128 threads each of kRegsIssue + kRegsExpand + 2 kRegsSoftmax = 4 x 128
     const bool idle = bad || (int)blockIdx.z >= parts;  // nothing issued: on to the TMEM release
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
-    if (idle) {
-    } else if (warp == 0) {
-        const int* bt = a.block_table + (size_t)slot * a.bt_stride;
-        const int last_page = pos_last / kPageTokens;
-        bool ok = true;
-        int ids = 0;                                   // lane l: page 32 b + l of the part
-        for (int j = 0; ok && j < n_blocks; ++j) {
-            if ((j & 7) == 0) {
-                const int p = (first + j) * PAGES + lane;
-                ids = p <= last_page ? bt[p] : -1;
-                if (p <= last_page && (ids < 0 || ids >= a.n_pages)) {
-                    ids = -1;                          // its tokens are left out
-                    record_error(a.err, kDevErrBadPage);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        if (idle) {
+        } else if (warp == 0) {
+            const int* bt = a.block_table + (size_t)slot * a.bt_stride;
+            const int last_page = pos_last / kPageTokens;
+            bool ok = true;
+            int ids = 0;                                   // lane l: page 32 b + l of the part
+            for (int j = 0; ok && j < n_blocks; ++j) {
+                if ((j & 7) == 0) {
+                    const int p = (first + j) * PAGES + lane;
+                    ids = p <= last_page ? bt[p] : -1;
+                    if (p <= last_page && (ids < 0 || ids >= a.n_pages)) {
+                        ids = -1;                          // its tokens are left out
+                        record_error(a.err, kDevErrBadPage);
+                    }
                 }
-            }
-            const int s = j % RAW;
-            if (j >= RAW) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.raw_empty[s], (uint32_t)(j / RAW - 1) & 1u));
-            if (!ok) break;
-            int id[PAGES], have = 0;
-#pragma unroll
-            for (int q = 0; q < PAGES; ++q) {
-                id[q] = __shfl_sync(0xffffffffu, ids, (j & 7) * PAGES + q);
-                have |= (id[q] >= 0) << q;
-            }
-            if (lane == 0) {
-                S.raw_pages[s] = have;
-                mbar_arrive_expect_tx(&S.raw_full[s], __popc(have) * kTileBytes);
+                const int s = j % RAW;
+                if (j >= RAW) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.raw_empty[s], (uint32_t)(j / RAW - 1) & 1u));
+                if (!ok) break;
+                int id[PAGES], have = 0;
 #pragma unroll
                 for (int q = 0; q < PAGES; ++q) {
-                    if (id[q] < 0) continue;
-                    const int row = (id[q] * a.Hkv + h) * (kTileBytes / 128);
-                    tma_load_2d(S.raw[s][q], &tm_pool, 0, row, &S.raw_full[s]);
-                    bulk_copy_g2s(S.raw_scales[s][q], a.pool + (size_t)row * 128 + kScaleOff,
-                                  2 * kPageTokens * sizeof(float), &S.raw_full[s]);
+                    id[q] = __shfl_sync(0xffffffffu, ids, (j & 7) * PAGES + q);
+                    have |= (id[q] >= 0) << q;
                 }
-                S.issued = j + 1;
+                if (lane == 0) {
+                    S.raw_pages[s] = have;
+                    mbar_arrive_expect_tx(&S.raw_full[s], __popc(have) * kTileBytes);
+#pragma unroll
+                    for (int q = 0; q < PAGES; ++q) {
+                        if (id[q] < 0) continue;
+                        const int row = (id[q] * a.Hkv + h) * (kTileBytes / 128);
+                        tma_load_2d(S.raw[s][q], &tm_pool, 0, row, &S.raw_full[s]);
+                        bulk_copy_g2s(S.raw_scales[s][q], a.pool + (size_t)row * 128 + kScaleOff,
+                                      2 * kPageTokens * sizeof(float), &S.raw_full[s]);
+                    }
+                    S.issued = j + 1;
+                }
+                __syncwarp();
+            }
+            if (!ok && lane == 0) S.err = 1;
+        } else if (warp == 1) {
+            if (n_blocks > 0) {
+                // The whole warp runs the loop and one lane issues: the operands of an MMA then stay in
+                // uniform registers (issued from a divergent branch, moving them there took longer than
+                // the MMAs: 2070 cycles a block).
+                constexpr uint32_t kIdS = idesc_f16(128, KB, false, false);
+                constexpr uint32_t kIdPV = idesc_f16(128, D, false, true);
+                const uint32_t one = elect_one();
+                const uint64_t k_desc = smem_desc_k128(S.k[0][0]), v_desc = smem_desc_mn128(S.v[0][0], KB * 64 * 2);
+                const uint64_t q_desc = smem_desc_k128(S.q_lo[0]);
+                bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.q_ready, 0));
+                // S of block j + 2 before O of block j: with three S buffers it needs only block j - 1's
+                // product, so a group finds its next S ready when it ends a block
+                for (int i = 0; ok && i < n_blocks + 2; ++i) {
+                    if (i < n_blocks) {
+                        const int s = i % TILES;
+                        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.kv_full[s], (uint32_t)(i / TILES) & 1u));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t d_s = tmem + (uint32_t)(i % SBUF * KB);
+                        const uint64_t db = k_desc + (uint32_t)(s * (int)sizeof(S.k[0]) >> 4);
+                        // the low parts first: the sums are cut off at the size of the low products then, and
+                        // only the eight steps of the high parts at that of a score
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk) {
+                            const uint64_t in_tile = (kk >> 2) * (int)sizeof(S.k[0][0]) / 16 + (kk & 3) * 32 / 16;
+                            const uint64_t in_q = (kk >> 2) * (int)sizeof(S.q_lo[0]) / 16 + (kk & 3) * 32 / 16;
+                            tc_mma_f16_if(one, d_s, q_desc + in_q, db + in_tile, kIdS, kk > 0 ? 1u : 0u);
+                        }
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk) {
+                            const uint64_t in_tile = (kk >> 2) * (int)sizeof(S.k[0][0]) / 16 + (kk & 3) * 32 / 16;
+                            tc_mma_f16_ts_if(one, d_s, tmem + COL_Q + 8 * kk, db + in_tile, kIdS, 1u);
+                        }
+                        tc_commit_if(one, &S.s_full[i % SBUF]);
+                    }
+                    if (i >= 2) {
+                        const int j = i - 2, s = j % TILES;
+                        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.p_ready[j % SBUF], (uint32_t)(j / SBUF) & 1u));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t d_p = tmem + (uint32_t)(j % SBUF * KB), d_o = tmem + COL_O + (uint32_t)((j & 1) * D);
+                        const uint64_t db = v_desc + (uint32_t)(s * (int)sizeof(S.v[0]) >> 4);
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            const uint64_t at = db + kk * 16 * 64 * 2 / 16;
+                            tc_mma_f16_ts_if(one, d_o, d_p + 8 * kk, at, kIdPV, (j % STRETCH > 1 || kk > 0) ? 1u : 0u);
+                            tc_mma_f16_ts_if(one, d_o, d_p + 32 + 8 * kk, at, kIdPV, 1u);
+                        }
+                        tc_commit_if(one, &S.kv_empty[s]);
+                        tc_commit_if(one, &S.o_done[j & 1]);
+                    }
+                }
+                tc_commit_if(one, &S.drain);
+                if (!mbar_wait_bounded(&S.drain, 0)) ok = false;
+                if (!ok && lane == 0) S.err = 1;
             }
             __syncwarp();
         }
-        if (!ok && lane == 0) S.err = 1;
-    } else if (warp == 1) {
-        if (n_blocks > 0) {
-            // The whole warp runs the loop and one lane issues: the operands of an MMA then stay in
-            // uniform registers (issued from a divergent branch, moving them there took longer than
-            // the MMAs: 2070 cycles a block).
-            constexpr uint32_t kIdS = idesc_f16(128, KB, false, false);
-            constexpr uint32_t kIdPV = idesc_f16(128, D, false, true);
-            const uint32_t one = elect_one();
-            const uint64_t k_desc = smem_desc_k128(S.k[0][0]), v_desc = smem_desc_mn128(S.v[0][0], KB * 64 * 2);
-            const uint64_t q_desc = smem_desc_k128(S.q_lo[0]);
-            bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.q_ready, 0));
-            // S of block j + 2 before O of block j: with three S buffers it needs only block j - 1's
-            // product, so a group finds its next S ready when it ends a block
-            for (int i = 0; ok && i < n_blocks + 2; ++i) {
-                if (i < n_blocks) {
-                    const int s = i % TILES;
-                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.kv_full[s], (uint32_t)(i / TILES) & 1u));
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t d_s = tmem + (uint32_t)(i % SBUF * KB);
-                    const uint64_t db = k_desc + (uint32_t)(s * (int)sizeof(S.k[0]) >> 4);
-                    // the low parts first: the sums are rounded at the size of the low products then, and
-                    // only the eight steps of the high parts at that of a score
-#pragma unroll
-                    for (int kk = 0; kk < 8; ++kk) {
-                        const uint64_t in_tile = (kk >> 2) * (int)sizeof(S.k[0][0]) / 16 + (kk & 3) * 32 / 16;
-                        const uint64_t in_q = (kk >> 2) * (int)sizeof(S.q_lo[0]) / 16 + (kk & 3) * 32 / 16;
-                        tc_mma_f16_if(one, d_s, q_desc + in_q, db + in_tile, kIdS, kk > 0 ? 1u : 0u);
-                    }
-#pragma unroll
-                    for (int kk = 0; kk < 8; ++kk) {
-                        const uint64_t in_tile = (kk >> 2) * (int)sizeof(S.k[0][0]) / 16 + (kk & 3) * 32 / 16;
-                        tc_mma_f16_ts_if(one, d_s, tmem + COL_Q + 8 * kk, db + in_tile, kIdS, 1u);
-                    }
-                    tc_commit_if(one, &S.s_full[i % SBUF]);
-                }
-                if (i >= 2) {
-                    const int j = i - 2, s = j % TILES;
-                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.p_ready[j % SBUF], (uint32_t)(j / SBUF) & 1u));
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t d_p = tmem + (uint32_t)(j % SBUF * KB), d_o = tmem + COL_O + (uint32_t)((j & 1) * D);
-                    const uint64_t db = v_desc + (uint32_t)(s * (int)sizeof(S.v[0]) >> 4);
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        const uint64_t at = db + kk * 16 * 64 * 2 / 16;
-                        tc_mma_f16_ts_if(one, d_o, d_p + 8 * kk, at, kIdPV, (j % STRETCH > 1 || kk > 0) ? 1u : 0u);
-                        tc_mma_f16_ts_if(one, d_o, d_p + 32 + 8 * kk, at, kIdPV, 1u);
-                    }
-                    tc_commit_if(one, &S.kv_empty[s]);
-                    tc_commit_if(one, &S.o_done[j & 1]);
-                }
-            }
-            tc_commit_if(one, &S.drain);
-            if (!mbar_wait_bounded(&S.drain, 0)) ok = false;
-            if (!ok && lane == 0) S.err = 1;
-        }
-        __syncwarp();
-    }
     } else if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsExpand));
         // expansion: a thread takes 8 bytes, dims 8 c .., of every eighth token, K and V (one 16-byte
@@ -496,232 +507,235 @@ __global__ void __launch_bounds__(THREADS, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         if (!idle) {
-        // Warps 8-11 the even blocks, 12-15 the odd ones, each with its own running maximum, sum
-        // and O: while one group works on S of a block, the MMAs make the other's. Thread t of a
-        // group owns TMEM lane t = query vector t (a warp may only touch lanes 32 * (warp % 4) ..).
-        const int odd = warp >= 12 ? 1 : 0;
-        const int quarter = warp & 3;
-        const int t = 32 * quarter + lane;
-        const int r = t % R, head = t / R;
-        const int row = tile.x + r;
-        bool live = head < G && r < tile.y;
-        int pos = pos_last;                            // lanes without a row mask no more than the others
-        if (live) {
-            pos = a.pos[row];
-            if (row_bad(a, row) || (pos >= 0 && a.slot[row] != slot)) {
-                if (h == 0 && blockIdx.z == 0 && head == 0 && !odd) record_error(a.err, kDevErrBadLen);
-                live = false;
-                pos = pos_last;
-            }
-        }
-        const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16);
-        const size_t o_at = ((size_t)row * a.Hq + h * G + head) * D;
-        if (n_blocks > 0) {
-            // Q as a pair: low parts to shared memory as they are, high parts by way of the last tile
-            // of the f16 ring, since a lane writes a whole row of TMEM
-            unsigned char* stage = reinterpret_cast<unsigned char*>(S.k[TILES - 1][0]);
-            unsigned char* stage2 = reinterpret_cast<unsigned char*>(S.v[TILES - 1][0]);
-            const int hf = lane >> 4, chunk = (lane & 15) >> 1;
-            const uint32_t sub = (uint32_t)(lane & 1) * 8;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int v = (warp - 8) * 16 + k;
-                const float4 x = qv[k];
-                const float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-                const float p2 = pow2_floor(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))));
-                const float up = pow2_inverse(p2);
-                uint2 hi, lo;
-                split2(x.x * up, x.y * up, hi.x, lo.x);
-                split2(x.z * up, x.w * up, hi.y, lo.y);
-                const uint32_t off = sw128(v, chunk) + sub;
-                *reinterpret_cast<uint2*>((hf ? stage2 : stage) + off) = hi;
-                *reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(S.q_lo[hf]) + off) = lo;
-                if (lane == 0) S.qs[v] = p2 * kLog2e;
-            }
-            group_sync();
-            // each group writes half of the dims
-            uint32_t row_hi[32];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const uint4 x = lds128((odd ? stage2 : stage) + sw128(t, c));
-                row_hi[4 * c] = x.x;
-                row_hi[4 * c + 1] = x.y;
-                row_hi[4 * c + 2] = x.z;
-                row_hi[4 * c + 3] = x.w;
-            }
-            TMEM_ST_X32(tl + COL_Q + 32 * odd, row_hi);
-            tmem_wait_st();
-            fence_proxy_async_smem();
-            tc_fence_before();
-            mbar_arrive(&S.q_ready);
-        }
-        const float qs = n_blocks > 0 ? S.qs[t] : 0.0f;
-        const float lazy = fminf(kLazy / qs, 1e37f), room = fminf(kRoom / qs, 1e37f);
-        const uint32_t to = tl + COL_O + (uint32_t)(odd * D);
-        const size_t at = part_index(a, blockIdx.y, h, max_parts, blockIdx.z) + t;
-        // over the stretches joined so far: maximum, sum, and the group's half of the dims
-        float all_max = -INFINITY, all_sum = 0.0f, acc[64];
-#pragma unroll
-        for (int e = 0; e < 64; ++e) acc[e] = 0.0f;
-        bool ok = true;
-        for (int j0 = 0; j0 == 0 || j0 < n_blocks; j0 += STRETCH) {
-        const int j1 = min(j0 + STRETCH, n_blocks);
-        // running maximum of dk S (before qs), the same in log2 units, and the sum of weights
-        float top = -INFINITY, top2 = -INFINITY, sum = 0.0f, sigma = 0.0f;
-        for (int j = j0 + odd; ok && j < j1; j += 2) {
-            const int d = j % TILES;
-            const bool got = mbar_wait_bounded(&S.kv_full[d], (uint32_t)(j / TILES) & 1u) &&
-                             mbar_wait_bounded(&S.s_full[j % SBUF], (uint32_t)(j / SBUF) & 1u);
-            if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t ts = tl + (uint32_t)(j % SBUF * KB);
-            uint32_t sv[KB];
-            TMEM_LD_X32(ts, sv);
-            TMEM_LD_X32(ts + 32, (sv + 32));
-            tmem_wait_ld();
-            const int key0 = (first + j) * KB;
-            const int have = S.pages[d];
-            const bool masked = !__all_sync(0xffffffffu, key0 + KB - 1 <= pos && have == (1 << PAGES) - 1);
-            const float4* dk = reinterpret_cast<const float4*>(S.dk[d]);
-            float bmax = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < KB; c += 4) {
-                const float4 f = dk[c >> 2];
-                const float2 x = attn::fmul2(make_float2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), make_float2(f.x, f.y));
-                const float2 y = attn::fmul2(make_float2(__uint_as_float(sv[c + 2]), __uint_as_float(sv[c + 3])), make_float2(f.z, f.w));
-                sv[c] = __float_as_uint(x.x);
-                sv[c + 1] = __float_as_uint(x.y);
-                sv[c + 2] = __float_as_uint(y.x);
-                sv[c + 3] = __float_as_uint(y.y);
-            }
-            uint32_t seen[2] = {~0u, ~0u};             // keys of the block that the row attends to
-            if (masked) {
-                const int n = min(max(pos + 1 - key0, 0), KB);
-                uint64_t bits = n == KB ? ~0ull : (1ull << n) - 1;
-#pragma unroll
-                for (int q = 0; q < PAGES; ++q)
-                    if (!((have >> q) & 1)) bits &= ~(0xffffull << (16 * q));
-                seen[0] = (uint32_t)bits;
-                seen[1] = (uint32_t)(bits >> 32);
-#pragma unroll
-                for (int c = 0; c < KB; ++c)
-                    if (!((seen[c >> 5] >> (c & 31)) & 1)) sv[c] = 0xff800000u;        // -inf
-            }
-#pragma unroll
-            for (int c = 0; c < KB; ++c) bmax = fmaxf(bmax, __uint_as_float(sv[c]));
-            // a sigma of the row's own where it does not see every key: a large V that it may not see must
-            // not scale its weights away
-            float next_sigma = S.sigma[d];
-            if (masked) {
-                const float4* raw = reinterpret_cast<const float4*>(S.dv_raw[d]);
-                uint32_t own = 11u << 23;
-#pragma unroll
-                for (int c = 0; c < KB; c += 4) {
-                    const float4 f = raw[c >> 2];
-                    const uint32_t in = seen[c >> 5] >> (c & 31);
-                    if (in & 1) own = max(own, finite_exponent(f.x));
-                    if (in & 2) own = max(own, finite_exponent(f.y));
-                    if (in & 4) own = max(own, finite_exponent(f.z));
-                    if (in & 8) own = max(own, finite_exponent(f.w));
+            // Warps 8-11 the even blocks, 12-15 the odd ones, each with its own running maximum, sum
+            // and O: while one group works on S of a block, the MMAs make the other's. Thread t of a
+            // group owns TMEM lane t = query vector t (a warp may only touch lanes 32 * (warp % 4) ..).
+            const int odd = warp >= 12 ? 1 : 0;
+            const int quarter = warp & 3;
+            const int t = 32 * quarter + lane;
+            const int r = t % R, head = t / R;
+            const int row = tile.x + r;
+            bool live = head < G && r < tile.y;
+            int pos = pos_last;                            // lanes without a row mask no more than the others
+            if (live) {
+                pos = a.pos[row];
+                if (row_bad(a, row) || (pos >= 0 && a.slot[row] != slot)) {
+                    if (h == 0 && blockIdx.z == 0 && head == 0 && !odd) record_error(a.err, kDevErrBadLen);
+                    live = false;
+                    pos = pos_last;
                 }
-                next_sigma = fmaxf(sigma, __uint_as_float(own - (kSigmaShift << 23)));
             }
-            float alpha = j - j0 > 1 ? sigma * pow2_inverse(next_sigma) : 1.0f;
-            sigma = next_sigma;
-            if (top == -INFINITY) {
-                top = bmax + room;                     // first block with a key: O holds nothing of this row
-                top2 = __fmul_rn(top, qs);
-            } else if (bmax > top + lazy) {
-                top = bmax + room;
-                const float next = __fmul_rn(top, qs);
-                const float f = exp2f(top2 - next);
-                top2 = next;
-                alpha *= f;
-                sum *= f;
+            const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16);
+            const size_t o_at = ((size_t)row * a.Hq + h * G + head) * D;
+            if (n_blocks > 0) {
+                // Q as a pair: low parts to shared memory as they are, high parts by way of the last tile
+                // of the f16 ring, since a lane writes a whole row of TMEM
+                unsigned char* stage = reinterpret_cast<unsigned char*>(S.k[TILES - 1][0]);
+                unsigned char* stage2 = reinterpret_cast<unsigned char*>(S.v[TILES - 1][0]);
+                const int hf = lane >> 4, chunk = (lane & 15) >> 1;
+                const uint32_t sub = (uint32_t)(lane & 1) * 8;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int v = (warp - 8) * 16 + k;
+                    const float4 x = qv[k];
+                    const float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+                    const float p2 = pow2_floor(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))));
+                    const float up = pow2_inverse(p2);
+                    uint2 hi, lo;
+                    split2(x.x * up, x.y * up, hi.x, lo.x);
+                    split2(x.z * up, x.w * up, hi.y, lo.y);
+                    const uint32_t off = sw128(v, chunk) + sub;
+                    *reinterpret_cast<uint2*>((hf ? stage2 : stage) + off) = hi;
+                    *reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(S.q_lo[hf]) + off) = lo;
+                    if (lane == 0) S.qs[v] = p2 * kLog2e;
+                }
+                group_sync();
+                // each group writes half of the dims
+                uint32_t row_hi[32];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const uint4 x = lds128((odd ? stage2 : stage) + sw128(t, c));
+                    row_hi[4 * c] = x.x;
+                    row_hi[4 * c + 1] = x.y;
+                    row_hi[4 * c + 2] = x.z;
+                    row_hi[4 * c + 3] = x.w;
+                }
+                TMEM_ST_X32(tl + COL_Q + 32 * odd, row_hi);
+                tmem_wait_st();
+                fence_proxy_async_smem();
+                tc_fence_before();
+                mbar_arrive(&S.q_ready);
             }
-            if (j - j0 > 1 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-                const bool od = mbar_wait_bounded(&S.o_done[odd], (uint32_t)((j >> 1) - 1) & 1u);
-                if (!__all_sync(0xffffffffu, od)) { ok = false; break; }
-                tc_fence_after();
+            const float qs = n_blocks > 0 ? S.qs[t] : 0.0f;
+            const float lazy = fminf(kLazy / qs, 1e37f), room = fminf(kRoom / qs, 1e37f);
+            const uint32_t to = tl + COL_O + (uint32_t)(odd * D);
+            const size_t at = part_index(a, blockIdx.y, h, max_parts, blockIdx.z) + t;
+            // over the stretches joined so far: maximum, sum, and the group's half of the dims
+            float all_max = -INFINITY, all_sum = 0.0f, acc[64];
+#pragma unroll
+            for (int e = 0; e < 64; ++e) acc[e] = 0.0f;
+            bool ok = true;
+            for (int j0 = 0; j0 == 0 || j0 < n_blocks; j0 += STRETCH) {
+                const int j1 = min(j0 + STRETCH, n_blocks);
+                // running maximum of dk S (before qs), the same in log2 units, and the sum of weights
+                float top = -INFINITY, top2 = -INFINITY, sum = 0.0f, sigma = 0.0f;
+                for (int j = j0 + odd; ok && j < j1; j += 2) {
+                    const int d = j % TILES;
+                    const bool got = mbar_wait_bounded(&S.kv_full[d], (uint32_t)(j / TILES) & 1u) &&
+                                     mbar_wait_bounded(&S.s_full[j % SBUF], (uint32_t)(j / SBUF) & 1u);
+                    if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t ts = tl + (uint32_t)(j % SBUF * KB);
+                    uint32_t sv[KB];
+                    TMEM_LD_X32(ts, sv);
+                    TMEM_LD_X32(ts + 32, (sv + 32));
+                    tmem_wait_ld();
+                    const int key0 = (first + j) * KB;
+                    const int have = S.pages[d];
+                    const bool masked = !__all_sync(0xffffffffu, key0 + KB - 1 <= pos && have == (1 << PAGES) - 1);
+                    const float4* dk = reinterpret_cast<const float4*>(S.dk[d]);
+                    float bmax = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < KB; c += 4) {
+                        const float4 f = dk[c >> 2];
+                        const float2 x = attn::fmul2(make_float2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])),
+                                                     make_float2(f.x, f.y));
+                        const float2 y =
+                            attn::fmul2(make_float2(__uint_as_float(sv[c + 2]), __uint_as_float(sv[c + 3])),
+                                        make_float2(f.z, f.w));
+                        sv[c] = __float_as_uint(x.x);
+                        sv[c + 1] = __float_as_uint(x.y);
+                        sv[c + 2] = __float_as_uint(y.x);
+                        sv[c + 3] = __float_as_uint(y.y);
+                    }
+                    uint32_t seen[2] = {~0u, ~0u};             // keys of the block that the row attends to
+                    if (masked) {
+                        const int n = min(max(pos + 1 - key0, 0), KB);
+                        uint64_t bits = n == KB ? ~0ull : (1ull << n) - 1;
+#pragma unroll
+                        for (int q = 0; q < PAGES; ++q)
+                            if (!((have >> q) & 1)) bits &= ~(0xffffull << (16 * q));
+                        seen[0] = (uint32_t)bits;
+                        seen[1] = (uint32_t)(bits >> 32);
+#pragma unroll
+                        for (int c = 0; c < KB; ++c)
+                            if (!((seen[c >> 5] >> (c & 31)) & 1)) sv[c] = 0xff800000u;        // -inf
+                    }
+#pragma unroll
+                    for (int c = 0; c < KB; ++c) bmax = fmaxf(bmax, __uint_as_float(sv[c]));
+                    // a sigma of the row's own where it does not see every key: a large V that it may not see must
+                    // not scale its weights away
+                    float next_sigma = S.sigma[d];
+                    if (masked) {
+                        const float4* raw = reinterpret_cast<const float4*>(S.dv_raw[d]);
+                        uint32_t own = 11u << 23;
+#pragma unroll
+                        for (int c = 0; c < KB; c += 4) {
+                            const float4 f = raw[c >> 2];
+                            const uint32_t in = seen[c >> 5] >> (c & 31);
+                            if (in & 1) own = max(own, finite_exponent(f.x));
+                            if (in & 2) own = max(own, finite_exponent(f.y));
+                            if (in & 4) own = max(own, finite_exponent(f.z));
+                            if (in & 8) own = max(own, finite_exponent(f.w));
+                        }
+                        next_sigma = fmaxf(sigma, __uint_as_float(own - (kSigmaShift << 23)));
+                    }
+                    float alpha = j - j0 > 1 ? sigma * pow2_inverse(next_sigma) : 1.0f;
+                    sigma = next_sigma;
+                    if (top == -INFINITY) {
+                        top = bmax + room;                     // first block with a key: O holds nothing of this row
+                        top2 = __fmul_rn(top, qs);
+                    } else if (bmax > top + lazy) {
+                        top = bmax + room;
+                        const float next = __fmul_rn(top, qs);
+                        const float f = exp2f(top2 - next);
+                        top2 = next;
+                        alpha *= f;
+                        sum *= f;
+                    }
+                    if (j - j0 > 1 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                        const bool od = mbar_wait_bounded(&S.o_done[odd], (uint32_t)((j >> 1) - 1) & 1u);
+                        if (!__all_sync(0xffffffffu, od)) { ok = false; break; }
+                        tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < D; c += 16) {
-                    uint32_t ov[16];
-                    TMEM_LD_X16(to + c, ov);
-                    tmem_wait_ld();
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t ov[16];
+                            TMEM_LD_X16(to + c, ov);
+                            tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-                    TMEM_ST_X16(to + c, ov);
+                            for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+                            TMEM_ST_X16(to + c, ov);
+                        }
+                    }
+                    const float2 psum = masked ? weights<true>(sv, S.dv_raw[d], pow2_inverse(sigma), seen, qs, top2, ts)
+                                               : weights<false>(sv, S.dv[d], 1.0f, seen, qs, top2, ts);
+                    sum += psum.x + psum.y;
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&S.p_ready[j % SBUF]);
+                }
+                // the group's last product of the stretch: block j1 - 1 or j1 - 2
+                const int last_j = ((j1 - 1 - odd) & ~1) + odd;
+                if (ok && last_j >= j0 && j1 > odd) {
+                    const bool od = mbar_wait_bounded(&S.o_done[odd], (uint32_t)(last_j >> 1) & 1u);
+                    ok = __all_sync(0xffffffffu, od);
+                }
+                if (!ok && lane == 0) S.err = 1;
+                S.state[odd][0][t] = top2;
+                S.state[odd][1][t] = sum;
+                S.state[odd][2][t] = sigma;
+                tc_fence_before();
+                group_sync();
+                tc_fence_after();
+                if (!S.err) {
+                    // the two groups and the stretches before joined: acc = O0 f0 + O1 f1 + fa acc, each group half
+                    // of the dims
+                    const float m0 = S.state[0][0][t], m1 = S.state[1][0][t], best = fmaxf(fmaxf(m0, m1), all_max);
+                    float f0 = m0 == best ? 1.0f : exp2f(m0 - best), f1 = m1 == best ? 1.0f : exp2f(m1 - best);
+                    const float fa = all_max == best ? 1.0f : exp2f(all_max - best);
+                    all_sum = S.state[0][1][t] * f0 + S.state[1][1][t] * f1 + all_sum * fa;
+                    all_max = best;
+                    f0 *= S.state[0][2][t];
+                    f1 *= S.state[1][2][t];
+#pragma unroll
+                    for (int c = 0; c < 64; c += 16) {
+                        uint32_t ov[16];
+                        if (j1 > j0) {
+                            TMEM_LD_X16(tl + COL_O + 64 * odd + c, ov);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(__uint_as_float(ov[e]), f0, acc[c + e] * fa);
+                        }
+                        if (j1 - j0 > 1) {
+                            TMEM_LD_X16(tl + COL_O + D + 64 * odd + c, ov);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(__uint_as_float(ov[e]), f1, acc[c + e]);
+                        }
+                    }
+                }
+                tc_fence_before();
+                group_sync();                                  // O and the state may be written again
+                tc_fence_after();
+            }
+            if (!S.err) {
+                // the part's un-normalised sum, or the output
+                const float inv = parts > 1 ? 1.0f : all_sum == 0.0f ? 0.0f : 1.0f / all_sum;
+                if (parts > 1 && !odd) part_ml[at] = make_float2(all_max, all_sum);
+#pragma unroll
+                for (int c = 0; c < 64; c += 8) {
+                    float o[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] = acc[c + e] * inv;
+                    if (parts > 1) {
+                        float4* dst = reinterpret_cast<float4*>(part_o + at * D + 64 * odd + c);
+                        dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+                        dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+                    } else if (live) {
+                        store_values<8>(a, o_at + 64 * odd + c, o);
+                    }
                 }
             }
-            const float2 psum = masked ? weights<true>(sv, S.dv_raw[d], pow2_inverse(sigma), seen, qs, top2, ts)
-                                       : weights<false>(sv, S.dv[d], 1.0f, seen, qs, top2, ts);
-            sum += psum.x + psum.y;
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&S.p_ready[j % SBUF]);
-        }
-        // the group's last product of the stretch: block j1 - 1 or j1 - 2
-        const int last_j = ((j1 - 1 - odd) & ~1) + odd;
-        if (ok && last_j >= j0 && j1 > odd) {
-            const bool od = mbar_wait_bounded(&S.o_done[odd], (uint32_t)(last_j >> 1) & 1u);
-            ok = __all_sync(0xffffffffu, od);
-        }
-        if (!ok && lane == 0) S.err = 1;
-        S.state[odd][0][t] = top2;
-        S.state[odd][1][t] = sum;
-        S.state[odd][2][t] = sigma;
-        tc_fence_before();
-        group_sync();
-        tc_fence_after();
-        if (!S.err) {
-            // the two groups and the stretches before joined: acc = O0 f0 + O1 f1 + fa acc, each group half
-            // of the dims
-            const float m0 = S.state[0][0][t], m1 = S.state[1][0][t], best = fmaxf(fmaxf(m0, m1), all_max);
-            float f0 = m0 == best ? 1.0f : exp2f(m0 - best), f1 = m1 == best ? 1.0f : exp2f(m1 - best);
-            const float fa = all_max == best ? 1.0f : exp2f(all_max - best);
-            all_sum = S.state[0][1][t] * f0 + S.state[1][1][t] * f1 + all_sum * fa;
-            all_max = best;
-            f0 *= S.state[0][2][t];
-            f1 *= S.state[1][2][t];
-#pragma unroll
-            for (int c = 0; c < 64; c += 16) {
-                uint32_t ov[16];
-                if (j1 > j0) {
-                    TMEM_LD_X16(tl + COL_O + 64 * odd + c, ov);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(__uint_as_float(ov[e]), f0, acc[c + e] * fa);
-                }
-                if (j1 - j0 > 1) {
-                    TMEM_LD_X16(tl + COL_O + D + 64 * odd + c, ov);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(__uint_as_float(ov[e]), f1, acc[c + e]);
-                }
-            }
-        }
-        tc_fence_before();
-        group_sync();                                  // O and the state may be written again
-        tc_fence_after();
-        }
-        if (!S.err) {
-            // the part's un-normalised sum, or the output
-            const float inv = parts > 1 ? 1.0f : all_sum == 0.0f ? 0.0f : 1.0f / all_sum;
-            if (parts > 1 && !odd) part_ml[at] = make_float2(all_max, all_sum);
-#pragma unroll
-            for (int c = 0; c < 64; c += 8) {
-                float o[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = acc[c + e] * inv;
-                if (parts > 1) {
-                    float4* dst = reinterpret_cast<float4*>(part_o + at * D + 64 * odd + c);
-                    dst[0] = make_float4(o[0], o[1], o[2], o[3]);
-                    dst[1] = make_float4(o[4], o[5], o[6], o[7]);
-                } else if (live) {
-                    store_values<8>(a, o_at + 64 * odd + c, o);
-                }
-            }
-        }
         }
     }
     tc_fence_before();
