@@ -48,7 +48,7 @@ constexpr int PAGES = KB / kPageTokens;
 constexpr int RAW = 3;                        // raw ring (8-bit blocks)
 constexpr int TILES = 4;                      // f16 ring
 constexpr int THREADS = 512;
-constexpr int kRegsIssue = 56, kRegsExpand = 72, kRegsSoftmax = 192;
+constexpr int kRegsIssue = 32, kRegsExpand = 64, kRegsSoftmax = 208;
 static_assert(kRegsIssue + kRegsExpand + 2 * kRegsSoftmax <= 4 * 128, "registers of the launch");
 // Blocks summed in TMEM at a time. The tensor core's f32 sums are truncated, so their error grows
 // with their length (2.4e-6 of the output over 60 blocks, 1.6e-6 with stretches); stretches are
@@ -575,10 +575,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 64; ++e) acc[e] = 0.0f;
             bool ok = true;
+            // running maximum of dk S (before qs), the same in log2 units, and sigma
+            float top = -INFINITY, top2 = -INFINITY, sigma = 0.0f;
             for (int j0 = 0; j0 == 0 || j0 < n_blocks; j0 += STRETCH) {
                 const int j1 = min(j0 + STRETCH, n_blocks);
-                // running maximum of dk S (before qs), the same in log2 units, and the sum of weights
-                float top = -INFINITY, top2 = -INFINITY, sum = 0.0f, sigma = 0.0f;
+                float sum = 0.0f;                      // of the stretch's weights
                 for (int j = j0 + odd; ok && j < j1; j += 2) {
                     const int d = j % TILES;
                     const bool got = mbar_wait_bounded(&S.kv_full[d], (uint32_t)(j / TILES) & 1u) &&
