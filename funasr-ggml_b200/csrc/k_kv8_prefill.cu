@@ -25,11 +25,13 @@
 // mbarrier wait is bounded; on a timeout the CTA records the error, drains its copies and MMAs
 // and frees TMEM.
 //
-// Bound: per block of 64 keys and 128 query vectors the MMAs take 1170 cycles (with the pairs'
-// second products twice those of plain f16) and the kernel about 1560: softmax issue and the
-// hand-over between softmax and MMAs are the rest. 4 chunks of 417 to 512 rows at 3500 tokens (16
-// query heads on 8, 248 CTAs of one SM each) take 130 us; 300 with one softmax group, 174 with two
-// S buffers, 142 to 155 with masked and whole blocks in one pass. A chunk of 112 rows takes 14.6 us.
+// Bound: per block of 64 keys and 128 query vectors the MMAs take 1160 cycles (with the pairs'
+// second products twice those of plain f16) and the kernel about 1500: the way from S over the
+// softmax to O is longer than the MMAs between, and a rescale or a late page on it is not made up
+// for. 4 chunks of 417 to 512 rows at 3500 tokens (16 query heads on 8, 248 CTAs of one SM each)
+// take 122 us; 300 with one softmax group, 174 with two S buffers, 142 to 155 with masked and
+// whole blocks in one pass, 146 with each block halved between the groups (ten rescales a warp,
+// each on the way of the next product). A chunk of 112 rows takes 14.5 us.
 // A persistent form with an even split of the blocks took 160 and 26: every change of tile costs
 // 10 us of queries, joins and output, which separate CTAs overlap.
 #include "k_attn_body.cuh"
@@ -84,7 +86,8 @@ struct PfSmem {
     uint64_t kv_full[TILES];
     uint64_t kv_empty[TILES];
     uint64_t s_full[SBUF];
-    uint64_t p_ready[SBUF];
+    uint64_t p_half[SBUF];                    // weights of the block's first 32 keys are in TMEM
+    uint64_t p_ready[SBUF];                   // all of them are
     uint64_t q_ready;
     uint64_t o_done[2];
     uint64_t drain;
@@ -212,11 +215,11 @@ __host__ __device__ inline size_t part_index(const Kv8AttnArgs& a, int tile, int
 
 // The second pass over a block's scores (dk S in sv): p = exp2(dk S qs - top2), whose sum is
 // returned, and the weights p f (f: V scales over sigma, times `more` where MASKED) as f16 pairs
-// to TMEM over S. Keys not in `seen` weigh nothing: by selection, since the maximum may be -inf
+// to TMEM over S, the first half of them announced at half_bar. Keys not in `seen` weigh nothing: by selection, since the maximum may be -inf
 // and a scale NaN.
 template <bool MASKED>
 __device__ __forceinline__ float2 weights(const uint32_t (&sv)[KB], const float* factors, float more,
-                                          const uint32_t (&seen)[2], float qs, float top2, uint32_t ts) {
+                                          const uint32_t (&seen)[2], float qs, float top2, uint32_t ts, uint64_t* half_bar) {
     const float4* dv = reinterpret_cast<const float4*>(factors);
     const float2 qs2 = make_float2(qs, qs), neg = make_float2(-top2, -top2), minus = make_float2(-1.0f, -1.0f);
     float2 psum = make_float2(0.0f, 0.0f);
@@ -247,6 +250,11 @@ __device__ __forceinline__ float2 weights(const uint32_t (&sv)[KB], const float*
         }
         TMEM_ST_X16(ts + 16 * half, hi);
         TMEM_ST_X16(ts + 32 + 16 * half, lo);
+        if (half == 0) {
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(half_bar);
+        }
     }
     return psum;
 }
@@ -275,6 +283,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int s = 0; s < SBUF; ++s) {
             mbar_init(&S.s_full[s], 1);
             mbar_init(&S.p_ready[s], 128);
+            mbar_init(&S.p_half[s], 128);
         }
         mbar_init(&S.o_done[0], 1);
         mbar_init(&S.o_done[1], 1);
@@ -405,17 +414,25 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                     if (i >= 2) {
                         const int j = i - 2, s = j % TILES;
-                        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.p_ready[j % SBUF], (uint32_t)(j / SBUF) & 1u));
+                        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.p_half[j % SBUF], (uint32_t)(j / SBUF) & 1u));
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t d_p = tmem + (uint32_t)(j % SBUF * KB), d_o = tmem + COL_O + (uint32_t)((j & 1) * D);
+                        const uint32_t d_p = tmem + (uint32_t)(j % SBUF * KB);
+                        const uint32_t d_o = tmem + COL_O + (uint32_t)((j & 1) * D);
                         const uint64_t db = v_desc + (uint32_t)(s * (int)sizeof(S.v[0]) >> 4);
+                        // the first 32 keys' products as soon as their weights are there
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
+                            if (kk == 2) {
+                                ok = __all_sync(0xffffffffu,
+                                                mbar_wait_bounded(&S.p_ready[j % SBUF], (uint32_t)(j / SBUF) & 1u));
+                                tc_fence_after();
+                            }
                             const uint64_t at = db + kk * 16 * 64 * 2 / 16;
                             tc_mma_f16_ts_if(one, d_o, d_p + 8 * kk, at, kIdPV, (j % STRETCH > 1 || kk > 0) ? 1u : 0u);
                             tc_mma_f16_ts_if(one, d_o, d_p + 32 + 8 * kk, at, kIdPV, 1u);
                         }
+                        if (!ok) break;
                         tc_commit_if(one, &S.kv_empty[s]);
                         tc_commit_if(one, &S.o_done[j & 1]);
                     }
@@ -659,17 +676,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                         if (!__all_sync(0xffffffffu, od)) { ok = false; break; }
                         tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 16) {
-                            uint32_t ov[16];
-                            TMEM_LD_X16(to + c, ov);
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t ov[32];
+                            TMEM_LD_X32(to + c, ov);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-                            TMEM_ST_X16(to + c, ov);
+                            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+                            TMEM_ST_X32(to + c, ov);
                         }
                     }
-                    const float2 psum = masked ? weights<true>(sv, S.dv_raw[d], pow2_inverse(sigma), seen, qs, top2, ts)
-                                               : weights<false>(sv, S.dv[d], 1.0f, seen, qs, top2, ts);
+                    const float2 psum = masked ? weights<true>(sv, S.dv_raw[d], pow2_inverse(sigma), seen, qs, top2, ts, &S.p_half[j % SBUF])
+                                               : weights<false>(sv, S.dv[d], 1.0f, seen, qs, top2, ts, &S.p_half[j % SBUF]);
                     sum += psum.x + psum.y;
                     tmem_wait_st();
                     tc_fence_before();
