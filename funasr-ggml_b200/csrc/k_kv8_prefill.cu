@@ -10,9 +10,9 @@
 //   p  = exp2(dk S - m) one query vector per thread; w = p dv / sigma, sigma a power of two under
 //                       the largest dv that the row has seen: f16 pairs, written over S in TMEM
 //   O += w . V          M 128, N 128 (dims), K 64 (keys), V MN-major
-// A weight's pair is exact to 2^-25 at the least, so an output is off by up to 2^-24 of the
-// largest |V| that its row attends to (and of nothing that it does not attend to), which is what
-// f32 sums of the values give too unless the largest V has next to no weight.
+// A pair's rounding is 2^-25 at most, against 4 or more for the largest V at the running maximum:
+// an output is off by 2^-27 a key, as they fall together much less, of the largest |V| that its
+// row attends to (and of nothing that it does not attend to).
 // w and Q's high parts, the A operands of three quarters of the MMAs, are in TMEM: with all of Q
 // and w in shared memory a block would read 128 KB of it for its MMAs, against 1024 cycles that
 // they take. The running maximum is lazy: O is rescaled when a block exceeds it by 2^kLazy or
@@ -53,8 +53,8 @@ constexpr int THREADS = 512;
 constexpr int kRegsIssue = 32, kRegsExpand = 64, kRegsSoftmax = 208;
 static_assert(kRegsIssue + kRegsExpand + 2 * kRegsSoftmax <= 4 * 128, "registers of the launch");
 // Blocks summed in TMEM at a time. The tensor core's f32 sums are truncated, so their error grows
-// with their length (2.4e-6 of the output over 60 blocks, 1.6e-6 with stretches); stretches are
-// joined in f32 arithmetic rounded to nearest, which costs 6 % over one sum.
+// with their length (2.0e-6 of the output over 57 blocks, 1.2e-6 with stretches of 32); stretches
+// are joined in f32 arithmetic rounded to nearest, which costs 1 %.
 constexpr int STRETCH = 32;
 constexpr int kMaxParts = 16;                 // key ranges of one tile and head
 constexpr int kMinPartBlocks = 8;
@@ -63,8 +63,9 @@ constexpr int kMinPartBlocks = 8;
 constexpr int SBUF = 3;
 constexpr uint32_t TMEM_COLS = 512, COL_O = 192, COL_Q = 448;
 // A running maximum is set kRoom above the block's and stays until a block exceeds it by kLazy
-// (log2 units): weights reach 2^kLazy, and O is rescaled once in kRoom + kLazy.
-constexpr float kLazy = 11.0f, kRoom = 4.0f;
+// (log2 units): weights reach 2^kLazy, and O is rescaled once in kRoom + kLazy. More room rescales
+// less and leaves the weights fewer bits (4: as fast, 1.8e-6 of the output instead of 1.2e-6).
+constexpr float kLazy = 11.0f, kRoom = 1.0f;
 constexpr uint32_t kSigmaShift = 3;           // the largest V scale over sigma is 2^3 to 2^4: w < 2^15
 
 struct PfSmem {
