@@ -74,27 +74,42 @@ namespace {
 //
 // Bound: HBM. 128 rows of 2048 tokens (16 heads on 8, 554 MB of tiles) take 95-98 us: 84 us of
 // pages at the rate of a copy, then some 5 us each of start (lengths, split, page look-ups: four
-// dependent loads) and of merge; without its arithmetic the kernel takes as long. Short calls are
-// those two chains: one row of 256 tokens 8.2 us, 16 rows of 1 to 1021 tokens 11.3 us. 12 or 6
-// warps a CTA took 98.6 and 98.9 us; two to four CTAs' worth of grid a slot 102 to 109; the
-// merge inside the kernel (arrival words) 101, and 10.3 for the one row.
+// dependent loads) and of merge; without its arithmetic the kernel takes as long. 12 or 6 warps a
+// CTA took 98.6 and 98.9 us, grids of two to four waves 102 to 109, the merge inside the kernel
+// (arrival words) 101. Short calls are latency: the loads of the start, and 0.45 us a page and
+// warp (K's MMAs, softmax and V's depend on each other).
 constexpr int kWarps = 4;
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 148 * kCtasPerSm;     // one resident wave of a B200
 constexpr int kItemUnits = 2;                  // with ranges per warp: 16 ragged rows 25.6 -> 12.8 us
 
 constexpr int kStages = 3;                     // 128 rows x 2048 tokens: 2 stages 97, 3 95, 4 98 us
-template <int NT>
+
+// Short contexts: a CTA per (row, KV head), whose warps share its pages evenly, needs no list and
+// no merge kernel. It is taken while those CTAs are one resident wave and the block table bounds
+// the context to so many pages that the uneven rows and idle SMs cost less than they save (us, int8,
+// 16 heads on 8, list / CTA per item):
+//   1 row of 64 tokens 7.9 / 4.4, 256 7.9 / 6.5, 512 8.8 / 8.2, 1024 9.2 / 11.7
+//   16 rows of 256 9.9 / 6.8, 512 11.7 / 8.6, 1024 15.8 / 13.0, 1 to 1024 11.8 / 11.6
+//   55 rows of 256 14.9 / 9.9, 1024 30.1 / 24.8, 1 to 1024 22.3 / 21.7, 1 to 2048 31.9 / 36.3
+//   128 rows (more than a wave) of 256 23.9 / 24.9, 1024 54.8 / 58.7
+// Up to an item an SM it has eight warps (4 rows of 512: 8.2 us, with four 9.3, with twelve 8.5).
+constexpr int kItemWarps = 8;
+bool cta_per_item(long long items, int bt_stride) {
+    return items <= kMaxCtas && bt_stride <= (items > 64 ? 64 : 32);
+}
+
+template <int NT, int W>
 struct DecodeSmem {
-    unsigned char tiles[kWarps][kStages][2 * kPartBytes];   // K then V, 128 B swizzle
-    float scales[kWarps][kStages][2 * kPageTokens];         // K then V
+    unsigned char tiles[W][kStages][2 * kPartBytes];   // K then V, 128 B swizzle
+    float scales[W][kStages][2 * kPageTokens];         // K then V
     // the warps' first partials; their last ones go over the warp's ring once it is drained
-    float acc[kWarps][4 * NT][D];
-    float2 ml[kWarps][2][4 * NT];                               // running maximum (log2 units), sum
-    int4 item[kWarps][2];                                       // (row, KV head, first page, pages), row -1: none
-    uint64_t bars[kWarps][kStages];
-    long long scan[kWarps];
-    int np[kWarps][2];
+    float acc[W][4 * NT][D];
+    float2 ml[W][2][4 * NT];                               // running maximum (log2 units), sum
+    int4 item[W][2];                                       // (row, KV head, first page, pages), row -1: none
+    uint64_t bars[W][kStages];
+    long long scan[W];
+    int np[W][2];
     int start[3];                                               // the CTA's first row, KV head, unit
 };
 
@@ -229,12 +244,12 @@ __device__ __forceinline__ float split_query(const float (&x)[32], int g, int t,
     return __shfl_sync(0xffffffffu, p2, 8 * t) * kLog2e;          // held by the lanes of columns 2t, 2t + 1
 }
 
-template <int FMT, int NT>
-__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
+template <int FMT, int NT, int W, bool ITEM>
+__global__ void __launch_bounds__(W * 32, W == kWarps ? kCtasPerSm : 1)
     kv8_decode_kernel(const __grid_constant__ CUtensorMap tm_pool, const Kv8AttnArgs a, void* scratch) {
     constexpr int ST = kStages;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    DecodeSmem<NT>& S = *reinterpret_cast<DecodeSmem<NT>*>(smem_raw);
+    DecodeSmem<NT, W>& S = *reinterpret_cast<DecodeSmem<NT, W>*>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t = lane & 3;
     const int G = a.Hq / a.Hkv;
@@ -244,79 +259,94 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     // the list's length, and where this CTA's chunk begins
     if (tid == 0) {
         tma_prefetch_desc(&tm_pool);
-        for (int w = 0; w < kWarps; ++w)
+        for (int w = 0; w < W; ++w)
             for (int s = 0; s < ST; ++s) mbar_init(&S.bars[w][s], 1);
         fence_mbar_init();
     }
-    const int per = (a.M + kWarps * 32 - 1) / (kWarps * 32);
-    const int r0 = min(tid * per, a.M), r1 = min(r0 + per, a.M);
-    long long mine = 0;
-    for (int m = r0; m < r1; ++m) {
-        const int np = row_pages(a, m);
-        mine += np ? np + kItemUnits : 0;
-    }
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 31) S.scan[warp] = incl;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) incl += S.scan[w];
-        total += S.scan[w];
-    }
-    total *= a.Hkv;
-    const int per_warp = (int)ceil_div(total, gridDim.x * kWarps);
-    const long long begin = (long long)blockIdx.x * kWarps * per_warp;
-    const bool work = begin < total;
-    long long before = (incl - mine) * a.Hkv;
-    if (work && before <= begin && begin < incl * a.Hkv) {
-        for (int m = r0; m < r1; ++m) {
-            const int np = row_pages(a, m), units = np ? np + kItemUnits : 0;
-            if (begin < before + (long long)units * a.Hkv) {
-                const int h = (int)floor_div(begin - before, units);
-                S.start[0] = m;
-                S.start[1] = h;
-                S.start[2] = (int)(begin - before - (long long)h * units);
-                break;
-            }
-            before += (long long)units * a.Hkv;
+    // rows without pages: padding is zeroed, one that cannot be served is flagged and left
+    auto rows_without_pages = [&] {
+        for (int m = blockIdx.x; m < a.M; m += gridDim.x) {
+            if (a.pos[m] == -1)
+                for (int d = 4 * tid; d < a.Hq * D; d += W * 128)
+                    store4(a, (size_t)m * a.Hq * D + d, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 1.0f);
+            else if (tid == 0 && row_bad(a, m)) record_error(a.err, kDevErrBadLen);
         }
-    }
-    // rows without pages: padding is zeroed, a row that cannot be served is flagged and left
-    for (int m = blockIdx.x; m < a.M; m += gridDim.x) {
-        if (a.pos[m] == -1)
-            for (int d = 4 * tid; d < a.Hq * D; d += kWarps * 128)
-                store4(a, (size_t)m * a.Hq * D + d, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 1.0f);
-        else if (tid == 0 && row_bad(a, m)) record_error(a.err, kDevErrBadLen);
-    }
-    __syncthreads();
+    };
     Place at{-1, 0, 0, 0};
-    if (work) {
-        at = Place{S.start[0], S.start[1], S.start[2], 0};
+    int nw = 0;                                  // pages of the warp's range, which begins at `at`
+    if (ITEM) {
+        at.m = blockIdx.x / a.Hkv;
+        at.h = blockIdx.x % a.Hkv;
         at.np = row_pages(a, at.m);
-    }
-    if (tid == 0) {
-        part.begin[blockIdx.x] = make_int4(at.m, at.h, at.u, at.np);
-        if (blockIdx.x == 0) *part.chunk = kWarps * per_warp;
-    }
-    if (!work) return;
-
-    // the warp's range: per_warp units from `at`, nw pages among them
-    skip_units(a, at, warp * per_warp);
-    int nw = 0;
-    {
-        Place x = at;
-        for (int left = per_warp; left > 0 && x.m < a.M; next_item(a, x)) {
-            nw += max(0, min(x.np - x.u, left));
-            left -= min(left, x.np + kItemUnits - x.u);
+        rows_without_pages();
+        __syncthreads();
+        if (at.np == 0) return;
+        const int per_warp = (at.np + W - 1) / W;
+        at.u = min(warp * per_warp, at.np);
+        nw = min(per_warp, at.np - at.u);
+    } else {
+        const int per = (a.M + W * 32 - 1) / (W * 32);
+        const int r0 = min(tid * per, a.M), r1 = min(r0 + per, a.M);
+        long long mine = 0;
+        for (int m = r0; m < r1; ++m) {
+            const int np = row_pages(a, m);
+            mine += np ? np + kItemUnits : 0;
         }
+        long long incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) S.scan[warp] = incl;
+        __syncthreads();
+        long long total = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w < warp) incl += S.scan[w];
+            total += S.scan[w];
+        }
+        total *= a.Hkv;
+        const int per_warp = (int)ceil_div(total, gridDim.x * W);
+        const long long begin = (long long)blockIdx.x * W * per_warp;
+        const bool work = begin < total;
+        long long before = (incl - mine) * a.Hkv;
+        if (work && before <= begin && begin < incl * a.Hkv) {
+            for (int m = r0; m < r1; ++m) {
+                const int np = row_pages(a, m), units = np ? np + kItemUnits : 0;
+                if (begin < before + (long long)units * a.Hkv) {
+                    const int h = (int)floor_div(begin - before, units);
+                    S.start[0] = m;
+                    S.start[1] = h;
+                    S.start[2] = (int)(begin - before - (long long)h * units);
+                    break;
+                }
+                before += (long long)units * a.Hkv;
+            }
+        }
+        rows_without_pages();
+        __syncthreads();
+        if (work) {
+            at = Place{S.start[0], S.start[1], S.start[2], 0};
+            at.np = row_pages(a, at.m);
+        }
+        if (tid == 0) {
+            part.begin[blockIdx.x] = make_int4(at.m, at.h, at.u, at.np);
+            if (blockIdx.x == 0) *part.chunk = W * per_warp;
+        }
+        if (!work) return;
+
+        // the warp's range: per_warp units from `at`
+        skip_units(a, at, warp * per_warp);
+        {
+            Place x = at;
+            for (int left = per_warp; left > 0 && x.m < a.M; next_item(a, x)) {
+                nw += max(0, min(x.np - x.u, left));
+                left -= min(left, x.np + kItemUnits - x.u);
+            }
+        }
+        if (nw > 0 && at.u >= at.np) next_item(a, at);                // begins in the units behind an item's pages
     }
-    if (nw > 0 && at.u >= at.np) next_item(a, at);                // begins in the units behind an item's pages
     float qx[NT][32];                            // the first item's queries, under way while its pages are looked up
 #pragma unroll
     for (int c = 0; c < NT; ++c) load_query(a, at, nw > 0 ? G : 0, 4 * c + (g >> 1), t, qx[c]);
@@ -542,17 +572,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     }
 
     // The warps' partials in list order, lane k the k-th: those of one (row, KV head) are
-    // neighbours, a run. Warp w joins the runs of heads w, w + kWarps, ..., lane l dims 4 l ..
+    // neighbours, a run. Warp w joins the runs of heads w, w + W, ..., lane l dims 4 l ..
     __syncthreads();
-    static_assert(2 * kWarps <= 32, "a lane per partial");
+    static_assert(2 * W <= 32, "a lane per partial");
     int4 it = make_int4(-1, 0, 0, 0);
     int np = 0;
-    if (lane < 2 * kWarps) {
+    if (lane < 2 * W) {
         it = S.item[lane >> 1][lane & 1];
         np = S.np[lane >> 1][lane & 1];
     }
     const uint32_t parts = __ballot_sync(0xffffffffu, it.x >= 0);
-    for (int head = warp; head < G; head += kWarps) {
+    for (int head = warp; head < G; head += W) {
         const float2 ml = it.x >= 0 ? S.ml[lane >> 1][lane & 1][head] : make_float2(-INFINITY, 0.0f);
         for (uint32_t todo = parts; todo;) {
             const int k0 = __ffs(todo) - 1;
@@ -583,7 +613,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
                 O.z = fmaf(v.z, fk, O.z);
                 O.w = fmaf(v.w, fk, O.w);
             }
-            if (sum_pages == pages) {
+            if (ITEM || sum_pages == pages) {
                 store4(a, ((size_t)m * a.Hq + h * G + head) * D + 4 * lane, O, L);
             } else {
                 // the item that the CTA begins inside (or with) goes to its first slot, one that it does not
@@ -703,8 +733,22 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv8_merge_kernel(const Kv8At
 }
 
 template <int FMT, int NT>
-cudaError_t launch_decode(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scratch, int grid, cudaStream_t s) {
-    kv8_decode_kernel<FMT, NT><<<grid, kWarps * 32, sizeof(DecodeSmem<NT>), s>>>(tm, a, scratch);
+cudaError_t launch_decode(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scratch, cudaStream_t s) {
+    const long long items = (long long)a.M * a.Hkv;
+    const bool per_item = cta_per_item(items, a.bt_stride);
+    if (per_item && items <= 148) {
+        kv8_decode_kernel<FMT, NT, kItemWarps, true>
+            <<<(int)items, kItemWarps * 32, sizeof(DecodeSmem<NT, kItemWarps>), s>>>(tm, a, scratch);
+        return cudaGetLastError();
+    }
+    if (per_item) {
+        kv8_decode_kernel<FMT, NT, kWarps, true>
+            <<<(int)items, kWarps * 32, sizeof(DecodeSmem<NT, kWarps>), s>>>(tm, a, scratch);
+        return cudaGetLastError();
+    }
+    const int grid = (int)std::min<long long>(items * a.bt_stride, kMaxCtas);   // no more CTAs than there can be pages
+    kv8_decode_kernel<FMT, NT, kWarps, false>
+        <<<grid, kWarps * 32, sizeof(DecodeSmem<NT, kWarps>), s>>>(tm, a, scratch);
     if (grid == 1) return cudaGetLastError();
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
@@ -721,15 +765,22 @@ cudaError_t launch_decode(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scr
     return cudaLaunchKernelEx(&cfg, kv8_merge_kernel, a, scratch, grid);
 }
 
+template <int FMT, int NT>
+void configure_decode() {
+    const cudaFuncAttribute attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    cudaFuncSetAttribute(kv8_decode_kernel<FMT, NT, kWarps, false>, attr, (int)sizeof(DecodeSmem<NT, kWarps>));
+    cudaFuncSetAttribute(kv8_decode_kernel<FMT, NT, kWarps, true>, attr, (int)sizeof(DecodeSmem<NT, kWarps>));
+    cudaFuncSetAttribute(kv8_decode_kernel<FMT, NT, kItemWarps, true>, attr, (int)sizeof(DecodeSmem<NT, kItemWarps>));
+}
+
 }  // namespace
 
 // Opt the kernels into their dynamic shared memory on the current device.
 void configure_kv8_attention() {
-    const cudaFuncAttribute attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    cudaFuncSetAttribute(kv8_decode_kernel<kInt8, 1>, attr, (int)sizeof(DecodeSmem<1>));
-    cudaFuncSetAttribute(kv8_decode_kernel<kInt8, 2>, attr, (int)sizeof(DecodeSmem<2>));
-    cudaFuncSetAttribute(kv8_decode_kernel<kE4m3, 1>, attr, (int)sizeof(DecodeSmem<1>));
-    cudaFuncSetAttribute(kv8_decode_kernel<kE4m3, 2>, attr, (int)sizeof(DecodeSmem<2>));
+    configure_decode<kInt8, 1>();
+    configure_decode<kInt8, 2>();
+    configure_decode<kE4m3, 1>();
+    configure_decode<kE4m3, 2>();
 }
 
 }  // namespace fa
@@ -755,15 +806,13 @@ extern "C" FA_API int fa_op_paged_attention_kv8(const float* q, int M, int n_hea
     CUtensorMap tm;
     if (!make_kv8_tile_map(&tm, pool_layer, (long long)n_pages * n_kv_heads * (kTileBytes / 128)))
         return report_op_error(FA_ERR_CUDA, "fa_op_paged_attention_kv8: cannot build the page-pool tensor map");
-    // no more CTAs than there can be pages
-    const int grid = (int)std::min<long long>((long long)M * n_kv_heads * bt_stride, kMaxCtas);
     const bool wide = n_heads / n_kv_heads > 4;
     const cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e;
     if (format == FA_KV8_INT8)
-        e = wide ? launch_decode<kInt8, 2>(tm, a, scratch, grid, st) : launch_decode<kInt8, 1>(tm, a, scratch, grid, st);
+        e = wide ? launch_decode<kInt8, 2>(tm, a, scratch, st) : launch_decode<kInt8, 1>(tm, a, scratch, st);
     else
-        e = wide ? launch_decode<kE4m3, 2>(tm, a, scratch, grid, st) : launch_decode<kE4m3, 1>(tm, a, scratch, grid, st);
+        e = wide ? launch_decode<kE4m3, 2>(tm, a, scratch, st) : launch_decode<kE4m3, 1>(tm, a, scratch, st);
     if (e == cudaSuccess) return FA_OK;
     cudaGetLastError();
     return report_op_error(FA_ERR_CUDA, (std::string("fa_op_paged_attention_kv8: ") + cudaGetErrorString(e)).c_str());

@@ -593,6 +593,42 @@ def test_decode_attention_flags_bad_rows(torch_cuda, bad):
         assert rel_rms(got[m], P.attention(q[m], k, v).reshape(-1)) <= 5e-6
 
 
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,M,pages", [
+    (16, 8, 1, 32), (16, 8, 1, 33), (16, 8, 8, 33), (16, 8, 9, 64), (16, 8, 9, 65), (16, 8, 18, 64), (16, 8, 19, 20),
+    (16, 8, 55, 9), (16, 8, 56, 9), (32, 4, 30, 12), (32, 4, 50, 12), (7, 1, 100, 3), (1, 1, 3, 1)])
+def test_decode_attention_table_widths(torch_cuda, fmt, hq, hkv, M, pages):
+    """Rows of any length up to the table's, the longest among them, with padding rows, a bad slot
+    and a bad page: on both sides of the sizes at which a call is cut into work another way."""
+    torch = torch_cuda
+    rng = np.random.default_rng(100 * pages + M)
+    lens = rng.integers(1, 16 * pages + 1, M)
+    lens[0] = 16 * pages
+    pool, bt, n_pages = _filled(rng, lens.tolist(), 1, hkv, fmt)
+    assert bt.shape[1] == pages
+    pos, slot = (lens - 1).astype(np.int32), np.arange(M, dtype=np.int32)
+    kb, left, missing = bt.copy(), {}, -1
+    if M > 4:
+        pos[2], slot[3] = -1, -5
+        left = {2: 0.0, 3: 5.0}
+        missing = int(np.argmax(lens[4:])) + 4                    # loses its first page
+        kb[missing, 0] = n_pages + 7
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    err = _err(torch)
+    got = _decode(torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, slot), dev(torch, kb), n_pages, fmt,
+                  dev(torch, pool), err).cpu().numpy()
+    assert int(err) == (10 if M > 4 else 0)
+    for m in range(M):
+        if m in left:
+            assert (got[m] == left[m]).all()
+            continue
+        k, v = (x[0] for x in P.read(pool, bt[m], 0, lens[m], fmt))
+        if m == missing:
+            k, v = k[:, 16:], v[:, 16:]
+        want = P.attention(q[m], k, v).reshape(-1) if k.shape[1] else np.zeros(hq * 128)
+        assert np.abs(got[m] - want).max() <= (_bound(q[m], k, v) if k.shape[1] else 0), m
+
+
 # ----------------------------------------------------------------- prefill --
 @pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
 @pytest.mark.parametrize("hq,hkv,chunks", [
