@@ -520,7 +520,8 @@ extern "C" FA_API int fa_op_kv8_append(const void* k, const void* v, int src_typ
     if (misaligned(k, 16) || misaligned(v, 16) || misaligned(pool, 128))
         return report_op_error(FA_ERR_INVALID_ARG, "fa_op_kv8_append: k and v must be 16-byte, pool 128-byte aligned");
     const long long pairs = (long long)n_layers * n_kv_heads;
-    if (pairs > 0x7fffffffll) return report_op_error(FA_ERR_CAPACITY, "fa_op_kv8_append: too many vectors for one call");
+    if (pairs > 0x7fffffffll)
+        return report_op_error(FA_ERR_CAPACITY, "fa_op_kv8_append: too many vectors for one call");
     const bool four = several_per_warp(M * pairs);
     const long long per_row = four ? (pairs + 31) / 32 : (pairs + 7) / 8;
     if (M * per_row > 0x7fffffffll)

@@ -29,9 +29,9 @@
 // second products twice those of plain f16) and the kernel about 1500: the way from S over the
 // softmax to O is longer than the MMAs between, and a rescale or a late page on it is not made up
 // for. 4 chunks of 417 to 512 rows at 3500 tokens (16 query heads on 8, 248 CTAs of one SM each)
-// take 122 us; 300 with one softmax group, 174 with two S buffers, 142 to 155 with masked and
+// take 120 us; 300 with one softmax group, 174 with two S buffers, 142 to 155 with masked and
 // whole blocks in one pass, 146 with each block halved between the groups (ten rescales a warp,
-// each on the way of the next product). A chunk of 112 rows takes 14.5 us.
+// each on the way of the next product). A chunk of 112 rows takes 13.9 us.
 // A persistent form with an even split of the blocks took 160 and 26: every change of tile costs
 // 10 us of queries, joins and output, which separate CTAs overlap.
 #include "k_attn_body.cuh"
@@ -78,6 +78,7 @@ struct PfSmem {
     float dv[TILES][KB];                      // V scales / sigma, for rows that see the whole block
     float dv_raw[TILES][KB];                  // V scales, for the others
     float sigma[TILES];                       // of all keys up to the block's last
+    int live[128];                            // the query vector has a row that can be served
     float qs[128];                            // what takes dk S of a query vector to log2 units
     float state[2][3][128];                   // even / odd blocks' maximum, sum and sigma of each vector
     int raw_pages[RAW];                       // bit q: page q of the block was copied
@@ -216,11 +217,12 @@ __host__ __device__ inline size_t part_index(const Kv8AttnArgs& a, int tile, int
 
 // The second pass over a block's scores (dk S in sv): p = exp2(dk S qs - top2), whose sum is
 // returned, and the weights p f (f: V scales over sigma, times `more` where MASKED) as f16 pairs
-// to TMEM over S, the first half of them announced at half_bar. Keys not in `seen` weigh nothing: by selection, since the maximum may be -inf
-// and a scale NaN.
+// to TMEM over S, the first 32 keys' announced at half_bar. Keys not in `seen` weigh nothing: by
+// selection, since the maximum may be -inf and a scale NaN.
 template <bool MASKED>
 __device__ __forceinline__ float2 weights(const uint32_t (&sv)[KB], const float* factors, float more,
-                                          const uint32_t (&seen)[2], float qs, float top2, uint32_t ts, uint64_t* half_bar) {
+                                          const uint32_t (&seen)[2], float qs, float top2, uint32_t ts,
+                                          uint64_t* half_bar) {
     const float4* dv = reinterpret_cast<const float4*>(factors);
     const float2 qs2 = make_float2(qs, qs), neg = make_float2(-top2, -top2), minus = make_float2(-1.0f, -1.0f);
     float2 psum = make_float2(0.0f, 0.0f);
@@ -306,12 +308,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     // warps 8-15: 16 query vectors each, lane l dims [4 l, 4 l + 4); vectors without a row are zero
     float4 qv[16];
     if (warp >= 8) {
+        int head = (warp - 8) * 16 / R, r = (warp - 8) * 16 - head * R;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-            const int v = (warp - 8) * 16 + k, r = v % R, head = v / R;
             qv[k] = !bad && head < G && r < tile.y
                         ? reinterpret_cast<const float4*>(a.q + ((size_t)(tile.x + r) * a.Hq + h * G + head) * D)[lane]
                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (++r == R) {
+                r = 0;
+                ++head;
+            }
         }
     }
     if (warp == 2) {
@@ -353,7 +359,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                 }
                 const int s = j % RAW;
-                if (j >= RAW) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.raw_empty[s], (uint32_t)(j / RAW - 1) & 1u));
+                if (j >= RAW)
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.raw_empty[s], (uint32_t)(j / RAW - 1) & 1u));
                 if (!ok) break;
                 int id[PAGES], have = 0;
 #pragma unroll
@@ -544,7 +551,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
             const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16);
-            const size_t o_at = ((size_t)row * a.Hq + h * G + head) * D;
             if (n_blocks > 0) {
                 // Q as a pair: low parts to shared memory as they are, high parts by way of the last tile
                 // of the f16 ring, since a lane writes a whole row of TMEM
@@ -686,8 +692,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                             TMEM_ST_X32(to + c, ov);
                         }
                     }
-                    const float2 psum = masked ? weights<true>(sv, S.dv_raw[d], pow2_inverse(sigma), seen, qs, top2, ts, &S.p_half[j % SBUF])
-                                               : weights<false>(sv, S.dv[d], 1.0f, seen, qs, top2, ts, &S.p_half[j % SBUF]);
+                    uint64_t* half_bar = &S.p_half[j % SBUF];
+                    const float2 psum =
+                        masked ? weights<true>(sv, S.dv_raw[d], pow2_inverse(sigma), seen, qs, top2, ts, half_bar)
+                               : weights<false>(sv, S.dv[d], 1.0f, seen, qs, top2, ts, half_bar);
                     sum += psum.x + psum.y;
                     tmem_wait_st();
                     tc_fence_before();
@@ -737,21 +745,34 @@ __global__ void __launch_bounds__(THREADS, 1)
                 group_sync();                                  // O and the state may be written again
                 tc_fence_after();
             }
+            // the part's un-normalised sum, or the output, by way of the K tiles (no MMA reads them any
+            // more), so that a warp stores whole rows: from a row per thread, 112 rows took 3 us longer
+            unsigned char* stage = reinterpret_cast<unsigned char*>(S.k[0][0]);
+            const float inv = parts > 1 ? 1.0f : all_sum == 0.0f ? 0.0f : 1.0f / all_sum;
+            if (parts > 1 && !odd && !S.err) part_ml[at] = make_float2(all_max, all_sum);
+            if (!odd) S.live[t] = live;
+#pragma unroll
+            for (int c = 0; c < 64; c += 4)
+                *reinterpret_cast<float4*>(stage + t * 512 + (((16 * odd + (c >> 2)) ^ (t & 7)) << 4)) =
+                    make_float4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv, acc[c + 3] * inv);
+            group_sync();
             if (!S.err) {
-                // the part's un-normalised sum, or the output
-                const float inv = parts > 1 ? 1.0f : all_sum == 0.0f ? 0.0f : 1.0f / all_sum;
-                if (parts > 1 && !odd) part_ml[at] = make_float2(all_max, all_sum);
-#pragma unroll
-                for (int c = 0; c < 64; c += 8) {
-                    float o[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] = acc[c + e] * inv;
+                const int v0 = (warp - 8) * 16;
+                const size_t part_at = part_index(a, blockIdx.y, h, max_parts, blockIdx.z);
+                int vh = v0 / R, vr = v0 - vh * R;
+#pragma unroll 4
+                for (int k = 0; k < 16; ++k) {
+                    const int v = v0 + k;
+                    const float4 o = *reinterpret_cast<const float4*>(stage + v * 512 + ((lane ^ (v & 7)) << 4));
                     if (parts > 1) {
-                        float4* dst = reinterpret_cast<float4*>(part_o + at * D + 64 * odd + c);
-                        dst[0] = make_float4(o[0], o[1], o[2], o[3]);
-                        dst[1] = make_float4(o[4], o[5], o[6], o[7]);
-                    } else if (live) {
-                        store_values<8>(a, o_at + 64 * odd + c, o);
+                        reinterpret_cast<float4*>(part_o + (part_at + v) * D)[lane] = o;
+                    } else if (S.live[v]) {
+                        const float x[4] = {o.x, o.y, o.z, o.w};
+                        store_values<4>(a, ((size_t)(tile.x + vr) * a.Hq + h * G + vh) * D + 4 * lane, x);
+                    }
+                    if (++vr == R) {
+                        vr = 0;
+                        ++vh;
                     }
                 }
             }
