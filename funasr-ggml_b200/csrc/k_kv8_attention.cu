@@ -16,29 +16,27 @@ bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p
 }  // namespace
 
 // The arguments that decode and prefill share, checked; FA_OK or the recorded error.
-int kv8_attention_check(const std::string& what, const Kv8AttnArgs& a, int format, const void* scratch,
+int kv8_attention_check(const char* what, const Kv8AttnArgs& a, int format, const void* scratch,
                         size_t scratch_bytes, size_t need) {
+    auto refuse = [&](int code, const std::string& why) { return report_op_error(code, (what + why).c_str()); };
     if (!a.q || !a.pos || !a.slot || !a.block_table || !a.pool || (!a.out16 && !a.out32) || a.M <= 0 || a.Hq <= 0 ||
         a.Hkv <= 0 || a.bt_stride <= 0 || a.n_pages <= 0)
-        return report_op_error(FA_ERR_INVALID_ARG, (what + ": null or non-positive argument").c_str());
+        return refuse(FA_ERR_INVALID_ARG, ": null or non-positive argument");
     if (a.out16_lo && !a.out16)
-        return report_op_error(FA_ERR_INVALID_ARG, (what + ": out16_lo needs out16").c_str());
+        return refuse(FA_ERR_INVALID_ARG, ": out16_lo needs out16");
     if (format != FA_KV8_INT8 && format != FA_KV8_E4M3)
-        return report_op_error(FA_ERR_INVALID_ARG, (what + ": unknown format").c_str());
+        return refuse(FA_ERR_INVALID_ARG, ": unknown format");
     if (a.Hq % a.Hkv || a.Hq / a.Hkv > 8)
-        return report_op_error(FA_ERR_INVALID_ARG,
-                               (what + ": n_heads must be 1 to 8 times n_kv_heads").c_str());
+        return refuse(FA_ERR_INVALID_ARG, ": n_heads must be 1 to 8 times n_kv_heads");
     if (misaligned(a.q, 16) || misaligned(a.pool, 128) || misaligned(a.out16, 16) || misaligned(a.out16_lo, 16) ||
         misaligned(a.out32, 16) || misaligned(scratch, 16))
-        return report_op_error(FA_ERR_INVALID_ARG,
-                               (what + ": q, outputs and scratch must be 16-byte, pool 128-byte aligned").c_str());
+        return refuse(FA_ERR_INVALID_ARG, ": q, outputs and scratch must be 16-byte, pool 128-byte aligned");
     if (a.Hq > 65535 || (long long)a.bt_stride * kPageTokens > (1ll << 30))
-        return report_op_error(FA_ERR_CAPACITY, (what + ": n_heads or bt_stride too large").c_str());
+        return refuse(FA_ERR_CAPACITY, ": n_heads or bt_stride too large");
     if ((long long)a.n_pages * a.Hkv * (kTileBytes / 128) > 0x7fffffffll)
-        return report_op_error(FA_ERR_CAPACITY, (what + ": the pool has too many pages").c_str());
+        return refuse(FA_ERR_CAPACITY, ": the pool has too many pages");
     if (need && (!scratch || scratch_bytes < need))
-        return report_op_error(FA_ERR_INVALID_ARG, (what + ": scratch of " + std::to_string(need) +
-                                                    " bytes required").c_str());
+        return refuse(FA_ERR_INVALID_ARG, ": scratch of " + std::to_string(need) + " bytes required");
     return FA_OK;
 }
 

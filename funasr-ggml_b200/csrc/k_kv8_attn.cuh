@@ -95,7 +95,7 @@ __device__ __forceinline__ void store4(const Kv8AttnArgs& a, size_t o, float4 x,
 }  // namespace kv8
 
 // The arguments that decode and prefill share, checked; FA_OK or the recorded error.
-int kv8_attention_check(const std::string& what, const kv8::Kv8AttnArgs& a, int format, const void* scratch,
+int kv8_attention_check(const char* what, const kv8::Kv8AttnArgs& a, int format, const void* scratch,
                         size_t scratch_bytes, size_t need);
 // The pool as rows of 128 bytes (33 a tile: 16 of K, 16 of V, the scales); a box is K and V.
 bool make_kv8_tile_map(CUtensorMap* tm, const void* pool, long long rows);
