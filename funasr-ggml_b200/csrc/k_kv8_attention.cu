@@ -63,10 +63,11 @@ namespace {
 //   S[16 tokens][8 columns] = K . q     K expanded to f16 exactly; a query head is two columns,
 //                                       hi = f16(q') and lo = f16(q' - hi), q' = q scaled by a
 //                                       power of two to [1, 2): 22 bits of q
-//   softmax: lane (g, t) = (lane / 4, lane % 4) holds tokens g and g + 8 of head t; running
-//            maximum per head, sums per lane
+//   softmax: lane (g, t) = (lane / 4, lane % 4) holds tokens g and g + 8 of head t; sums per
+//            lane; the running maximum of a head stays until a score exceeds it by kLazy (log2
+//            units), which one vote a page finds out
 //   O[16 dims x 8][8 columns] += V^T . w   w = p dv as a hi / lo pair, scaled by a power of two
-//                                       that takes the page's largest dv to [2^10, 2^11)
+//                                       that takes the page's largest dv to [2^5, 2^6)
 // The page's product starts from zero and is added to the running output by one f32 fma per
 // value, so the sum over pages is rounded to nearest.
 //
@@ -75,12 +76,15 @@ namespace {
 // dependent loads) and of merge; without its arithmetic the kernel takes as long. 12 or 6 warps a
 // CTA took 98.6 and 98.9 us, grids of two to four waves 102 to 109, the merge inside the kernel
 // (arrival words) 101. Short calls are latency: the loads of the start, and 0.45 us a page and
-// warp (K's MMAs, softmax and V's depend on each other).
+// warp (K's MMAs, softmax and V's depend on each other). With eight query heads to a KV head long
+// batches are bound by issue: 256 rows of 2048 tokens on 4 KV heads 126 us (a copy's rate: 85); 142
+// with the maximum exchanged and O rescaled for every page.
 constexpr int kWarps = 4;
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = 148 * kCtasPerSm;     // one resident wave of a B200
 constexpr int kItemUnits = 2;                  // with ranges per warp: 16 ragged rows 25.6 -> 12.8 us
 
+constexpr float kLazy = 8.0f;                  // weights reach 2^(6 + kLazy)
 constexpr int kStages = 3;                     // 128 rows x 2048 tokens: 2 stages 97, 3 95, 4 98 us
 
 // Short contexts: a CTA per (row, KV head), whose warps share its pages evenly, needs no list and
@@ -440,27 +444,40 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? kCtasPerSm : 1)
             const float k0 = scale[g], k1 = scale[g + 8];
             const bool in0 = g < valid, in1 = g + 8 < valid;
             const float v0 = in0 ? scale[kPageTokens + g] : 0.0f, v1 = in1 ? scale[kPageTokens + g + 8] : 0.0f;
-            // the power of two at the page's largest V scale, over 2^10
+            // the power of two at the page's largest V scale, over 2^5
             const float back = __uint_as_float(
                 max(__reduce_max_sync(0xffffffffu, max(__float_as_uint(v0), __float_as_uint(v1)) & 0x7f800000u),
-                    11u << 23) - (10u << 23));
+                    11u << 23) - (5u << 23));
             const float inv = pow2_inverse(back);
             const float u0 = v0 * inv, u1 = v1 * inv;
-            uint32_t w0[NT], w1[NT];
-            float alpha[NT];
+            float s0[NT], s1[NT];
+            bool above = false;
 #pragma unroll
             for (int c = 0; c < NT; ++c) {
-                const float s0 = in0 ? (sc[c][0] + sc[c][1]) * (k0 * qs[c]) : -INFINITY;
-                const float s1 = in1 ? (sc[c][2] + sc[c][3]) * (k1 * qs[c]) : -INFINITY;
-                float top = fmaxf(s0, s1);
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                top = fmaxf(top, mx[c]);
-                alpha[c] = mx[c] == top ? 1.0f : exp2f(mx[c] - top);
-                mx[c] = top;
-                const float p0 = in0 ? exp2f(s0 - top) : 0.0f, p1 = in1 ? exp2f(s1 - top) : 0.0f;
-                sum[c] = sum[c] * alpha[c] + (p0 + p1);
+                s0[c] = in0 ? (sc[c][0] + sc[c][1]) * (k0 * qs[c]) : -INFINITY;
+                s1[c] = in1 ? (sc[c][2] + sc[c][3]) * (k1 * qs[c]) : -INFINITY;
+                above |= fmaxf(s0[c], s1[c]) > mx[c] + kLazy;
+            }
+            if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                for (int c = 0; c < NT; ++c) {
+                    float top = fmaxf(s0[c], s1[c]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    top = fmaxf(top, mx[c]);
+                    const float alpha = mx[c] == top ? 1.0f : exp2f(mx[c] - top);
+                    mx[c] = top;
+                    sum[c] *= alpha;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[c][k] *= alpha;
+                }
+            }
+            uint32_t w0[NT], w1[NT];
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const float p0 = in0 ? ex2(s0[c] - mx[c]) : 0.0f, p1 = in1 ? ex2(s1[c] - mx[c]) : 0.0f;
+                sum[c] += p0 + p1;
                 w0[c] = hi_lo(in0 ? p0 * u0 : 0.0f);
                 w1[c] = hi_lo(in1 ? p1 * u1 : 0.0f);
             }
@@ -504,8 +521,8 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? kCtasPerSm : 1)
                         mma16816(acc, fa, wb[c][0], wb[c][1]);
                         float& oa = o[c][4 * d + e];
                         float& ob = o[c][4 * d + e + 1];
-                        oa = fmaf(acc[0] + acc[1], back, oa * alpha[c]);
-                        ob = fmaf(acc[2] + acc[3], back, ob * alpha[c]);
+                        oa = fmaf(acc[0] + acc[1], back, oa);
+                        ob = fmaf(acc[2] + acc[3], back, ob);
                     }
                 }
             }

@@ -51,6 +51,13 @@ __device__ __forceinline__ float pow2_floor(float x) {
 }
 __device__ __forceinline__ float pow2_inverse(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
 
+// 2^x, results below 2^-126 as zero: weights of a softmax.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // N consecutive outputs from offset o, a multiple of 4.
 template <int N>
 __device__ __forceinline__ void store_values(const Kv8AttnArgs& a, size_t o, const float (&v)[N]) {

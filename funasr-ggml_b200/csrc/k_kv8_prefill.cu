@@ -118,12 +118,6 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
     lo = pack2(__fsub_rn(a, f.x), __fsub_rn(b, f.y));
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // One lane of a converged warp.
 __device__ __forceinline__ uint32_t elect_one() {
     uint32_t one;

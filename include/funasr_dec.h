@@ -442,7 +442,8 @@ FA_API int fa_op_kv8_gather(const void* pool_dev, int format, int n_layers, int 
  * aligned, of any content; calls that overlap on the GPU (captured graphs that run at the same
  * time among them) need scratch of their own. A position below -1 or past the block-table row
  * or a negative slot sets error bit 8 and that row is not written; a page outside the pool sets
- * bit 2 and its tokens are left out. bt_stride is limited to 2^26 pages. */
+ * bit 2 and its tokens are left out. bt_stride is limited to 2^26 pages. Sums are f32; an error
+ * is relative to the largest |V| that the row attends to (some 2^-20 of it). */
 FA_API size_t fa_op_attention_kv8_scratch_bytes(int M, int n_heads, int n_kv_heads);
 FA_API int fa_op_paged_attention_kv8(const float* q_dev, int M, int n_heads, int n_kv_heads, const int* pos_dev,
                                      const int* slot_dev, const int* block_table_dev, int bt_stride, int n_pages,

@@ -538,6 +538,35 @@ def test_nan_vectors_reach_their_own_rows_only(torch_cuda, fmt, which):
     assert np.array_equal(nan, want)
 
 
+@pytest.mark.parametrize("step", [0.05, 0.4, 3.0, -0.05, -0.4, -3.0])
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_scores_that_rise_or_fall_along_the_context(torch_cuda, fmt, which, step):
+    """Score t is step * t of the row's largest length and a little noise: the running maximum
+    rises by less and by more than what a kernel may leave it behind, or is the first score."""
+    torch = torch_cuda
+    rng = np.random.default_rng(17)
+    hq, hkv, n, M = 16, 8, 333, 12
+    pool, bt, n_pages = _filled(rng, [n], 1, hkv, fmt)
+    raw, scales = P.parts(pool)
+    way = rng.choice([-1.0, 1.0], 128)
+    t = np.arange(n)
+    k = way * (step * t / 128)[:, None] + 0.002 * rng.standard_normal((hkv, n, 128)) * max(abs(step), 0.1)
+    qk, dk = P.quantise(k.astype(np.float32), fmt)
+    raw[0, bt[0, t // 16], :, 0, t % 16] = qk.transpose(1, 0, 2)
+    scales[0, bt[0, t // 16], :, 0, t % 16] = dk.T
+    q = (way + 0.01 * rng.standard_normal((M, hq, 128))).astype(np.float32)
+    pos = np.arange(n - M, n).astype(np.int32)
+    args = (torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, np.zeros(M, np.int32)), dev(torch, bt), n_pages,
+            fmt, dev(torch, pool))
+    err = _err(torch)
+    got = (_decode(*args, err) if which == "decode" else _prefill(*args, _tiles([(0, M)], 64), err)).cpu().numpy()
+    assert int(err) == 0
+    for m in range(M):
+        kk, v = (x[0] for x in P.read(pool, bt[0], 0, pos[m] + 1, fmt))
+        assert np.abs(got[m] - P.attention(q[m], kk, v).reshape(-1)).max() <= _bound(q[m], kk, v), m
+
+
 @pytest.mark.parametrize("base,M", [(0, 70), (37, 64), (500, 100), (1000, 20)])
 @pytest.mark.parametrize("which", ["decode", "prefill"])
 @pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
