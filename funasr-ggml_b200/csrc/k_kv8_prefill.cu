@@ -186,17 +186,17 @@ __device__ __forceinline__ int part_blocks(int nb, int max_parts, int part, int&
 // By one warp: the last key that the rows of a tile attend to (-1: none) and their slot, the
 // one of the row that attends furthest.
 __device__ __forceinline__ int tile_extent(const Kv8AttnArgs& a, int2 tile, int lane, int& slot) {
-    int best = -1, row = 0;
+    int best = -1, of = 0;
     for (int r = lane; r < tile.y; r += 32) {
-        const int m = tile.x + r;
-        if (!row_bad(a, m) && a.pos[m] > best) {
-            best = a.pos[m];
-            row = m;
+        const int m = tile.x + r, pos = a.pos[m], at = a.slot[m];
+        if (!row_bad(a, m) && pos > best) {
+            best = pos;
+            of = at;
         }
     }
     const int last = __reduce_max_sync(0xffffffffu, best);
-    const int who = __ffs(__ballot_sync(0xffffffffu, best == last)) - 1;
-    slot = last >= 0 ? a.slot[__shfl_sync(0xffffffffu, row, who)] : 0;
+    of = __shfl_sync(0xffffffffu, of, __ffs(__ballot_sync(0xffffffffu, best == last)) - 1);
+    slot = last >= 0 ? of : 0;
     return last;
 }
 __device__ __forceinline__ bool tile_bad(const Kv8AttnArgs& a, int2 tile) {
@@ -300,8 +300,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int2 tile = a.tiles[blockIdx.y];
     const bool bad = tile_bad(a, tile);
     // warps 8-15: 16 query vectors each, lane l dims [4 l, 4 l + 4); vectors without a row are zero
-    float4 qv[16];
+    // (thread t of each four warps looks after vector t later)
+    const int my_r = (threadIdx.x & 127) % R, my_head = (threadIdx.x & 127) / R;
+    int my_pos = 0, my_slot = 0;
+    bool my_bad = false;
+    unsigned char* stage = reinterpret_cast<unsigned char*>(S.k[TILES - 1][0]);
+    unsigned char* stage2 = reinterpret_cast<unsigned char*>(S.v[TILES - 1][0]);
     if (warp >= 8) {
+        float4 qv[16];
         int head = (warp - 8) * 16 / R, r = (warp - 8) * 16 - head * R;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
@@ -313,18 +319,48 @@ __global__ void __launch_bounds__(THREADS, 1)
                 ++head;
             }
         }
+        if (my_head < G && my_r < tile.y && !bad) {
+            my_pos = a.pos[tile.x + my_r];
+            my_slot = a.slot[tile.x + my_r];
+            my_bad = row_bad(a, tile.x + my_r);
+        }
+        // Q as a pair: low parts to shared memory as they are, high parts by way of the last tile
+        // of the f16 ring, since a lane writes a whole row of TMEM
+        const int hf = lane >> 4, chunk = (lane & 15) >> 1;
+        const uint32_t sub = (uint32_t)(lane & 1) * 8;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int v = (warp - 8) * 16 + k;
+            const float4 x = qv[k];
+            const float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+            const float p2 = pow2_floor(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))));
+            const float up = pow2_inverse(p2);
+            uint2 hi, lo;
+            split2(x.x * up, x.y * up, hi.x, lo.x);
+            split2(x.z * up, x.w * up, hi.y, lo.y);
+            const uint32_t off = sw128(v, chunk) + sub;
+            *reinterpret_cast<uint2*>((hf ? stage2 : stage) + off) = hi;
+            *reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(S.q_lo[hf]) + off) = lo;
+            if (lane == 0) S.qs[v] = p2 * kLog2e;
+        }
     }
-    if (warp == 2) {
+    if (warp == 0) {
         int slot = 0;
-        const int last = bad ? -1 : tile_extent(a, tile, lane, slot);
+        const int pos_last = bad ? -1 : tile_extent(a, tile, lane, slot);
         if (lane == 0) {
-            S.pos_last = last;
+            S.pos_last = pos_last;
             S.slot = slot;
         }
     }
     if (bad && threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.z == 0) record_error(a.err, kDevErrBadPos);
+    // warp 0 goes on to the copies without waiting for the others
     tc_fence_before();
-    __syncthreads();
+    if (warp == 0) {
+        __syncwarp();
+        asm volatile("bar.arrive 2, 512;" ::: "memory");
+    } else {
+        asm volatile("bar.sync 2, 512;" ::: "memory");
+    }
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, S.tmem_base, 0);
     const int pos_last = S.pos_last, slot = S.slot;
@@ -339,23 +375,21 @@ __global__ void __launch_bounds__(THREADS, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         if (idle) {
         } else if (warp == 0) {
-            const int* bt = a.block_table + (size_t)slot * a.bt_stride;
-            const int last_page = pos_last / kPageTokens;
             bool ok = true;
             int ids = 0;                                   // lane l: page 32 b + l of the part
-            for (int j = 0; ok && j < n_blocks; ++j) {
+            for (int j = 0; j < n_blocks; ++j) {
+                if (j >= RAW)
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.raw_empty[j % RAW], (uint32_t)(j / RAW - 1) & 1u));
+                if (!ok) break;
                 if ((j & 7) == 0) {
-                    const int p = (first + j) * PAGES + lane;
-                    ids = p <= last_page ? bt[p] : -1;
+                    const int p = (first + j) * PAGES + lane, last_page = pos_last / kPageTokens;
+                    ids = p <= last_page ? a.block_table[(size_t)slot * a.bt_stride + p] : -1;
                     if (p <= last_page && (ids < 0 || ids >= a.n_pages)) {
-                        ids = -1;                          // its tokens are left out
+                        ids = -1;                              // its tokens are left out
                         record_error(a.err, kDevErrBadPage);
                     }
                 }
                 const int s = j % RAW;
-                if (j >= RAW)
-                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&S.raw_empty[s], (uint32_t)(j / RAW - 1) & 1u));
-                if (!ok) break;
                 int id[PAGES], have = 0;
 #pragma unroll
                 for (int q = 0; q < PAGES; ++q) {
@@ -532,42 +566,18 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int odd = warp >= 12 ? 1 : 0;
             const int quarter = warp & 3;
             const int t = 32 * quarter + lane;
-            const int r = t % R, head = t / R;
-            const int row = tile.x + r;
-            bool live = head < G && r < tile.y;
-            int pos = pos_last;                            // lanes without a row mask no more than the others
+            bool live = my_head < G && my_r < tile.y;
+            int pos = pos_last;                        // lanes without a row mask no more than the others
             if (live) {
-                pos = a.pos[row];
-                if (row_bad(a, row) || (pos >= 0 && a.slot[row] != slot)) {
-                    if (h == 0 && blockIdx.z == 0 && head == 0 && !odd) record_error(a.err, kDevErrBadLen);
+                pos = my_pos;
+                if (my_bad || (pos >= 0 && my_slot != slot)) {
+                    if (h == 0 && blockIdx.z == 0 && my_head == 0 && !odd) record_error(a.err, kDevErrBadLen);
                     live = false;
                     pos = pos_last;
                 }
             }
             const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16);
             if (n_blocks > 0) {
-                // Q as a pair: low parts to shared memory as they are, high parts by way of the last tile
-                // of the f16 ring, since a lane writes a whole row of TMEM
-                unsigned char* stage = reinterpret_cast<unsigned char*>(S.k[TILES - 1][0]);
-                unsigned char* stage2 = reinterpret_cast<unsigned char*>(S.v[TILES - 1][0]);
-                const int hf = lane >> 4, chunk = (lane & 15) >> 1;
-                const uint32_t sub = (uint32_t)(lane & 1) * 8;
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const int v = (warp - 8) * 16 + k;
-                    const float4 x = qv[k];
-                    const float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-                    const float p2 = pow2_floor(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))));
-                    const float up = pow2_inverse(p2);
-                    uint2 hi, lo;
-                    split2(x.x * up, x.y * up, hi.x, lo.x);
-                    split2(x.z * up, x.w * up, hi.y, lo.y);
-                    const uint32_t off = sw128(v, chunk) + sub;
-                    *reinterpret_cast<uint2*>((hf ? stage2 : stage) + off) = hi;
-                    *reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(S.q_lo[hf]) + off) = lo;
-                    if (lane == 0) S.qs[v] = p2 * kLog2e;
-                }
-                group_sync();
                 // each group writes half of the dims
                 uint32_t row_hi[32];
 #pragma unroll
@@ -752,21 +762,27 @@ __global__ void __launch_bounds__(THREADS, 1)
             group_sync();
             if (!S.err) {
                 const int v0 = (warp - 8) * 16;
-                const size_t part_at = part_index(a, blockIdx.y, h, max_parts, blockIdx.z);
+                const uint32_t lives = __ballot_sync(0xffffffffu, S.live[v0 + (lane & 15)] != 0);
+                float4* to_part = reinterpret_cast<float4*>(part_o + (at - t + v0) * D) + lane;
                 int vh = v0 / R, vr = v0 - vh * R;
-#pragma unroll 4
-                for (int k = 0; k < 16; ++k) {
-                    const int v = v0 + k;
-                    const float4 o = *reinterpret_cast<const float4*>(stage + v * 512 + ((lane ^ (v & 7)) << 4));
-                    if (parts > 1) {
-                        reinterpret_cast<float4*>(part_o + (part_at + v) * D)[lane] = o;
-                    } else if (S.live[v]) {
-                        const float x[4] = {o.x, o.y, o.z, o.w};
-                        store_values<4>(a, ((size_t)(tile.x + vr) * a.Hq + h * G + vh) * D + 4 * lane, x);
-                    }
-                    if (++vr == R) {
-                        vr = 0;
-                        ++vh;
+#pragma unroll 1
+                for (int k0 = 0; k0 < 16; k0 += 8) {
+                    float4 o[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        o[k] = *reinterpret_cast<const float4*>(stage + (v0 + k0 + k) * 512 + ((lane ^ k) << 4));
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        if (parts > 1) {
+                            to_part[(k0 + k) * (D / 4)] = o[k];
+                        } else if ((lives >> (k0 + k)) & 1) {
+                            const float x[4] = {o[k].x, o[k].y, o[k].z, o[k].w};
+                            store_values<4>(a, ((size_t)(tile.x + vr) * a.Hq + h * G + vh) * D + 4 * lane, x);
+                        }
+                        if (++vr == R) {
+                            vr = 0;
+                            ++vh;
+                        }
                     }
                 }
             }
