@@ -29,9 +29,9 @@
 // second products twice those of plain f16) and the kernel about 1500: the way from S over the
 // softmax to O is longer than the MMAs between, and a rescale or a late page on it is not made up
 // for. 4 chunks of 417 to 512 rows at 3500 tokens (16 query heads on 8, 248 CTAs of one SM each)
-// take 120 us; 300 with one softmax group, 174 with two S buffers, 142 to 155 with masked and
+// take 119 us; 300 with one softmax group, 174 with two S buffers, 142 to 155 with masked and
 // whole blocks in one pass, 146 with each block halved between the groups (ten rescales a warp,
-// each on the way of the next product). A chunk of 112 rows takes 13.9 us.
+// each on the way of the next product). A chunk of 112 rows takes 13.3 us.
 // A persistent form with an even split of the blocks took 160 and 26: every change of tile costs
 // 10 us of queries, joins and output, which separate CTAs overlap.
 #include "k_attn_body.cuh"
