@@ -6,9 +6,10 @@
 // vectors (vector v = row v % R, head v / R) are the M side of every MMA, so a page is read and
 // expanded to f16 once for all of them. Per block of 64 keys (4 pages):
 //   S  = Q . K^T        tcgen05.mma kind::f16, M 128, N 64, K 128; Q as the pair hi = f16(q'),
-//                       lo = f16(q' - hi), q' = q scaled by a power of two to [1, 2): 22 bits
-//   p  = exp2(dk S - m) one query vector per thread; w = p dv / sigma, sigma a power of two under
-//                       the largest dv that the row has seen: f16 pairs, written over S in TMEM
+//                       lo = f16(q' - hi), q' = q log2(e) / qs, qs the power of two that takes the
+//                       largest to [0.72, 1.44): 22 bits
+//   p  = exp2(qs (dk S - m))  one query vector per thread; w = p dv / sigma, sigma a power of two
+//                       under the largest dv that the row has seen: f16 pairs, written over S in TMEM
 //   O += w . V          M 128, N 128 (dims), K 64 (keys), V MN-major
 // A pair's rounding is 2^-25 at most, against 4 or more for the largest V at the running maximum:
 // an output is off by 2^-27 a key, as they fall together much less, of the largest |V| that its
@@ -16,7 +17,8 @@
 // w and Q's high parts, the A operands of three quarters of the MMAs, are in TMEM: with all of Q
 // and w in shared memory a block would read 128 KB of it for its MMAs, against 1024 cycles that
 // they take. The running maximum is lazy: O is rescaled when a block exceeds it by 2^kLazy or
-// sigma grows.
+// sigma grows. qs is a power of two so that qs m is exact: rounded by itself, the maximum of scores
+// of 1e8 and more would lie several log2 units from the scores that it is taken off.
 //
 // Roles (512 threads): warp 0 issues the page copies (one TMA box and one bulk copy of scales
 // per page) into a ring of raw blocks; warps 4-7 expand a raw block into the f16 K / V tiles of
@@ -79,7 +81,7 @@ struct PfSmem {
     float dv_raw[TILES][KB];                  // V scales, for the others
     float sigma[TILES];                       // of all keys up to the block's last
     int live[128];                            // the query vector has a row that can be served
-    float qs[128];                            // what takes dk S of a query vector to log2 units
+    float qs[128];                            // the power of two that takes dk S of a query vector to log2 units
     float state[2][3][128];                   // even / odd blocks' maximum, sum and sigma of each vector
     int raw_pages[RAW];                       // bit q: page q of the block was copied
     int pages[TILES];
@@ -209,6 +211,12 @@ __host__ __device__ inline size_t part_index(const Kv8AttnArgs& a, int tile, int
     return (((size_t)tile * a.Hkv + h) * parts + part) * 128;
 }
 
+// A maximum in log2 units: exact, or NaN (as the outputs are then) where a score passes f32's range.
+__device__ __forceinline__ float in_log2(float top, float qs) {
+    const float x = __fmul_rn(top, qs);
+    return x == INFINITY ? NAN : x;
+}
+
 // The second pass over a block's scores (dk S in sv): p = exp2(dk S qs - top2), whose sum is
 // returned, and the weights p f (f: V scales over sigma, times `more` where MASKED) as f16 pairs
 // to TMEM over S, the first 32 keys' announced at half_bar. Keys not in `seen` weigh nothing: by
@@ -334,14 +342,14 @@ __global__ void __launch_bounds__(THREADS, 1)
             const float4 x = qv[k];
             const float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
             const float p2 = pow2_floor(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))));
-            const float up = pow2_inverse(p2);
+            const float up = 0.5f * kLog2e * pow2_inverse(p2);
             uint2 hi, lo;
             split2(x.x * up, x.y * up, hi.x, lo.x);
             split2(x.z * up, x.w * up, hi.y, lo.y);
             const uint32_t off = sw128(v, chunk) + sub;
             *reinterpret_cast<uint2*>((hf ? stage2 : stage) + off) = hi;
             *reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(S.q_lo[hf]) + off) = lo;
-            if (lane == 0) S.qs[v] = p2 * kLog2e;
+            if (lane == 0) S.qs[v] = 2.0f * p2;
         }
     }
     if (warp == 0) {
@@ -673,10 +681,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                     sigma = next_sigma;
                     if (top == -INFINITY) {
                         top = bmax + room;                     // first block with a key: O holds nothing of this row
-                        top2 = __fmul_rn(top, qs);
+                        top2 = in_log2(top, qs);
                     } else if (bmax > top + lazy) {
                         top = bmax + room;
-                        const float next = __fmul_rn(top, qs);
+                        const float next = in_log2(top, qs);
                         const float f = exp2f(top2 - next);
                         top2 = next;
                         alpha *= f;

@@ -443,7 +443,10 @@ FA_API int fa_op_kv8_gather(const void* pool_dev, int format, int n_layers, int 
  * time among them) need scratch of their own. A position below -1 or past the block-table row
  * or a negative slot sets error bit 8 and that row is not written; a page outside the pool sets
  * bit 2 and its tokens are left out. bt_stride is limited to 2^26 pages. Sums are f32; an error
- * is relative to the largest |V| that the row attends to (some 2^-20 of it). */
+ * is relative to the largest |V| that the row attends to (some 2^-20 of it). A score is off by
+ * some 2^-22 of its sum of |q k|: that much, where scores are large, is the difference between
+ * two tokens. Scores, 2^8 times the largest |K| and 2^11 times the largest |V| times the row's
+ * tokens have to stay within f32's range; a row whose largest score passes it is NaN. */
 FA_API size_t fa_op_attention_kv8_scratch_bytes(int M, int n_heads, int n_kv_heads);
 FA_API int fa_op_paged_attention_kv8(const float* q_dev, int M, int n_heads, int n_kv_heads, const int* pos_dev,
                                      const int* slot_dev, const int* block_table_dev, int bt_stride, int n_pages,

@@ -998,3 +998,94 @@ def test_two_decode_calls_on_two_streams(torch_cuda):
     for a, b in zip(alone, outs):
         assert torch.equal(a, b)
     assert int(err) == 0
+
+
+# ------------------------------------------------------------ large scores --
+def _one_hot_rows(got, q, pos, pool, bt, fmt):
+    """Checks got [M][Hq][128] of rows whose scores are far larger than 1 (sequence 0): every
+    output is finite and within the values that its row attends to, and where the definition
+    gives the largest score all the weight, the output is that token's value. A score is off by
+    2^-18 of sum |q k| at most (see _bound), two of them by twice that; a lead of 40 beyond it
+    leaves the others e^-40 each. An output is then the weight's pair (2^-22), the division and
+    a few f32 roundings away from the value, and a pair's smallest step from that of the largest
+    V: 2^-20 of it together. Returns the share of (row, head)s with such a lead."""
+    M, hq, clear = len(q), q.shape[1], 0
+    for m in range(M):
+        k, v = (x[0] for x in P.read(pool, bt[0], 0, pos[m] + 1, fmt))
+        g = hq // len(k)
+        for h in range(hq):
+            kh, vh, qh = k[h // g], v[h // g], q[m, h].astype(np.float64)
+            tol = 2.0 ** -20 * np.abs(vh).max()
+            assert np.isfinite(got[m, h]).all(), (m, h)
+            assert (got[m, h] <= vh.max(0) + tol).all() and (got[m, h] >= vh.min(0) - tol).all(), (m, h)
+            s = kh @ qh
+            lead = np.sort(s)[-1] - np.sort(s)[-2] if len(s) > 1 else np.inf
+            if lead >= 2.0 ** -17 * (np.abs(kh) @ np.abs(qh)).max() + 40:
+                clear += 1
+                assert np.abs(got[m, h] - vh[s.argmax()]).max() <= tol, (m, h)
+    return clear / (M * hq)
+
+
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e7, 1e8, 3e8, 1e9, 1e10, 1e12, 1e20, 1e30])
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_large_scores(torch_cuda, fmt, which, size):
+    """Scores of 1e4 to 1e31: the maximum that a kernel takes off them is theirs, not a rounded one."""
+    torch = torch_cuda
+    rng = np.random.default_rng(31)
+    hq, hkv, n, M = 16, 8, 300, 20
+    pool, bt, n_pages = _filled(rng, [n], 1, hkv, fmt)
+    q = (rng.standard_normal((M, hq, 128)) * 0.3 * size).astype(np.float32)
+    pos = np.arange(n - M, n).astype(np.int32)
+    args = (torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, np.zeros(M, np.int32)), dev(torch, bt), n_pages,
+            fmt, dev(torch, pool))
+    err = _err(torch)
+    got = _decode(*args, err) if which == "decode" else _prefill(*args, _tiles([(0, M)], 64), err)
+    assert int(err) == 0
+    assert _one_hot_rows(got.cpu().numpy().reshape(M, hq, 128), q, pos, pool, bt, fmt) > 0.9
+
+
+@pytest.mark.parametrize("base,M", [(0, 70), (37, 64), (1000, 20)])
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_rows_that_see_large_keys_and_values(torch_cuda, fmt, which, base, M):
+    """K and V of 1e30 in the second half of a chunk, for the rows that attend to them."""
+    torch = torch_cuda
+    rng = np.random.default_rng(base + M)
+    hq, hkv, n = 16, 8, base + M
+    pool, bt, n_pages = _filled(rng, [n], 1, hkv, fmt)
+    _, scales = P.parts(pool)
+    late = np.arange(base + M // 2, n)
+    for part in (0, 1):
+        scales[0, bt[0, late // 16], :, part, late % 16] *= np.float32(1e30)
+    pos = np.arange(base, n).astype(np.int32)
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    args = (torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, np.zeros(M, np.int32)), dev(torch, bt), n_pages,
+            fmt, dev(torch, pool))
+    err = _err(torch)
+    got = _decode(*args, err) if which == "decode" else _prefill(*args, _tiles([(0, M)], 64), err)
+    assert int(err) == 0
+    at = np.arange(M // 2, M)
+    assert _one_hot_rows(got.cpu().numpy().reshape(M, hq, 128)[at], q[at], pos[at], pool, bt, fmt) > 0.8      # the first rows see few such keys
+
+
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_scores_past_f32_are_nan(torch_cuda, fmt, which):
+    """A row whose largest score passes f32's range has no finite answer, least of all zeros."""
+    torch = torch_cuda
+    rng = np.random.default_rng(32)
+    hq, hkv, n, M = 16, 8, 130, 4
+    pool, bt, n_pages = _filled(rng, [n], 1, hkv, fmt)
+    _, scales = P.parts(pool)
+    t = np.arange(n)
+    scales[0, bt[0, t // 16], :, 0, t % 16] *= np.float32(1e25)
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    q[:, ::2] *= np.float32(1e25)                                 # the even heads: scores of 1e50; the odd ones 1e25
+    pos = np.full(M, n - 1, np.int32)
+    args = (torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, np.zeros(M, np.int32)), dev(torch, bt), n_pages,
+            fmt, dev(torch, pool))
+    err = _err(torch)
+    got = (_decode(*args, err) if which == "decode" else _prefill(*args, _tiles([(0, M)], 64), err)).cpu().numpy()
+    got = got.reshape(M, hq, 128)
+    assert np.isnan(got[:, ::2]).all() and np.isfinite(got[:, 1::2]).all() and int(err) == 0
