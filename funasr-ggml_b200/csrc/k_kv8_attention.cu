@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? kCtasPerSm : 1)
             for (int c = 0; c < NT; ++c) {
                 s0[c] = in0 ? (sc[c][0] + sc[c][1]) * (k0 * qs[c]) : -INFINITY;
                 s1[c] = in1 ? (sc[c][2] + sc[c][3]) * (k1 * qs[c]) : -INFINITY;
-                above |= fmaxf(s0[c], s1[c]) > mx[c] + kLazy;
+                above |= fmaxf(s0[c], s1[c]) - mx[c] > kLazy;   // exact where it decides, which mx + kLazy is not
             }
             if (__any_sync(0xffffffffu, above)) {
 #pragma unroll

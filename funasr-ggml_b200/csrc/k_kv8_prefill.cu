@@ -682,7 +682,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (top == -INFINITY) {
                         top = bmax + room;                     // first block with a key: O holds nothing of this row
                         top2 = in_log2(top, qs);
-                    } else if (bmax > top + lazy) {
+                    } else if (bmax - top > lazy) {            // exact where it decides, which top + lazy is not
                         top = bmax + room;
                         const float next = in_log2(top, qs);
                         const float f = exp2f(top2 - next);

@@ -1089,3 +1089,32 @@ def test_scores_past_f32_are_nan(torch_cuda, fmt, which):
     got = (_decode(*args, err) if which == "decode" else _prefill(*args, _tiles([(0, M)], 64), err)).cpu().numpy()
     got = got.reshape(M, hq, 128)
     assert np.isnan(got[:, ::2]).all() and np.isfinite(got[:, 1::2]).all() and int(err) == 0
+
+
+@pytest.mark.parametrize("period", [16, 64, 128])
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_large_scores_that_rise_by_their_last_place(torch_cuda, fmt, which, period):
+    """Scores of 1e8, whose last place is 16 in log2 units, rising by it: a step is more than a
+    kernel may leave its running maximum behind, though the sum of the two may round to it."""
+    torch = torch_cuda
+    rng = np.random.default_rng(33)
+    hq, hkv, n, M = 16, 8, 1024, 20
+    pool, bt, n_pages = _filled(rng, [n], 1, hkv, fmt)
+    raw, scales = P.parts(pool)
+    t = np.arange(n)
+    # K: the largest stored value in dimension 0 alone, under scales that rise by one step of f32
+    top = 127.0 if fmt == P.INT8 else 448.0
+    raw[0, bt[0, t // 16], :, 0, t % 16] = 0
+    raw[0, bt[0, t // 16], :, 0, t % 16, 0] = 127 if fmt == P.INT8 else 126
+    d = (np.float32(1.03).view(np.int32) + (t + 40) // period).astype(np.int32).view(np.float32)
+    scales[0, bt[0, t // 16], :, 0, t % 16] = d[:, None]
+    q = np.zeros((M, hq, 128), np.float32)
+    q[..., 0] = np.linspace(0.94e8, 1.85e8, M * hq).reshape(M, hq) / (top * 1.03)      # in log2 units 2^27 to 2^28
+    pos = np.full(M, n - 1, np.int32)
+    args = (torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, np.zeros(M, np.int32)), dev(torch, bt), n_pages,
+            fmt, dev(torch, pool))
+    err = _err(torch)
+    got = _decode(*args, err) if which == "decode" else _prefill(*args, _tiles([(0, M)], 64), err)
+    assert int(err) == 0
+    _one_hot_rows(got.cpu().numpy().reshape(M, hq, 128), q, pos, pool, bt, fmt)
