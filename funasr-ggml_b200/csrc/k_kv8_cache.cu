@@ -10,6 +10,7 @@
 #include "funasr_dec.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <string>
 
@@ -181,9 +182,17 @@ __device__ __forceinline__ void load4(const float* vec, int lane, float (&x)[4])
 // and a rotation by 4, whose terms together reach sqrt(2) of it), so their bytes can differ from
 // those of the exact values only next to a border: where one lies within that distance (for int8
 // twice that and an ulp, since the scale is off by as much), the vector is computed again in 64
-// bits, a few vectors in a hundred.
+// bits, a few vectors in a hundred. So is one whose f32 values are not known that well: where a
+// square, their mean, a product or a rotation may have left f32's normal range.
 template <int FMT>
 constexpr float kKeyError = (FMT == kInt8 ? 23.5f : 12.5f) / (1 << 24);
+// Mean square and epsilon within 2^-120 .. 2^120: squares that are lost below 2^-149 then weigh
+// less than 2^-28 of the mean, and none of 128 reached 2^128.
+__device__ __forceinline__ bool norm_in_range(float scale) { return scale >= 0x1p-60f && scale <= 0x1p60f; }
+// The last place of a subnormal is 2^-49 of such a vector's largest, or less; that of a normalised
+// value is so once more, and then multiplied by a weight of at most w_max.
+__device__ __forceinline__ bool key_in_range(float amax) { return amax >= 0x1p-100f && amax <= FLT_MAX; }
+__device__ __forceinline__ bool weights_in_range(float w_max, float e) { return w_max <= e * 0x1p120f; }
 
 // pack4 of key values, unless a value that differs by e may round otherwise (near).
 template <int FMT>
@@ -202,7 +211,8 @@ __device__ __forceinline__ uint32_t pack_key(const float (&x)[4], float d, float
     return q;
 }
 
-// A key vector in 64 bits, by a warp: the lane's four stored bytes, and the scale.
+// A key vector in 64 bits, by a warp: the lane's four stored bytes, and the scale. A value that is
+// past f32's range counts as infinite.
 template <int FMT>
 __device__ __noinline__ uint32_t exact_key(const float* vec, int lane, const float* w, const float2* rot, float eps,
                                            float& d) {
@@ -213,6 +223,7 @@ __device__ __noinline__ uint32_t exact_key(const float* vec, int lane, const flo
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const double scale = rsqrt(ss * (1.0 / D) + (double)eps);
     double amax = 0.0;
+    bool finite = true;
 #pragma unroll
     for (int k = 0; k < 4; ++k) y[k] *= scale * (double)w[k];
 #pragma unroll
@@ -221,10 +232,15 @@ __device__ __noinline__ uint32_t exact_key(const float* vec, int lane, const flo
         y[k] = a * c - b * s;
         y[k + 2] = a * s + b * c;
         amax = fmax(amax, fmax(fabs(y[k]), fabs(y[k + 2])));
+        finite = finite && fabs(y[k]) <= FLT_MAX && fabs(y[k + 2]) <= FLT_MAX;
+    }
+    uint32_t q = 0;
+    if (!__all_sync(0xffffffffu, finite)) {
+        d = __uint_as_float(0x7fffffffu);
+        return q;
     }
 #pragma unroll 1
     for (int o = 16; o > 0; o >>= 1) amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    uint32_t q = 0;
     if (FMT == kInt8) {
         d = fmaxf(__double2float_rn(amax / 127.0), kMinScale);
         const double inv = 1.0 / (double)d;
@@ -280,6 +296,7 @@ __global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
     const int page =
         stores ? token_page(a.block_table, a.bt_stride, a.n_pages, a.slot[m], pos, a.err, lane == 0) : -1;
     float scale[V];
+    uint32_t far;                                                 // bit 8 u: not norm_in_range
     if (V == 4) {
         double two[2];
 #pragma unroll
@@ -291,6 +308,7 @@ __global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const float mine = norm_scale(ss, a.eps);                 // lane l: vector l / 8
+        far = __ballot_sync(0xffffffffu, !norm_in_range(mine));
 #pragma unroll
         for (int u = 0; u < V; ++u) scale[u] = __shfl_sync(0xffffffffu, mine, 8 * u);
     } else {
@@ -298,6 +316,7 @@ __global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         scale[0] = norm_scale(ss, a.eps);
+        far = !norm_in_range(scale[0]);
     }
     uint32_t top = 0;                                             // lane l: of the warp's stored vector l % V
 #pragma unroll
@@ -321,11 +340,11 @@ __global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
     if (page < 0) return;
     const float d_mine = scale_of<FMT>(top), inv_mine = __frcp_rn(d_mine);
     const float amax_mine = __uint_as_float(top), e_mine = amax_mine * kKeyError<FMT>;
-    // e4m3 scales that the error of the largest value may change
-    const uint32_t unsure =
-        FMT == kInt8 ? 0u
-                     : __ballot_sync(0xffffffffu, scale_of<FMT>(__float_as_uint(amax_mine + e_mine)) !=
-                                                      scale_of<FMT>(__float_as_uint(amax_mine - e_mine)));
+    // keys out of range, and e4m3 scales that the error of the largest value may change
+    const uint32_t unsure = __ballot_sync(
+        0xffffffffu, !key_in_range(amax_mine) || (FMT != kInt8 && scale_of<FMT>(__float_as_uint(amax_mine + e_mine)) !=
+                                                                      scale_of<FMT>(__float_as_uint(amax_mine - e_mine))));
+    const float w_max = fmaxf(fmaxf(fabsf(kw[0]), fabsf(kw[1])), fmaxf(fabsf(kw[2]), fabsf(kw[3])));   // the lane's
     const int t = pos % kPageTokens;
 #pragma unroll
     for (int u = 0; u < V; ++u) {
@@ -336,15 +355,15 @@ __global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
         float d = __shfl_sync(0xffffffffu, d_mine, u);
         const float inv = __shfl_sync(0xffffffffu, inv_mine, u);
         uint32_t q = 0;
-        if (d == d) {
-            if (part == 0) {
-                bool near;
-                q = pack_key<FMT>(x[u], d, inv, __shfl_sync(0xffffffffu, e_mine, u), near);
-                if (((unsure >> u) & 1) || __any_sync(0xffffffffu, near))
-                    q = exact_key<FMT>(a.qkv + ((size_t)m * n_vec + j) * D, lane, kw, rot, a.eps, d);
-            } else {
-                q = pack4<FMT>(x[u], d, inv);
-            }
+        if (part == 0) {
+            bool near;
+            const float e = __shfl_sync(0xffffffffu, e_mine, u);
+            q = pack_key<FMT>(x[u], d, inv, e, near);
+            near = near || !weights_in_range(w_max, e);
+            if (((unsure >> u | far >> 8 * u) & 1) || __any_sync(0xffffffffu, near))
+                q = exact_key<FMT>(a.qkv + ((size_t)m * n_vec + j) * D, lane, kw, rot, a.eps, d);
+        } else if (d == d) {
+            q = pack4<FMT>(x[u], d, inv);
         }
         unsigned char* tile = a.pool + ((size_t)page * a.Hkv + h) * kTileBytes;
         uint16_t* dst = reinterpret_cast<uint16_t*>(tile + part * kPartBytes + t * D) + lane;

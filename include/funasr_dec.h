@@ -418,8 +418,9 @@ FA_API int fa_op_kv8_append(const void* k_dev, const void* v_dev, int src_type, 
                             int* err_dev, void* stream);
 /* Kernel (1) with an 8-bit end: fa_op_qknorm_rope_append with qkv [M][n_heads + 2 n_kv_heads][128],
  * q_out [M][n_heads][128] in the same f32 arithmetic. K's stored bytes are those of the norm
- * and rotation in 64 bits, rounded once (its int8 scale is within 2^-20 of theirs); V is
- * quantised as it is. qkv, rope and q_out 16-byte, the norm weights 8-byte aligned. Errors as
+ * and rotation in 64 bits, rounded once (its int8 scale is within 2^-20 of theirs), also where
+ * the f32 arithmetic would overflow on the way; a result past f32's range counts as an infinity.
+ * V is quantised as it is. qkv, rope and q_out 16-byte, the norm weights 8-byte aligned. Errors as
  * for the raw append; a position past the rotation table sets bit 4 too. */
 FA_API int fa_op_qknorm_rope_append_kv8(const float* qkv_dev, int M, int n_heads, int n_kv_heads, const int* pos_dev,
                                         const int* slot_dev, const int* block_table_dev, int bt_stride, int n_pages,

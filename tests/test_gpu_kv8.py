@@ -1118,3 +1118,47 @@ def test_large_scores_that_rise_by_their_last_place(torch_cuda, fmt, which, peri
     got = _decode(*args, err) if which == "decode" else _prefill(*args, _tiles([(0, M)], 64), err)
     assert int(err) == 0
     _one_hot_rows(got.cpu().numpy().reshape(M, hq, 128), q, pos, pool, bt, fmt)
+
+
+# -------------------------------------------------- keys of any magnitude --
+@pytest.mark.parametrize("eps,size", [(1e-5, 1.0), (0.0, 1.0), (1e-5, 1e-37), (1e-5, 3e37), (1e-5, 3e38)])
+@pytest.mark.parametrize("M", [100, 600])                         # a key vector a warp, and several
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_qknorm_rope_append_keys_of_any_magnitude(torch_cuda, fmt, M, eps, size):
+    """K's bytes are those of 64 bits where f32 squares overflow or vanish, where the norm weights
+    take the values next to f32's limits, and for zero, infinite and NaN vectors."""
+    torch = torch_cuda
+    rng = np.random.default_rng(M)
+    hq, hkv, max_pos, eps = 1, 8, 640, np.float32(eps)
+    qkv = _vectors(rng, M, hq + 2 * hkv)
+    mag = 10.0 ** rng.uniform(-42, 36, (M, hkv, 1))
+    qkv[:, hq:hq + hkv] = (qkv[:, hq:hq + hkv] * mag).astype(np.float32)
+    qkv[1, hq], qkv[2, hq + 1, 5], qkv[3, hq + 2, 100], qkv[4, hq + 3, 0] = 0, np.inf, np.nan, -np.inf
+    qkv[5, hq + 4] = np.finfo(np.float32).max
+    kn = (rng.uniform(0.8, 1.1, 128) * size).astype(np.float32)
+    assert np.isfinite(kn).all()
+    rope = np.asarray(oracle.rope_table(max_pos), np.float32).reshape(max_pos, 64, 2)
+    pos, n_pages = np.arange(M, dtype=np.int32), max_pos // 16
+    bt = rng.permutation(n_pages).astype(np.int32)[None]
+    pool, err = torch.zeros((1, n_pages, hkv, P.TILE), dtype=torch.uint8, device="cuda"), _err(torch)
+    q = torch.zeros((M, hq, 128), device="cuda")
+    d = [dev(torch, a) for a in (qkv, pos, np.zeros(M, np.int32), bt, np.ones(128, np.float32), kn, rope)]
+    p = [x.data_ptr() for x in d]
+    fa_dec.op_qknorm_rope_append_kv8(p[0], M, hq, hkv, p[1], p[2], p[3], n_pages, n_pages, p[4], p[5], float(eps),
+                                     p[6], max_pos, fmt, pool.data_ptr(), q.data_ptr(), err.data_ptr(),
+                                     _stream(torch))
+    with np.errstate(all="ignore"):
+        y = P.norm_rotate_exact(qkv[:, hq:hq + hkv], kn, rope[:M], eps)
+    y = np.where(np.abs(y) > np.finfo(np.float32).max, np.inf, y)
+    want, d_want = P.quantise(np.where(np.isnan(y), np.inf, y), fmt)
+    raw, scales = P.parts(pool.cpu().numpy())
+    at = bt[0, pos // 16], pos % 16
+    got, d_got = raw[0, at[0], :, 0, at[1]], scales[0, at[0], :, 0, at[1]]
+    assert np.array_equal(np.isnan(d_got), np.isnan(d_want)) and np.isnan(d_want).any() and not np.isnan(d_want).all()
+    assert np.array_equal(got, want)
+    live = ~np.isnan(d_want)
+    off = np.abs(d_got[live].astype(np.float64) - d_want[live])
+    assert (off <= d_want[live].astype(np.float64) * (2.0 ** -20 if fmt == P.INT8 else 0)).all()
+    v, d_v = P.quantise(qkv[:, hq + hkv:], fmt)
+    assert np.array_equal(raw[0, at[0], :, 1, at[1]], v) and np.array_equal(scales[0, at[0], :, 1, at[1]], d_v)
+    assert int(err) == 0
