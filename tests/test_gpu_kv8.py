@@ -1162,3 +1162,145 @@ def test_qknorm_rope_append_keys_of_any_magnitude(torch_cuda, fmt, M, eps, size)
     v, d_v = P.quantise(qkv[:, hq + hkv:], fmt)
     assert np.array_equal(raw[0, at[0], :, 1, at[1]], v) and np.array_equal(scales[0, at[0], :, 1, at[1]], d_v)
     assert int(err) == 0
+
+
+# -------------------------------------------------- forms of the large calls --
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("src_type,layers,hkv,M", [(P.F16, 4, 8, 300), (P.F32, 3, 11, 300), (P.BF16, 1, 5, 2000),
+                                                   (P.F32, 28, 8, 45), (P.BF16, 2, 8, 601), (P.F16, 1, 1, 9500)])
+def test_append_of_many_vectors(torch_cuda, fmt, src_type, layers, hkv, M):
+    """Calls in which a warp takes several (layer, head) pairs: rows whose pairs do not fill a warp,
+    padding, a bad position and a bad page among them; bytes and error bits in full."""
+    torch = torch_cuda
+    rng = np.random.default_rng(M)
+    n_pages = -(-M // 16) + 2
+    bt = rng.permutation(n_pages)[:-(-M // 16)].astype(np.int32)[None]
+    pos, kb = rng.permutation(M).astype(np.int32), bt.copy()
+    want = pos.copy()
+    pos[[1, M // 2]] = want[[1, M // 2]] = -1
+    pos[M - 1], want[M - 1] = -7, -1
+    kb[0, 1] = n_pages
+    want[(want >= 16) & (want < 32)] = -1
+    ld, n = 2 * layers * hkv * 128 + 64, layers * hkv * 128
+    x = np.zeros((M, ld), np.float32)
+    x[:, :n], x[:, n:2 * n] = _vectors(rng, M, layers * hkv).reshape(M, n), _vectors(rng, M, layers * hkv).reshape(M, n)
+    x[0, :128], x[M // 3, n + 5] = 0, 1000
+    d_x, x = _src(torch, x, src_type)
+    k, v = (x[:, i * n:(i + 1) * n].reshape(M, layers, hkv, 128) for i in (0, 1))
+    pool, slot = _garbage_pool(rng, layers, n_pages, hkv), np.zeros(M, np.int32)
+    d_pool, d_err = dev(torch, pool), _err(torch)
+    _append(torch, d_x, d_x[:, n:], src_type, ld, M, layers, hkv, dev(torch, pos), dev(torch, slot), dev(torch, kb),
+            n_pages, fmt, d_pool, d_err)
+    P.write(pool, bt, slot, want, k, v, fmt)
+    assert np.array_equal(d_pool.cpu().numpy(), pool)
+    assert int(d_err) == 2 | 4
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,M", [(16, 8, 400), (12, 4, 500), (5, 5, 700), (16, 2, 480), (1, 1, 3200), (3, 1, 1999)])
+def test_qknorm_rope_append_of_many_rows(torch_cuda, fmt, hq, hkv, M):
+    """Calls in which a warp takes several head vectors: warps of queries, of keys, of values and
+    mixed ones; q_out, bytes, scales, padding and error bits in full."""
+    torch = torch_cuda
+    rng = np.random.default_rng(hq * 100 + M)
+    max_pos = -(-M // 16) * 16 + 16
+    n_pages = max_pos // 16 + 3
+    qkv = _vectors(rng, M, hq + 2 * hkv) * 2
+    qkv[0, hq] = 0
+    qn, kn = (rng.uniform(0.8, 1.2, 128).astype(np.float32) for _ in range(2))
+    rope = np.asarray(oracle.rope_table(max_pos), np.float32).reshape(max_pos, 64, 2)
+    bt = _table(rng, [max_pos], n_pages)
+    pos = rng.permutation(max_pos)[:M].astype(np.int32)
+    slot = np.zeros(M, np.int32)
+    pos[1], slot[1] = -1, 10 ** 6                                 # padding
+    pos[2], pos[3] = -9, max_pos                                  # bad
+    slot[4] = -1                                                  # bad: appends nothing
+    pool = _garbage_pool(rng, 1, n_pages, hkv)
+    d_pool, d_err = dev(torch, pool), _err(torch)
+    q_out = torch.full((M, hq, 128), 7.0, device="cuda")
+    d = [dev(torch, a) for a in (qkv, pos, slot, bt, qn, kn, rope)]
+    p = [x.data_ptr() for x in d]
+    fa_dec.op_qknorm_rope_append_kv8(p[0], M, hq, hkv, p[1], p[2], p[3], bt.shape[1], n_pages, p[4], p[5], 1e-5, p[6],
+                                     max_pos, fmt, d_pool.data_ptr(), q_out.data_ptr(), d_err.data_ptr(),
+                                     _stream(torch))
+    rot = rope[np.clip(pos, 0, max_pos - 1)]
+    q = P.norm_rotate(qkv[:, :hq], qn, rot) * np.float32(1 / np.sqrt(np.float32(128)))
+    q[1:4] = 7
+    got_q, rest = q_out.cpu().numpy(), np.r_[0:4, 5:M]
+    assert np.array_equal(got_q[rest], q[rest])
+    want = np.where(slot < 0, -1, np.where(pos < max_pos, pos, -1))
+    k = P.norm_rotate_exact(qkv[:, hq:hq + hkv], kn, rot)
+    P.write(pool, bt, np.zeros(M, np.int32), want, k[:, None], qkv[:, hq + hkv:][:, None], fmt)
+    (raw, d), (raw_w, d_w) = P.parts(d_pool.cpu().numpy()), P.parts(pool)
+    assert np.array_equal(raw, raw_w)
+    assert np.array_equal(d[..., 1, :].view(np.uint32), d_w[..., 1, :].view(np.uint32))
+    live = np.isfinite(d_w[..., 0, :])
+    assert np.array_equal(live, np.isfinite(d[..., 0, :]))
+    off = np.abs(d[..., 0, :][live].astype(np.float64) - d_w[..., 0, :][live])
+    assert (off <= np.abs(d_w[..., 0, :][live]) * (2.0 ** -20 if fmt == P.INT8 else 0)).all()
+    assert int(d_err) == 4
+
+
+@pytest.mark.parametrize("step", [0.0, 0.002, -0.002, 0.05, -0.05])
+@pytest.mark.parametrize("blocks", [(33, 70), (64, 65)])
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+def test_prefill_attention_many_tiles_over_long_contexts(torch_cuda, fmt, blocks, step):
+    """Calls of enough tiles that no context is cut into parts, over more than 32 blocks of 64 keys
+    (whose products are joined 32 blocks at a time, the last time one, six or 32 of them), with
+    scores that stay, rise or fall along the context."""
+    torch = torch_cuda
+    rng = np.random.default_rng(blocks[0])
+    hq, hkv, per = 16, 8, 3
+    lens = [64 * b for b in blocks]
+    pool, bt, n_pages = _filled(rng, lens, 1, hkv, fmt)
+    q = rng.standard_normal((10 * per, hq, 128)) * 0.3
+    if step:
+        raw, scales = P.parts(pool)
+        way = rng.choice([-1.0, 1.0], 128)
+        q = way + 0.01 * q
+        for i, n in enumerate(lens):
+            t = np.arange(n)
+            k = way * (step * t / 128)[:, None] + 0.02 * rng.standard_normal((hkv, n, 128))
+            qk, dk = P.quantise(k.astype(np.float32), fmt)
+            raw[0, bt[i, t // 16], :, 0, t % 16] = qk.transpose(1, 0, 2)
+            scales[0, bt[i, t // 16], :, 0, t % 16] = dk.T
+    q = q.astype(np.float32)
+    slot = np.repeat(np.arange(10) % 2, per).astype(np.int32)     # ten tiles of three rows
+    pos = np.array([lens[s] - per + m % per for m, s in enumerate(slot)], np.int32)
+    tiles = _tiles([(per * i, per) for i in range(10)], 64)
+    assert fa_dec.op_prefill_attention_kv8_scratch_bytes(len(tiles), hq, hkv) == 0
+    err = _err(torch)
+    got = _prefill(torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, slot), dev(torch, bt), n_pages, fmt,
+                   dev(torch, pool), tiles, err).cpu().numpy()
+    assert int(err) == 0
+    for m in range(len(pos)):
+        k, v = (x[0] for x in P.read(pool, bt[slot[m]], 0, pos[m] + 1, fmt))
+        want = P.attention(q[m], k, v).reshape(-1)
+        assert np.abs(got[m] - want).max() <= _bound(q[m], k, v), m
+        if abs(step) < 0.05:
+            assert rel_rms(got[m], want) <= 5e-6, m
+
+
+@pytest.mark.parametrize("fmt", FORMATS, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,M,pages", [
+    (16, 8, 1, 32), (16, 8, 9, 64), (16, 8, 9, 65), (16, 8, 18, 64), (16, 8, 19, 20), (16, 8, 55, 9), (16, 8, 56, 9),
+    (32, 4, 30, 12), (32, 4, 50, 12), (7, 1, 100, 3), (16, 8, 700, 8), (64, 64, 9, 57), (8, 2, 1500, 4),
+    (200, 200, 3, 10)])
+def test_decode_attention_counts_every_token(torch_cuda, fmt, hq, hkv, M, pages):
+    """Each way of cutting a call into work, at an accuracy that a token lost or taken twice
+    exceeds: one of 1024 tokens moves a row by some 1e-3 of itself."""
+    torch = torch_cuda
+    rng = np.random.default_rng(100 * pages + M)
+    lens = rng.integers(1, 16 * pages + 1, min(M, 24))
+    lens[0] = 16 * pages
+    pool, bt, n_pages = _filled(rng, lens.tolist(), 1, hkv, fmt)
+    slot = (np.arange(M) % len(lens)).astype(np.int32)
+    pos = (lens[slot] - 1).astype(np.int32)
+    q = (rng.standard_normal((M, hq, 128)) * 0.3).astype(np.float32)
+    err = _err(torch)
+    got = _decode(torch, dev(torch, q), hq, hkv, dev(torch, pos), dev(torch, slot), dev(torch, bt), n_pages, fmt,
+                  dev(torch, pool), err).cpu().numpy()
+    assert int(err) == 0
+    for m in np.unique(np.r_[np.arange(0, M, max(1, M // 24)), M - 1]):
+        k, v = (x[0] for x in P.read(pool, bt[slot[m]], 0, pos[m] + 1, fmt))
+        assert rel_rms(got[m], P.attention(q[m], k, v).reshape(-1)) <= 5e-6, (m, pos[m])
