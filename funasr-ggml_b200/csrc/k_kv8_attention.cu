@@ -761,10 +761,10 @@ cudaError_t launch_decode(const CUtensorMap& tm, const Kv8AttnArgs& a, void* scr
             <<<(int)items, kWarps * 32, sizeof(DecodeSmem<NT, kWarps>), s>>>(tm, a, scratch);
         return cudaGetLastError();
     }
-    const int grid = (int)std::min<long long>(items * a.bt_stride, kMaxCtas);   // no more CTAs than there can be pages
+    // no more CTAs than there can be pages (33 at least: fewer are a CTA per item)
+    const int grid = (int)std::min<long long>(items * a.bt_stride, kMaxCtas);
     kv8_decode_kernel<FMT, NT, kWarps, false>
         <<<grid, kWarps * 32, sizeof(DecodeSmem<NT, kWarps>), s>>>(tm, a, scratch);
-    if (grid == 1) return cudaGetLastError();
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     // launched while the decode kernel runs; it waits for that kernel's end before it reads
