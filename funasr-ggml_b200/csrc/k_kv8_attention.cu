@@ -71,7 +71,7 @@ namespace {
 // The page's product starts from zero and is added to the running output by one f32 fma per
 // value, so the sum over pages is rounded to nearest.
 //
-// Bound: HBM. 128 rows of 2048 tokens (16 heads on 8, 554 MB of tiles) take 95-98 us: 84 us of
+// Bound: HBM. 128 rows of 2048 tokens (16 heads on 8, 554 MB of tiles) take 96-99 us: 84 us of
 // pages at the rate of a copy, then some 5 us each of start (lengths, split, page look-ups: four
 // dependent loads) and of merge; without its arithmetic the kernel takes as long. 12 or 6 warps a
 // CTA took 98.6 and 98.9 us, grids of two to four waves 102 to 109, the merge inside the kernel
@@ -85,17 +85,18 @@ constexpr int kMaxCtas = 148 * kCtasPerSm;     // one resident wave of a B200
 constexpr int kItemUnits = 2;                  // with ranges per warp: 16 ragged rows 25.6 -> 12.8 us
 
 constexpr float kLazy = 8.0f;                  // weights reach 2^(6 + kLazy)
-constexpr int kStages = 3;                     // 128 rows x 2048 tokens: 2 stages 97, 3 95, 4 98 us
+constexpr int kStages = 3;                     // 128 rows x 2048 tokens: 2 stages 93, 3 96, 4 101 us
 
 // Short contexts: a CTA per (row, KV head), whose warps share its pages evenly, needs no list and
 // no merge kernel. It is taken while those CTAs are one resident wave and the block table bounds
 // the context to so many pages that the uneven rows and idle SMs cost less than they save (us, int8,
 // 16 heads on 8, list / CTA per item):
-//   1 row of 64 tokens 7.9 / 4.4, 256 7.9 / 6.5, 512 8.8 / 8.2, 1024 9.2 / 11.7
-//   16 rows of 256 9.9 / 6.8, 512 11.7 / 8.6, 1024 15.8 / 13.0, 1 to 1024 11.8 / 11.6
-//   55 rows of 256 14.9 / 9.9, 1024 30.1 / 24.8, 1 to 1024 22.3 / 21.7, 1 to 2048 31.9 / 36.3
-//   128 rows (more than a wave) of 256 23.9 / 24.9, 1024 54.8 / 58.7
-// Up to an item an SM it has eight warps (4 rows of 512: 8.2 us, with four 9.3, with twelve 8.5).
+//   1 row of 64 tokens 7.9 / 4.5, 256 8.0 / 6.1, 512 8.9 / 7.8, 1024 9.2 / 11.2
+//   16 rows of 256 9.8 / 6.7, 512 11.4 / 8.4, 1024 15.0 / 12.8, 1 to 1024 11.6 / 11.1
+//   55 rows of 256 14.2 / 9.2, 1024 29.0 / 24.3, 1 to 1024 21.9 / 20.5, 1 to 2048 31.7 / 34.4
+//   128 rows (more than a wave) of 256 23.3 / 24.1, 1024 54.1 / 58.6
+// The host sees the table's width alone: short rows of a wide table take the list.
+// Up to an item an SM it has eight warps (4 rows of 512: 7.8 us, with four 8.8, with twelve 8.0).
 constexpr int kItemWarps = 8;
 bool cta_per_item(long long items, int bt_stride) {
     return items <= kMaxCtas && bt_stride <= (items > 64 ? 64 : 32);

@@ -266,8 +266,9 @@ __device__ __noinline__ uint32_t exact_key(const float* vec, int lane, const flo
 // sums of squares are reduced over the warp together: each exchange halves the vectors a lane
 // carries, and the norms' square root and division, and the scales and reciprocals, are computed
 // once, side by side.
-// Bound: issue (2.7 instructions a cycle) and HBM. 4096 rows of 32 vectors (111 MB) take 26.2 us,
-// 4.25 TB/s; 22.2 with keys rounded from their f32 values.
+// Bound: issue (2.6 instructions a cycle, 140 a vector) and HBM. 4096 rows of 32 vectors (111 MB)
+// take 27.1 us, 4.1 TB/s; 26.5 without the checks of the keys' range, 22.2 with keys rounded from
+// their f32 values.
 template <int FMT, int V>
 __global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
     static_assert(V == 1 || V == 4, "the exchanges below");
@@ -341,9 +342,9 @@ __global__ void __launch_bounds__(kQkvWarps * 32) kv8_qkv_kernel(Kv8QkvArgs a) {
     const float d_mine = scale_of<FMT>(top), inv_mine = __frcp_rn(d_mine);
     const float amax_mine = __uint_as_float(top), e_mine = amax_mine * kKeyError<FMT>;
     // keys out of range, and e4m3 scales that the error of the largest value may change
-    const uint32_t unsure = __ballot_sync(
-        0xffffffffu, !key_in_range(amax_mine) || (FMT != kInt8 && scale_of<FMT>(__float_as_uint(amax_mine + e_mine)) !=
-                                                                      scale_of<FMT>(__float_as_uint(amax_mine - e_mine))));
+    const bool other_scale = FMT != kInt8 && scale_of<FMT>(__float_as_uint(amax_mine + e_mine)) !=
+                                                 scale_of<FMT>(__float_as_uint(amax_mine - e_mine));
+    const uint32_t unsure = __ballot_sync(0xffffffffu, !key_in_range(amax_mine) || other_scale);
     const float w_max = fmaxf(fmaxf(fabsf(kw[0]), fabsf(kw[1])), fmaxf(fabsf(kw[2]), fabsf(kw[3])));   // the lane's
     const int t = pos % kPageTokens;
 #pragma unroll
@@ -482,7 +483,9 @@ int launched(const char* what) {
 }
 
 // Whether a warp takes several vectors: once the warps of one vector each would fill the GPU
-// (148 SMs x 64 warps); below that more warps shorten the call.
+// (148 SMs x 64 warps); below that more warps shorten the call. One / four a warp (us): append, f16,
+// 4800 pairs 2.8 / 3.2, 9600 4.1 / 4.1, 19200 6.4 / 5.7, 76800 22.9 / 18.7; kernel (1), 4736 vectors
+// 4.2 / 5.3, 9472 5.2 / 5.9, 14208 6.5 / 6.2, 131072 42.2 / 27.0.
 bool several_per_warp(long long vectors) { return vectors > 148 * 64; }
 
 template <int FMT, typename T>

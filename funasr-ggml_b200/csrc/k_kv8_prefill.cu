@@ -15,10 +15,11 @@
 // an output is off by 2^-27 a key, as they fall together much less, of the largest |V| that its
 // row attends to (and of nothing that it does not attend to).
 // w and Q's high parts, the A operands of three quarters of the MMAs, are in TMEM: with all of Q
-// and w in shared memory a block would read 128 KB of it for its MMAs, against 1024 cycles that
-// they take. The running maximum is lazy: O is rescaled when a block exceeds it by 2^kLazy or
-// sigma grows. qs is a power of two so that qs m is exact: rounded by itself, the maximum of scores
-// of 1e8 and more would lie several log2 units from the scores that it is taken off.
+// and w in shared memory a block would read 160 KB of it for its MMAs (1280 cycles at 128 bytes a
+// cycle, 768 as it is), against 1024 cycles that they take. The running maximum is lazy: O is
+// rescaled when a block exceeds it by 2^kLazy or sigma grows. qs is a power of two so that qs m is
+// exact: rounded by itself, the maximum of scores of 1e8 and more would lie several log2 units from
+// the scores that it is taken off.
 //
 // Roles (512 threads): warp 0 issues the page copies (one TMA box and one bulk copy of scales
 // per page) into a ring of raw blocks; warps 4-7 expand a raw block into the f16 K / V tiles of
@@ -33,7 +34,8 @@
 // for. 4 chunks of 417 to 512 rows at 3500 tokens (16 query heads on 8, 248 CTAs of one SM each)
 // take 119 us; 300 with one softmax group, 174 with two S buffers, 142 to 155 with masked and
 // whole blocks in one pass, 146 with each block halved between the groups (ten rescales a warp,
-// each on the way of the next product). A chunk of 112 rows takes 13.3 us.
+// each on the way of the next product). A chunk of 112 rows takes 13.7 us; one chunk of 512 rows
+// (64 CTAs, two parts each) 43 us at 3500 tokens and 129 at 16000.
 // A persistent form with an even split of the blocks took 160 and 26: every change of tile costs
 // 10 us of queries, joins and output, which separate CTAs overlap.
 #include "k_attn_body.cuh"
@@ -58,7 +60,12 @@ static_assert(kRegsIssue + kRegsExpand + 2 * kRegsSoftmax <= 4 * 128, "registers
 // with their length (2.0e-6 of the output over 57 blocks, 1.2e-6 with stretches of 32); stretches
 // are joined in f32 arithmetic rounded to nearest, which costs 1 %.
 constexpr int STRETCH = 32;
-constexpr int kMaxParts = 16;                 // key ranges of one tile and head
+// Key ranges of one tile and head, and blocks of a range at least: more ranges spread a long context
+// over more SMs, and each costs a start and a share of the join. 64 rows on 8 KV heads at 16000 / 40000
+// keys with up to 8, 16, 32 ranges: 40 / 82, 30 / 52, 29 / 48 us; at 512 / 1024 / 3500 / 16000 keys
+// with 4, 8, 16 blocks at least: 16.4 / 16.8 / 19.8 / 30.3, 18.4 / 19.8 / 20.9 / 30.2,
+// 18.5 / 25.0 / 28.1 / 30.8 us.
+constexpr int kMaxParts = 16;
 constexpr int kMinPartBlocks = 8;
 // TMEM columns: S / w of block j at 64 (j % 3), O of the even blocks [192, 320) and of the odd
 // ones [320, 448), Q hi [448, 512)

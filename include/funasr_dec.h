@@ -402,7 +402,8 @@ FA_API int fa_op_q8p_gemm_argmax(const uint16_t* a16_dev, const uint16_t* a16_lo
  * head_dim 128. A row with pos -1 is padding (its slot is not looked at): it appends nothing,
  * its q_out row is left as it was, and its attention output is zero. All of these calls can
  * be captured into a CUDA graph; positions, lengths and block tables are read on the device
- * when it runs. */
+ * when it runs. Error bit 1 means that a bounded wait in an attention kernel gave up: that
+ * call's outputs are not valid. */
 #define FA_KV8_INT8 0
 #define FA_KV8_E4M3 1
 FA_API size_t fa_op_kv8_page_bytes(int n_kv_heads); /* one page of one layer; 0 for n_kv_heads <= 0 */
@@ -428,8 +429,8 @@ FA_API int fa_op_qknorm_rope_append_kv8(const float* qkv_dev, int M, int n_heads
                                         const float* rope_dev, int max_pos, int format, void* pool_layer_dev,
                                         float* q_out_dev, int* err_dev, void* stream);
 /* Reading the pool back (fa_op_kv_gather's 8-bit form): tokens [t0[m], t0[m] + n_tok[m]) of
- * sequence slot[m] (t0_dev NULL: from 0), in every layer, as d * q rounded once to out_type,
- * into k_out / v_out [n_layers][n_kv_heads][total_rows][128] at rows [row0[m], row0[m] +
+ * sequence slot[m] (t0_dev NULL: from 0), in every layer, as the f32 product d * q rounded to
+ * out_type (for f32 and for e4m3 that is one rounding of the stored value), into k_out / v_out [n_layers][n_kv_heads][total_rows][128] at rows [row0[m], row0[m] +
  * n_tok[m]) of each head plane; other rows are left as they are. n_tok[m] is 0 to max_tokens.
  * Bad lengths or row ranges set error bit 8, bad pages bit 2; those tokens are not written. */
 FA_API int fa_op_kv8_gather(const void* pool_dev, int format, int n_layers, int n_pages, int n_kv_heads,
@@ -443,7 +444,10 @@ FA_API int fa_op_kv8_gather(const void* pool_dev, int format, int n_layers, int 
  * aligned, of any content; calls that overlap on the GPU (captured graphs that run at the same
  * time among them) need scratch of their own. A position below -1 or past the block-table row
  * or a negative slot sets error bit 8 and that row is not written; a page outside the pool sets
- * bit 2 and its tokens are left out. bt_stride is limited to 2^26 pages. Sums are f32; an error
+ * bit 2 and its tokens are left out. bt_stride is limited to 2^26 pages. It also bounds the
+ * rows' lengths: up to 444 (row, KV head)s over tables of up to 32 pages (64 above 64 of them)
+ * take one launch and no join, 2 to 4 us less for rows of up to 512 tokens; wider tables do
+ * not, however short the rows are. Sums are f32; an error
  * is relative to the largest |V| that the row attends to (some 2^-20 of it). A score is off by
  * some 2^-22 of its sum of |q k|: that much, where scores are large, is the difference between
  * two tokens. Scores, 2^8 times the largest |K| and 2^11 times the largest |V| times the row's
