@@ -34,7 +34,7 @@
 // for. 4 chunks of 417 to 512 rows at 3500 tokens (16 query heads on 8, 248 CTAs of one SM each)
 // take 119 us; 300 with one softmax group, 174 with two S buffers, 142 to 155 with masked and
 // whole blocks in one pass, 146 with each block halved between the groups (ten rescales a warp,
-// each on the way of the next product). A chunk of 112 rows takes 13.7 us; one chunk of 512 rows
+// each on the way of the next product). A chunk of 112 rows takes 13.5 to 13.8 us; one chunk of 512 rows
 // (64 CTAs, two parts each) 43 us at 3500 tokens and 129 at 16000.
 // A persistent form with an even split of the blocks took 160 and 26: every change of tile costs
 // 10 us of queries, joins and output, which separate CTAs overlap.
